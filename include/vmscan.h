@@ -408,6 +408,93 @@ int vmscan_gemm_tf32x3(int64_t M, int64_t N, int64_t K,
                        vmscan_stream_t stream);
 
 /*
+ * Serving: the scan and the conv over a cache of request states, for packed
+ * prompts and single tokens, and low-rank adapters beside a shared projection
+ * (no counterparts in the reference, which runs whole sequences from a zero
+ * state).  Rows of all requests lie one after the other; every sequence
+ * tensor is a (rows, columns) array with unit column stride and an element
+ * row stride `ld*` (any alignment; rows that are only read may repeat with
+ * stride 0).  bf16 != 0: the sequence tensors are bf16, all arithmetic and
+ * the scan's state stay fp32.
+ *
+ * A request reads its state from slot `source` (-1: zeros, a fresh prompt)
+ * and leaves it in slot `slot` (-1: a padding request: its rows come out as
+ * zeros and no state is touched).  A slot that one request writes must not be
+ * written by another request of the call nor be read by another one; the
+ * caller checks that (mlx_vision_mamba_b200.RequestBatch does).  Slots outside
+ * [0, n_slots) are treated as -1, so no table can reach outside the cache.
+ *
+ * vmscan_request_pieces (host only) cuts requests into pieces of at most
+ * max_rows rows (0: one piece per request): it writes n records of 8 int32
+ * {t0, t1, begin, end, source, slot, carry row, 0 / 1} followed by n_chains
+ * records of 4 int32 {first carry row, pieces, source, 0} into `pieces`
+ * (capacity in int32) and {n_carry, n_chains, carry_rows} into info[3], and
+ * returns n; with pieces == NULL it only counts.  by_length != 0 orders the
+ * pieces for vmscan_cached_scan (pieces with a carry first, then long ones
+ * first); 0 keeps row order (vmscan_cached_conv1d_silu).  Negative on a bad
+ * argument.
+ *
+ * vmscan_cached_scan_rows (host only) gives max_rows for vmscan_cached_scan on
+ * the current device: 0 when one warp per request and 32 channels keeps the
+ * GPU busy, else the rows a piece should have.
+ */
+int64_t vmscan_request_pieces(int64_t count, const int32_t* lengths, const int32_t* slots, const int32_t* sources,
+                              int64_t max_rows, int by_length, int32_t* pieces, int64_t capacity, int64_t* info);
+int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d_inner);
+int64_t vmscan_cached_scan_workspace_bytes(int64_t d_inner, int64_t carry_rows);
+
+/*
+ * y = (selective_scan of every request from its source state) * silu(z)
+ * (z == NULL: no gate), and the final states into `state` (n_slots, d_inner,
+ * 16) fp32.  Formulas as vmscan_fwd.  pieces / chains: device copies of
+ * vmscan_request_pieces' records.
+ */
+int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
+                       const void* delta, int64_t lddelta, const float* A, const void* B, int64_t ldB, const void* C,
+                       int64_t ldC, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
+                       int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
+                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* workspace,
+                       size_t workspace_bytes, vmscan_stream_t stream);
+
+/*
+ * The same for single tokens: row i is request i, with slots[i] and
+ * sources[i] (device).
+ */
+int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
+                       const void* delta, int64_t lddelta, const float* A, const void* B, int64_t ldB, const void* C,
+                       int64_t ldC, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
+                       int64_t n_slots, const int32_t* slots, const int32_t* sources, vmscan_stream_t stream);
+
+/*
+ * out = silu(bias + causal depthwise conv1d) of every request, the rows before
+ * its first one taken from the K - 1 rows of its source slot, and its last
+ * K - 1 rows into its slot of `state` (n_slots, K - 1, channels), oldest row
+ * first, in the type of x (an exact copy).  weight (channels, K, 1), K in
+ * 1..8.  pieces: of at most vmscan_cached_conv_rows() rows, in row order.
+ */
+int vmscan_cached_conv_rows(void);
+int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int bf16, const void* x, int64_t ldx,
+                              const float* weight, const float* bias, void* out, int64_t ldo, void* state,
+                              int64_t n_slots, const int32_t* pieces, int64_t n_pieces, vmscan_stream_t stream);
+
+/*
+ * out_t = base_t + scale[a] (x_t A_a^T) B_a^T with a the adapter of row t's
+ * request (-1: out_t = base_t); A (adapters, rank, d_in) and B (adapters,
+ * d_out, rank) in the type of x, rank in 1..128, products and the rank-wide
+ * values in fp32.  out may be base.  vmscan_lora_tiles (host only) sorts the
+ * rows by adapter into row_index (one int32 per row) and cuts them into tiles
+ * of 4 int32; it returns the number of tiles that any assignment of adapters
+ * to these lengths can need, and fills them all (with row_index or tiles NULL
+ * it only counts).
+ */
+int64_t vmscan_lora_tiles(int64_t count, const int32_t* lengths, const int32_t* adapters, int64_t n_adapters,
+                          int32_t* row_index, int32_t* tiles, int64_t tile_capacity);
+int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int64_t n_adapters, int bf16,
+                    const void* x, int64_t ldx, const void* a, const void* b, const float* scale, const void* base,
+                    int64_t ldbase, void* out, int64_t ldout, const int32_t* row_index, int64_t n_index,
+                    const int32_t* tiles, int64_t n_tiles, vmscan_stream_t stream);
+
+/*
  * Host-only introspection (no CUDA call): writes the token index visited at
  * every scan step of `dir` into tokens[0..seqlen), computed the way the
  * kernels compute it.  mode 0 enumerates the TMA boxes (box coordinates +

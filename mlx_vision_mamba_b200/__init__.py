@@ -9,6 +9,7 @@ from .direction import BACKWARD, FORWARD, ScanDirection, directions_for
 from .mamba_block import (
     BidirectionalMambaBlock,
     MambaBlock,
+    MambaCache,
     MultiDirectionalMambaBlock,
     ResidualMambaBlock,
 )
@@ -22,11 +23,19 @@ from .scan import (
     selective_scan_metal_fused,
     selective_scan_metal_trainable,
 )
+from .serving import (
+    LoraAdapters,
+    RequestBatch,
+    conv1d_silu_cached_cuda,
+    lora_add_cuda,
+    selective_scan_cached_cuda,
+)
 from .vision_mamba import PatchEmbed, PatchEmbed3D, PatchEmbed4D, VisionMamba
 
 __version__ = "0.1.0"
 __all__ = [
     "MambaBlock",
+    "MambaCache",
     "ResidualMambaBlock",
     "BidirectionalMambaBlock",
     "MultiDirectionalMambaBlock",
@@ -46,4 +55,9 @@ __all__ = [
     "selective_scan_metal_fused",
     "conv1d_silu_cuda",
     "device_status",
+    "RequestBatch",
+    "LoraAdapters",
+    "selective_scan_cached_cuda",
+    "conv1d_silu_cached_cuda",
+    "lora_add_cuda",
 ]

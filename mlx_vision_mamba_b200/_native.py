@@ -124,6 +124,29 @@ SIGNATURES = {
         [_i64, _i64, _i64, _p, _p, _i64, ctypes.c_int, _p, _p, _i64, ctypes.c_int, _p, _i64, ctypes.c_int, _p, _i64,
          _p],
     ),
+    "vmscan_request_pieces": (_i64, [_i64, _p, _p, _p, _i64, ctypes.c_int, _p, _i64, _p]),
+    "vmscan_cached_scan_rows": (_i64, [_i64, _p, _i64]),
+    "vmscan_cached_scan_workspace_bytes": (_i64, [_i64, _i64]),
+    "vmscan_cached_scan": (
+        ctypes.c_int,
+        [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64,
+         _p, _i64, _i64, _p, _i64, _i64, _p, _sz, _p],
+    ),
+    "vmscan_cached_step": (
+        ctypes.c_int,
+        [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64,
+         _p, _p, _p],
+    ),
+    "vmscan_cached_conv_rows": (ctypes.c_int, []),
+    "vmscan_cached_conv1d_silu": (
+        ctypes.c_int,
+        [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p],
+    ),
+    "vmscan_lora_tiles": (_i64, [_i64, _p, _p, _i64, _p, _p, _i64]),
+    "vmscan_lora_add": (
+        ctypes.c_int,
+        [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
+    ),
     "vmscan_scan_order": (ctypes.c_int, [_i64, _D, ctypes.c_int, _p, _p]),
     "vmscan_device_status": (ctypes.c_int, [_p, ctypes.c_int]),
     "vmscan_wait_timeout_selftest": (ctypes.c_int, [ctypes.c_uint32, _p]),
@@ -158,6 +181,7 @@ TRACED = (
     "vmscan_fwd", "vmscan_bwd", "vmscan_fwd_bf16", "vmscan_bwd_bf16", "vmscan_bwd_noalloc", "vmscan_conv1d_silu_fwd", "vmscan_conv1d_silu_bwd",
     "vmscan_dt_softplus_fwd", "vmscan_dt_softplus_bwd", "vmscan_tf32_split", "vmscan_tf32_split_multi",
     "vmscan_gemm_tf32x3", "vmscan_sum_rows", "vmscan_layernorm_fwd", "vmscan_layernorm_bwd",
+    "vmscan_cached_scan", "vmscan_cached_step", "vmscan_cached_conv1d_silu", "vmscan_lora_add",
 )
 
 

@@ -12,15 +12,18 @@
 #include <cstdio>
 #include <algorithm>
 #include <mutex>
+#include <new>
 #include <type_traits>
 
 #include "../../include/vmscan.h"
 #include "vmscan_bwd.cuh"
+#include "vmscan_cached.cuh"
 #include "vmscan_common.cuh"
 #include "vmscan_conv.cuh"
 #include "vmscan_dt.cuh"
 #include "vmscan_fwd.cuh"
 #include "vmscan_gemm.cuh"
+#include "vmscan_lora.cuh"
 #include "vmscan_norm.cuh"
 
 using namespace vmscan;
@@ -1237,6 +1240,376 @@ int vmscan_device_status(vmscan_stream_t stream, int clear) {
     if (cudaMemcpyToSymbol(g_vmscan_status, &zero, sizeof(int)) != cudaSuccess) return VMSCAN_ERR_LAUNCH;
   }
   return v;
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---- cached scan / conv and adapters: host side ----
+
+// Read-only rows may repeat (stride 0) but not run backwards.
+int check_row_stride(const char* what, int64_t ld, int64_t rows) {
+  if (rows > 1 && ld < 0) return fail(VMSCAN_ERR_SHAPE, "%s row stride %lld is negative", what, (long long)ld);
+  return VMSCAN_OK;
+}
+
+int check_out_stride(const char* what, int64_t ld, int64_t cols, int64_t rows) {
+  if (rows > 1 && ld < cols)
+    return fail(VMSCAN_ERR_SHAPE, "%s row stride %lld is shorter than its %lld columns", what, (long long)ld,
+                (long long)cols);
+  return VMSCAN_OK;
+}
+
+int check_requests(int64_t count, const int32_t* lengths, const int32_t* slots, const int32_t* sources) {
+  if (count <= 0 || count > (int64_t(1) << 24)) return fail(VMSCAN_ERR_SHAPE, "%lld requests", (long long)count);
+  if (lengths == nullptr || slots == nullptr || sources == nullptr) return VMSCAN_ERR_NULL;
+  int64_t rows = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (lengths[i] < 0)
+      return fail(VMSCAN_ERR_SHAPE, "request %lld has %d rows", (long long)i, lengths[i]);
+    rows += lengths[i];
+  }
+  if (rows > (int64_t(1) << 30)) return fail(VMSCAN_ERR_SHAPE, "%lld rows", (long long)rows);
+  return VMSCAN_OK;
+}
+
+struct PieceRecord {
+  int32_t f[PF_COUNT];
+};
+
+// Pieces of a request of len rows: `count` pieces of `rows` rows (the last may
+// be shorter, none is empty but an empty request's only one).  even: equal
+// pieces, cut at multiples of 8 rows.
+struct PieceSplit {
+  int64_t count, rows;
+};
+
+PieceSplit split_request(int64_t len, int64_t max_rows, bool even) {
+  if (max_rows <= 0 || len <= max_rows) return {1, len};
+  int64_t rows = max_rows;
+  if (even) {
+    const int64_t k = (len + max_rows - 1) / max_rows;
+    rows = ((len + k - 1) / k + 7) / 8 * 8;
+  }
+  return {(len + rows - 1) / rows, rows};
+}
+
+int cached_scan_args(CachedScanArgs& a, int64_t rows, int64_t d_inner, int64_t d_state, const void* u, int64_t ldu,
+                     const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb, const void* C,
+                     int64_t ldc, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
+                     int64_t n_slots) {
+  VM_TRY(check_common(d_state, A, D));
+  if (rows < 0 || rows > (int64_t(1) << 30) || d_inner <= 0 || d_inner > (int64_t(1) << 24) || n_slots <= 0 ||
+      n_slots > INT32_MAX)
+    return fail(VMSCAN_ERR_SHAPE, "cached scan: rows %lld, d_inner %lld, slots %lld", (long long)rows,
+                (long long)d_inner, (long long)n_slots);
+  if (state == nullptr || (rows > 0 && (u == nullptr || delta == nullptr || B == nullptr || C == nullptr || y == nullptr)))
+    return VMSCAN_ERR_NULL;
+  if (!aligned16(A) || !aligned16(state)) return fail(VMSCAN_ERR_ALIGN, "A and state must be 16-byte aligned");
+  VM_TRY(check_row_stride("u", ldu, rows));
+  VM_TRY(check_row_stride("delta", ldd, rows));
+  VM_TRY(check_row_stride("B", ldb, rows));
+  VM_TRY(check_row_stride("C", ldc, rows));
+  if (z != nullptr) VM_TRY(check_row_stride("z", ldz, rows));
+  VM_TRY(check_out_stride("y", ldy, d_inner, rows));
+  a = CachedScanArgs{u, delta, B, C, z, y, A, D, state, ldu, ldd, ldb, ldc, ldz, ldy, n_slots, int(rows), int(d_inner)};
+  return VMSCAN_OK;
+}
+
+struct CachedScanPlan {
+  int groups;       // CTAs per piece
+  size_t carry, sums, total;
+};
+
+CachedScanPlan cached_scan_plan(int64_t d_inner, int64_t carry_rows) {
+  CachedScanPlan p;
+  p.groups = int((d_inner + CSC_WARPS * 32 - 1) / (CSC_WARPS * 32));
+  p.carry = align256(size_t(carry_rows) * d_inner * NS * 4);
+  p.sums = align256(size_t(carry_rows) * d_inner * 4);
+  p.total = carry_rows > 0 ? 2 * p.carry + p.sums : 0;
+  return p;
+}
+
+template <typename T>
+int launch_cached_scan(const CachedScanArgs& a, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
+                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* ws, cudaStream_t s) {
+  const CachedScanPlan p = cached_scan_plan(a.dn, carry_rows);
+  char* w = static_cast<char*>(ws);
+  float* carry_h = reinterpret_cast<float*>(w);
+  float* h_start = reinterpret_cast<float*>(w + p.carry);
+  float* carry_s = reinterpret_cast<float*>(w + 2 * p.carry);
+  if (n_chains > 0) {
+    cached_scan_kernel<T, false, true><<<unsigned(n_carry * p.groups), CSC_WARPS * 32, 0, s>>>(
+        a, pieces, p.groups, nullptr, carry_h, carry_s);
+    VM_TRY(check_launch());
+    cached_chain_kernel<<<dim3(unsigned((int64_t(a.dn) * NS + 127) / 128), unsigned(n_chains)), 128, 0, s>>>(
+        chains, a.A, a.state, a.n_slots, carry_h, carry_s, h_start, a.dn);
+    VM_TRY(check_launch());
+  }
+  const unsigned grid = unsigned(n_pieces * p.groups);
+  if (a.z != nullptr)
+    cached_scan_kernel<T, true, false><<<grid, CSC_WARPS * 32, 0, s>>>(a, pieces, p.groups, h_start, nullptr, nullptr);
+  else
+    cached_scan_kernel<T, false, false><<<grid, CSC_WARPS * 32, 0, s>>>(a, pieces, p.groups, h_start, nullptr, nullptr);
+  return check_launch();
+}
+
+template <typename T>
+int launch_cached_step(const CachedScanArgs& a, const int32_t* slots, const int32_t* sources, cudaStream_t s) {
+  const int groups = (a.dn + CST_WARPS * 32 - 1) / (CST_WARPS * 32);
+  const unsigned grid = unsigned(int64_t(a.rows) * groups);
+  if (a.z != nullptr)
+    cached_step_kernel<T, true><<<grid, CST_WARPS * 32, 0, s>>>(a, slots, sources, groups);
+  else
+    cached_step_kernel<T, false><<<grid, CST_WARPS * 32, 0, s>>>(a, slots, sources, groups);
+  return check_launch();
+}
+
+template <typename T>
+int launch_cached_conv(const CachedConvArgs& a, const int32_t* pieces, int64_t n_pieces, cudaStream_t s) {
+  const size_t q = 4 * sizeof(T);  // bytes of a four-channel access
+  const auto fits = [&](const void* p, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % q == 0 && (ld * int64_t(sizeof(T))) % int64_t(q) == 0;
+  };
+  const bool wide = a.channels % 4 == 0 && fits(a.x, a.ldx) && fits(a.out, a.ldo) && fits(a.state, a.channels);
+  const int groups = (a.channels + CCV_THREADS * (wide ? 4 : 1) - 1) / (CCV_THREADS * (wide ? 4 : 1));
+  if (n_pieces * groups > INT32_MAX) return fail(VMSCAN_ERR_SHAPE, "cached conv: %lld pieces", (long long)n_pieces);
+  const unsigned grid = unsigned(n_pieces * groups);
+  if (wide)
+    cached_conv_kernel<T, 4><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+  else
+    cached_conv_kernel<T, 1><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+  return check_launch();
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d_inner) {
+  if (count <= 0 || lengths == nullptr || d_inner <= 0) return -VMSCAN_ERR_SHAPE;
+  int64_t total = 0, longest = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    total += lengths[i];
+    longest = std::max<int64_t>(longest, lengths[i]);
+  }
+  // rows a warp would scan if the work were spread evenly over 16 warps an SM
+  const int64_t warps = (d_inner + 31) / 32;
+  const int64_t even = total * warps / (int64_t(sm_count()) * 16) + 1;
+  if (longest <= 2 * even + 64) return 0;
+  return std::max<int64_t>(even, 64);
+}
+
+int64_t vmscan_request_pieces(int64_t count, const int32_t* lengths, const int32_t* slots, const int32_t* sources,
+                              int64_t max_rows, int by_length, int32_t* pieces, int64_t capacity, int64_t* info) {
+  const int rc = check_requests(count, lengths, slots, sources);
+  if (rc != VMSCAN_OK) return -rc;
+  if (max_rows < 0 || info == nullptr) return -VMSCAN_ERR_SHAPE;
+  int64_t n = 0, n_carry = 0, n_chains = 0, carry_rows = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t k = split_request(lengths[i], max_rows, by_length != 0).count;
+    n += k;
+    if (k > 1) {
+      n_carry += k - 1;
+      n_chains += 1;
+      carry_rows += k;
+    }
+  }
+  if (n > INT32_MAX) return -VMSCAN_ERR_SHAPE;
+  info[0] = n_carry;
+  info[1] = n_chains;
+  info[2] = carry_rows;
+  if (pieces == nullptr) return n;
+  if (capacity < n * PF_COUNT + n_chains * 4) return -VMSCAN_ERR_WORKSPACE;
+  PieceRecord* out = reinterpret_cast<PieceRecord*>(pieces);
+  int32_t* chain = pieces + n * PF_COUNT;
+  int64_t at = 0, begin = 0, carry = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t len = lengths[i];
+    const PieceSplit sp = split_request(len, max_rows, by_length != 0);
+    const int64_t k = sp.count;
+    const int64_t source = slots[i] < 0 ? -1 : sources[i];
+    for (int64_t j = 0; j < k; ++j) {
+      PieceRecord r;
+      r.f[PF_T0] = int32_t(begin + j * sp.rows);
+      r.f[PF_T1] = int32_t(begin + (j + 1 < k ? (j + 1) * sp.rows : len));
+      r.f[PF_BEGIN] = int32_t(begin);
+      r.f[PF_END] = int32_t(begin + len);
+      r.f[PF_SOURCE] = int32_t(source);
+      r.f[PF_SLOT] = slots[i];
+      r.f[PF_CARRY] = k > 1 ? int32_t(carry + j) : -1;
+      r.f[PF_PAD] = k > 1 && j + 1 < k ? 1 : 0;
+      out[at++] = r;
+    }
+    if (k > 1) {
+      chain[0] = int32_t(carry);
+      chain[1] = int32_t(k);
+      chain[2] = int32_t(source);
+      chain[3] = 0;
+      chain += 4;
+      carry += k;
+    }
+    begin += len;
+  }
+  if (by_length)
+    std::sort(out, out + n, [](const PieceRecord& x, const PieceRecord& y) {
+      if (x.f[PF_PAD] != y.f[PF_PAD]) return x.f[PF_PAD] > y.f[PF_PAD];
+      const int32_t lx = x.f[PF_T1] - x.f[PF_T0], ly = y.f[PF_T1] - y.f[PF_T0];
+      if (lx != ly) return lx > ly;
+      if (x.f[PF_T0] != y.f[PF_T0]) return x.f[PF_T0] < y.f[PF_T0];
+      return x.f[PF_SLOT] < y.f[PF_SLOT];
+    });
+  return n;
+}
+
+int64_t vmscan_cached_scan_workspace_bytes(int64_t d_inner, int64_t carry_rows) {
+  if (d_inner <= 0 || d_inner > (int64_t(1) << 24) || carry_rows < 0 || carry_rows > (int64_t(1) << 30))
+    return -VMSCAN_ERR_SHAPE;
+  return int64_t(cached_scan_plan(d_inner, carry_rows).total);
+}
+
+int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
+                       const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb, const void* C,
+                       int64_t ldc, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
+                       int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
+                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* workspace,
+                       size_t workspace_bytes, vmscan_stream_t stream) {
+  CachedScanArgs a;
+  VM_TRY(cached_scan_args(a, rows, d_inner, d_state, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, y, ldy, state,
+                          n_slots));
+  if (pieces == nullptr || (n_chains > 0 && chains == nullptr)) return VMSCAN_ERR_NULL;
+  if (!aligned16(pieces) || !aligned16(chains)) return fail(VMSCAN_ERR_ALIGN, "pieces and chains must be 16-byte aligned");
+  const CachedScanPlan p = cached_scan_plan(d_inner, carry_rows);
+  if (n_pieces <= 0 || n_carry < 0 || n_carry > n_pieces || n_chains < 0 || n_chains > 65535 || carry_rows < 0 ||
+      (n_chains > 0) != (carry_rows > 0) || (n_chains > 0) != (n_carry > 0) || n_pieces * p.groups > INT32_MAX)
+    return fail(VMSCAN_ERR_SHAPE, "cached scan: %lld pieces (%lld with carries), %lld chains, %lld carry rows",
+                (long long)n_pieces, (long long)n_carry, (long long)n_chains, (long long)carry_rows);
+  if (p.total > 0 && (workspace == nullptr || workspace_bytes < p.total || !aligned16(workspace)))
+    return fail(VMSCAN_ERR_WORKSPACE, "cached scan: needs %zu bytes of 16-byte aligned workspace", p.total);
+  VM_TRY(ensure_context(state));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (bf16)
+    return launch_cached_scan<__nv_bfloat16>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
+  return launch_cached_scan<float>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
+}
+
+int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
+                       const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb, const void* C,
+                       int64_t ldc, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
+                       int64_t n_slots, const int32_t* slots, const int32_t* sources, vmscan_stream_t stream) {
+  CachedScanArgs a;
+  VM_TRY(cached_scan_args(a, rows, d_inner, d_state, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, y, ldy, state,
+                          n_slots));
+  if (slots == nullptr || sources == nullptr) return VMSCAN_ERR_NULL;
+  if (rows == 0 || rows * ((d_inner + CST_WARPS * 32 - 1) / (CST_WARPS * 32)) > INT32_MAX)
+    return fail(VMSCAN_ERR_SHAPE, "cached step: rows %lld, d_inner %lld", (long long)rows, (long long)d_inner);
+  VM_TRY(ensure_context(state));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return bf16 ? launch_cached_step<__nv_bfloat16>(a, slots, sources, s) : launch_cached_step<float>(a, slots, sources, s);
+}
+
+int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int bf16, const void* x, int64_t ldx,
+                              const float* weight, const float* bias, void* out, int64_t ldo, void* state,
+                              int64_t n_slots, const int32_t* pieces, int64_t n_pieces, vmscan_stream_t stream) {
+  if (ksize < 1 || ksize > CCV_KMAX) return VMSCAN_ERR_CONV;
+  if (rows < 0 || rows > (int64_t(1) << 30) || channels <= 0 || channels > (int64_t(1) << 24) || n_slots <= 0 ||
+      n_slots > INT32_MAX || n_pieces <= 0)
+    return fail(VMSCAN_ERR_SHAPE, "cached conv: rows %lld, channels %lld, slots %lld, pieces %lld", (long long)rows,
+                (long long)channels, (long long)n_slots, (long long)n_pieces);
+  if (weight == nullptr || bias == nullptr || pieces == nullptr || (ksize > 1 && state == nullptr) ||
+      (rows > 0 && (x == nullptr || out == nullptr)))
+    return VMSCAN_ERR_NULL;
+  if (!aligned16(pieces)) return fail(VMSCAN_ERR_ALIGN, "pieces must be 16-byte aligned");
+  VM_TRY(check_row_stride("x", ldx, rows));
+  VM_TRY(check_out_stride("out", ldo, channels, rows));
+  VM_TRY(ensure_context(pieces));
+  const CachedConvArgs a{x, out, state, weight, bias, ldx, ldo, n_slots, int(rows), int(channels), int(ksize)};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return bf16 ? launch_cached_conv<__nv_bfloat16>(a, pieces, n_pieces, s) : launch_cached_conv<float>(a, pieces, n_pieces, s);
+}
+
+int vmscan_cached_conv_rows(void) { return CCV_ROWS; }
+
+int64_t vmscan_lora_tiles(int64_t count, const int32_t* lengths, const int32_t* adapters, int64_t n_adapters,
+                          int32_t* row_index, int32_t* tiles, int64_t tile_capacity) {
+  const int rc = check_requests(count, lengths, adapters, adapters);
+  if (rc != VMSCAN_OK) return -rc;
+  if (n_adapters < 0 || n_adapters > INT32_MAX) return -VMSCAN_ERR_SHAPE;
+  int64_t most = 0;  // tiles when no two requests share an adapter
+  for (int64_t i = 0; i < count; ++i) {
+    if (adapters[i] < -1 || adapters[i] >= n_adapters) {
+      fail(VMSCAN_ERR_SHAPE, "request %lld has adapter %d of %lld", (long long)i, adapters[i], (long long)n_adapters);
+      return -VMSCAN_ERR_SHAPE;
+    }
+    most += (lengths[i] + LORA_ROWS - 1) / LORA_ROWS;
+  }
+  if (tiles == nullptr || row_index == nullptr) return most;
+  if (tile_capacity < most) return -VMSCAN_ERR_WORKSPACE;
+  // requests by adapter, then by position: {adapter, first row, rows}
+  struct Item {
+    int32_t adapter, begin, length;
+  };
+  Item* items = new (std::nothrow) Item[size_t(count)];
+  if (items == nullptr) return -VMSCAN_ERR_WORKSPACE;
+  int32_t begin = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    items[i] = {adapters[i], begin, lengths[i]};
+    begin += lengths[i];
+  }
+  std::sort(items, items + count, [](const Item& p, const Item& q) {
+    return p.adapter != q.adapter ? p.adapter < q.adapter
+                                  : (p.begin != q.begin ? p.begin < q.begin : p.length < q.length);
+  });
+  int64_t n = 0, at = 0;
+  for (int64_t i = 0; i < count;) {
+    const int32_t adapter = items[i].adapter;
+    int64_t first = at;
+    for (; i < count && items[i].adapter == adapter; ++i)
+      for (int32_t r = 0; r < items[i].length; ++r) row_index[at++] = items[i].begin + r;
+    for (; first < at; first += LORA_ROWS, ++n) {
+      tiles[4 * n] = int32_t(first);
+      tiles[4 * n + 1] = int32_t(std::min<int64_t>(LORA_ROWS, at - first));
+      tiles[4 * n + 2] = adapter;
+      tiles[4 * n + 3] = 0;
+    }
+  }
+  delete[] items;
+  for (; n < most; ++n)
+    for (int f = 0; f < 4; ++f) tiles[4 * n + f] = 0;
+  return most;
+}
+
+int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int64_t n_adapters, int bf16,
+                    const void* x, int64_t ldx, const void* a, const void* b, const float* scale, const void* base,
+                    int64_t ldbase, void* out, int64_t ldout, const int32_t* row_index, int64_t n_index,
+                    const int32_t* tiles, int64_t n_tiles, vmscan_stream_t stream) {
+  if (rows <= 0 || rows > (int64_t(1) << 30) || d_in <= 0 || d_in > (int64_t(1) << 24) || d_out <= 0 ||
+      d_out > (int64_t(1) << 24) || rank < 1 || rank > LORA_RMAX || n_adapters <= 0 || n_adapters > INT32_MAX ||
+      n_index < 0 || n_index > rows || n_tiles <= 0 || n_tiles > INT32_MAX)
+    return fail(VMSCAN_ERR_SHAPE, "lora: rows %lld, d_in %lld, d_out %lld, rank %lld (1..%d), adapters %lld, tiles %lld",
+                (long long)rows, (long long)d_in, (long long)d_out, (long long)rank, LORA_RMAX, (long long)n_adapters,
+                (long long)n_tiles);
+  if (x == nullptr || a == nullptr || b == nullptr || scale == nullptr || base == nullptr || out == nullptr ||
+      row_index == nullptr || tiles == nullptr)
+    return VMSCAN_ERR_NULL;
+  if (!aligned16(tiles)) return fail(VMSCAN_ERR_ALIGN, "lora: tiles must be 16-byte aligned");
+  VM_TRY(check_row_stride("x", ldx, rows));
+  VM_TRY(check_row_stride("base", ldbase, rows));
+  VM_TRY(check_out_stride("out", ldout, d_out, rows));
+  VM_TRY(ensure_context(out));
+  const LoraArgs l{x, a, b, base, out, scale, row_index, tiles, ldx, ldbase, ldout, int(rows), int(d_in), int(d_out),
+                   int(rank), int(n_adapters), int(n_index)};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  // enough column shares to give every SM a CTA
+  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>((d_out + 127) / 128, sm_count() * 2 / n_tiles));
+  const int cols = int((d_out + shares - 1) / shares);
+  const dim3 grid(unsigned(n_tiles), unsigned((d_out + cols - 1) / cols));
+  if (bf16)
+    lora_add_kernel<__nv_bfloat16><<<grid, LORA_THREADS, 0, s>>>(l, cols);
+  else
+    lora_add_kernel<float><<<grid, LORA_THREADS, 0, s>>>(l, cols);
+  return check_launch();
 }
 
 }  // extern "C"

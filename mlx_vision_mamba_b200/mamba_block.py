@@ -30,6 +30,13 @@ from .branches import block_core_forward, block_core_ok, branches_forward
 from .linear import linear_tc, supported as _tc_supported
 from .norm import layer_norm_cuda as _layer_norm_cuda, supported as _ln_supported
 from .scan import conv1d_silu_cuda, dt_softplus_cuda, selective_scan_cuda
+from .serving import (
+    LoraAdapters,
+    RequestBatch,
+    conv1d_silu_cached_cuda,
+    lora_add_cuda,
+    selective_scan_cached_cuda,
+)
 
 GPU_SCAN_MODES = ("cuda_fused", "metal_fused", "metal_train", "metal")
 CPU_SCAN_MODES = ("sequential", "chunked", "parallel")
@@ -81,6 +88,17 @@ class DepthwiseConv1d(nn.Module):
 
     def silu_along(self, x: torch.Tensor, direction: Optional[ScanDirection]) -> torch.Tensor:
         return conv1d_silu_cuda(x, self.weight, self.bias, direction)
+
+
+class MambaCache:
+    """What a MambaBlock keeps of each request between `serve` calls: the last
+    d_conv - 1 conv inputs, `conv` (slots, d_conv - 1, d_inner), and the
+    recurrent state, `ssm` (slots, d_inner, d_state), fp32, zeros at first."""
+
+    def __init__(self, block: "MambaBlock", slots: int):
+        like = dict(dtype=torch.float32, device=block.A_log.device)
+        self.conv = torch.zeros((slots, block.d_conv - 1, block.d_inner), **like)
+        self.ssm = torch.zeros((slots, block.d_inner, block.d_state), **like)
 
 
 class MambaBlock(nn.Module):
@@ -150,6 +168,45 @@ class MambaBlock(nn.Module):
         delta = dt_softplus_cuda(dt, self.dt_proj.weight, self.dt_proj.bias)
         A = -torch.exp(self.A_log)
         return selective_scan_cuda(x_branch, delta, A, B_proj, C_proj, self.D, z=z, direction=direction)
+
+    def new_cache(self, slots: int) -> MambaCache:
+        """A zeroed cache of `slots` request states for `serve`."""
+        return MambaCache(self, slots)
+
+    @torch.no_grad()
+    def serve(
+        self,
+        x: torch.Tensor,
+        cache: MambaCache,
+        batch: RequestBatch,
+        in_adapters: Optional[LoraAdapters] = None,
+        out_adapters: Optional[LoraAdapters] = None,
+    ) -> torch.Tensor:
+        """The causal block on packed rows of many requests: prompts of any
+        lengths and single new tokens in one call, each request from and to its
+        slot of `cache` (serving.RequestBatch).  x: (rows, d_model) CUDA fp32;
+        in_adapters / out_adapters: low-rank adapters of in_proj / out_proj,
+        chosen per request by the batch.  Returns (rows, d_model); no gradient.
+        Feeding a sequence in any pieces gives `forward`'s rows for it, up to
+        rounding (the reference has no incremental form)."""
+        if x.dim() != 2 or x.shape[1] != self.d_model or x.dtype != torch.float32:
+            raise ValueError(f"MambaBlock.serve: x must be (rows, {self.d_model}) fp32, got {tuple(x.shape)} {x.dtype}")
+        dn, r, n = self.d_inner, self.dt_rank, self.d_state
+        xz = project(x, self.in_proj.weight)
+        if in_adapters is not None:
+            lora_add_cuda(xz, x, in_adapters, batch, out=xz)
+        x_branch, z = xz[:, :dn], xz[:, dn:]
+        x_branch = conv1d_silu_cached_cuda(x_branch, self.conv1d.weight, self.conv1d.bias, cache.conv, batch)
+        x_dbc = project(x_branch, self.x_proj.weight)
+        delta = x_branch
+        if x.shape[0]:
+            delta = dt_softplus_cuda(x_dbc[None, :, :r], self.dt_proj.weight, self.dt_proj.bias)[0]
+        y = selective_scan_cached_cuda(x_branch, delta, -torch.exp(self.A_log), x_dbc[:, r:r + n], x_dbc[:, r + n:],
+                                       self.D, cache.ssm, batch, z=z)
+        out = project(y, self.out_proj.weight)
+        if out_adapters is not None:
+            lora_add_cuda(out, y, out_adapters, batch, out=out)
+        return out
 
 
 def project(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
@@ -240,6 +297,14 @@ class ResidualMambaBlock(nn.Module):
 
     def forward(self, x):
         return x + self.mamba(self.norm(x))
+
+    def new_cache(self, slots: int) -> MambaCache:
+        return self.mamba.new_cache(slots)
+
+    @torch.no_grad()
+    def serve(self, x, cache, batch, in_adapters=None, out_adapters=None):
+        """x + mamba.serve(norm(x)) on packed rows (MambaBlock.serve)."""
+        return x + self.mamba.serve(self.norm(x), cache, batch, in_adapters, out_adapters)
 
 
 class BidirectionalMambaBlock(nn.Module):

@@ -1,0 +1,197 @@
+"""Host side of the serving operators, without a GPU: the checks of
+RequestBatch and of the operators, and the tables that tell the kernels which
+rows, slots and adapters they work on."""
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_vision_mamba_b200 import (
+    LoraAdapters,
+    RequestBatch,
+    _native,
+    conv1d_silu_cached_cuda,
+    lora_add_cuda,
+    selective_scan_cached_cuda,
+)
+
+
+@pytest.mark.parametrize(
+    "kw",
+    [
+        dict(lengths=[]),
+        dict(lengths=[3, -1]),
+        dict(lengths=[1.5, 2.0]),
+        dict(lengths=[[1, 2]]),
+        dict(lengths=[1 << 30, 1]),
+        dict(lengths=[2, 2], slots=[0]),
+        dict(lengths=[2, 2], slots=[4, 4]),  # one slot written twice
+        dict(lengths=[2, 2], slots=[0, -2]),
+        dict(lengths=[2, 2], slots=[0, 1], sources=[1, 1]),  # reads a slot that the other writes
+        dict(lengths=[2, 2], slots=[0, 1], sources=[0, 0]),
+        dict(lengths=[0, 2], slots=[0, 1], sources=[0, 0]),
+        dict(lengths=[2, 2], slots=[0, 1], sources=[5]),
+        dict(lengths=[2, 2], adapters=[0]),
+        dict(lengths=[2, 2], adapters=[0, -2]),
+        dict(lengths=[2, 2], slots=[0, 1 << 31]),
+    ],
+)
+def test_bad_batches_are_refused(kw):
+    with pytest.raises(ValueError):
+        RequestBatch(**kw)
+
+
+def test_allowed_batches():
+    b = RequestBatch([2, 0, 5], slots=[3, -1, 4], sources=[7, 4, 7])  # a fork; a padding request reads nothing
+    assert b.tokens == 7 and b.count == 3 and b.max_slot == 7 and not b.single_tokens
+    assert b.sources.tolist() == [7, -1, 7]
+    assert RequestBatch([1, 1], slots=[-1, -1]).max_slot == -1
+    assert RequestBatch([1] * 5).single_tokens
+    assert RequestBatch(torch.tensor([4, 1])).sources.tolist() == [0, 1]
+    assert RequestBatch([1], sources=[-1]).sources.tolist() == [-1]
+
+
+def _pieces(batch, rows, by_length):
+    lib = _native.load()
+    info = np.zeros(3, dtype=np.int64)
+    p = lambda a: a.ctypes.data  # noqa: E731
+    args = (batch.count, p(batch.lengths), p(batch.slots), p(batch.sources), rows, by_length)
+    n = lib.vmscan_request_pieces(*args, None, 0, p(info))
+    table = np.full(8 * n + 4 * int(info[1]) + 8, 77, dtype=np.int32)
+    assert lib.vmscan_request_pieces(*args, p(table), 8 * n + 4 * int(info[1]), p(info)) == n
+    assert (table[8 * n + 4 * int(info[1]):] == 77).all()  # writes what it counted
+    assert lib.vmscan_request_pieces(*args, p(table), 8 * n + 4 * int(info[1]) - 1, p(info)) == -6
+    return table[:8 * n].reshape(n, 8), table[8 * n:8 * n + 4 * int(info[1])].reshape(-1, 4), info
+
+
+@pytest.mark.parametrize("by_length", [0, 1])
+@pytest.mark.parametrize("rows", [0, 1, 7, 8, 32, 64, 1000])
+@pytest.mark.parametrize("lengths", [[1], [0], [0, 0, 3], [65, 0, 1, 64, 63, 200], [1000], [8, 9, 7, 16, 17]])
+def test_pieces_cover_every_row_once(lengths, rows, by_length):
+    n = len(lengths)
+    slots = [i if i != 2 else -1 for i in range(n)]
+    batch = RequestBatch(lengths, slots=slots, sources=[(n + i) if i % 2 else -1 for i in range(n)])
+    pieces, chains, info = _pieces(batch, rows, by_length)
+    begins = np.concatenate([[0], np.cumsum(lengths)])
+    seen = np.zeros(int(begins[-1]), dtype=int)
+    owners = {}
+    for t0, t1, begin, end, source, slot, carry, later in pieces:
+        assert begin <= t0 <= t1 <= end
+        assert rows == 0 or t1 - t0 <= max(rows, (rows + 7) // 8 * 8 if by_length else rows)
+        seen[t0:t1] += 1
+        assert t1 > t0 or begin == end  # only an empty request has an empty piece
+        owners.setdefault((begin, end, slot), []).append((t0, t1, source, carry, later))
+    assert (seen == 1).all()
+    assert len(pieces) >= n
+    used = []
+    for i in range(n):
+        mine = sorted(owners[(begins[i], begins[i + 1], slots[i])])
+        assert mine[0][0] == begins[i] and mine[-1][1] == begins[i + 1]
+        assert all(m[2] == batch.sources[i] for m in mine)
+        if len(mine) == 1:
+            assert mine[0][3] == -1 and mine[0][4] == 0
+        else:
+            carries = [m[3] for m in mine]
+            assert carries == list(range(carries[0], carries[0] + len(mine)))
+            assert [m[4] for m in mine] == [1] * (len(mine) - 1) + [0]
+            assert [carries[0], len(mine), batch.sources[i], 0] in chains.tolist()
+            used += carries
+    assert sorted(used) == list(range(int(info[2]))) and len(chains) == info[1]
+    assert (pieces[:, 7] == 1).sum() == info[0]
+    if by_length:  # pieces with a carry first, then by length
+        assert (pieces[:int(info[0]), 7] == 1).all()
+        rest = (pieces[:, 1] - pieces[:, 0])[int(info[0]):]
+        assert (np.diff(rest) <= 0).all()
+    else:
+        assert (np.diff(pieces[:, 0]) >= 0).all()
+
+
+def test_scan_rows_rule():
+    """One long prompt is split, a full batch of even prompts is not."""
+    lib = _native.load()
+
+    def rows(lengths, dn):
+        a = np.asarray(lengths, np.int32)
+        return lib.vmscan_cached_scan_rows(a.size, a.ctypes.data, dn)
+
+    assert 0 < rows([32768], 768) < 8192
+    assert rows([512] * 256, 1536) == 0
+    assert rows([1] * 10, 64) == 0
+    assert lib.vmscan_cached_scan_rows(0, None, 64) == -2
+
+
+@pytest.mark.parametrize("lengths", [[1] * 40, [100, 0, 3, 17, 16, 1], [0, 0]])
+def test_lora_tiles(lengths):
+    lib = _native.load()
+    n = len(lengths)
+    rng = np.random.RandomState(n)
+    ads = rng.randint(-1, 3, n)
+    batch = RequestBatch(lengths, adapters=ads)
+    p = lambda a: a.ctypes.data  # noqa: E731
+    args = (n, p(batch.lengths), p(batch.adapters), 3)
+    most = lib.vmscan_lora_tiles(*args, None, None, 0)
+    index, tiles = np.full(batch.tokens + 4, -5, np.int32), np.full((most + 1, 4), -5, np.int32)
+    if most:
+        assert lib.vmscan_lora_tiles(*args, p(index), p(tiles), most) == most
+        assert lib.vmscan_lora_tiles(*args, p(index), p(tiles), most - 1) == -6
+    assert (index[batch.tokens:] == -5).all() and (tiles[most:] == -5).all()
+    assert sorted(index[:batch.tokens].tolist()) == list(range(batch.tokens))
+    of_row = np.repeat(ads, lengths)
+    covered = 0
+    for first, count, ad, _ in tiles[:most]:
+        assert (of_row[index[first:first + count]] == ad).all() or count == 0
+        covered += count
+    assert covered == batch.tokens
+    assert lib.vmscan_lora_tiles(n, p(batch.lengths), p(batch.adapters), 1, None, None, 0) == (-2 if ads.max() > 0 else most)
+
+
+def test_operators_refuse_cpu_tensors_and_wrong_batches():
+    b = RequestBatch([2], device="cpu")
+    x = torch.zeros(2, 4)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        selective_scan_cached_cuda(x, x, torch.zeros(4, 16), x, x, torch.zeros(4), torch.zeros(1, 4, 16), b)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        conv1d_silu_cached_cuda(x, torch.zeros(4, 4, 1), torch.zeros(4), torch.zeros(1, 3, 4), b)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        lora_add_cuda(x, x, None, b)
+    with pytest.raises(TypeError, match="RequestBatch"):
+        conv1d_silu_cached_cuda(x, torch.zeros(4, 4, 1), torch.zeros(4), torch.zeros(1, 3, 4), [2])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        LoraAdapters(torch.zeros(1, 2, 4), torch.zeros(1, 4, 2))
+
+
+def test_c_entry_points_validate():
+    """Every call here returns before any CUDA work."""
+    lib = _native.load()
+    P = 4096
+    scan = lambda **o: lib.vmscan_cached_scan(*[{**dict(  # noqa: E731
+        rows=4, dn=8, ds=16, bf16=0, u=P, ldu=8, dl=P, ldd=8, A=P, B=P, ldb=16, C=P, ldc=16, D=P, z=None, ldz=0, y=P,
+        ldy=8, state=P, slots=2, pieces=P, n=1, nc=0, chains=None, nch=0, cr=0, ws=None, wn=0, stream=None), **o}[k]
+        for k in ("rows dn ds bf16 u ldu dl ldd A B ldb C ldc D z ldz y ldy state slots pieces n nc chains nch cr ws wn "
+                  "stream").split()])
+    assert scan(ds=8) == 3
+    assert scan(A=None) == 1 and scan(u=None) == 1 and scan(state=None) == 1 and scan(pieces=None) == 1
+    assert scan(dn=0) == 2 and scan(rows=-1) == 2 and scan(slots=0) == 2 and scan(ldy=7) == 2 and scan(ldu=-8) == 2
+    assert scan(n=0) == 2 and scan(n=1, nc=2) == 2 and scan(cr=3) == 2
+    assert scan(A=P + 4) == 4 and scan(state=P + 8) == 4 and scan(pieces=P + 4) == 4
+    assert scan(n=4, nc=2, chains=P, nch=1, cr=3) == 6  # no workspace
+    need = lib.vmscan_cached_scan_workspace_bytes(8, 3)
+    assert need >= 3 * 8 * 33 * 4
+    assert scan(n=4, nc=2, chains=P, nch=1, cr=3, ws=P, wn=need - 1) == 6
+    assert lib.vmscan_cached_scan_workspace_bytes(0, 3) == -2
+    step = lambda **o: lib.vmscan_cached_step(*[{**dict(  # noqa: E731
+        rows=4, dn=8, ds=16, bf16=0, u=P, ldu=8, dl=P, ldd=8, A=P, B=P, ldb=16, C=P, ldc=16, D=P, z=None, ldz=0, y=P,
+        ldy=8, state=P, slots=2, slot=P, source=P, stream=None), **o}[k]
+        for k in "rows dn ds bf16 u ldu dl ldd A B ldb C ldc D z ldz y ldy state slots slot source stream".split()])
+    assert step(slot=None) == 1 and step(rows=0) == 2 and step(ds=4) == 3
+    conv = lambda **o: lib.vmscan_cached_conv1d_silu(*[{**dict(  # noqa: E731
+        rows=4, c=8, k=4, bf16=0, x=P, ldx=8, w=P, b=P, out=P, ldo=8, state=P, slots=2, pieces=P, n=1, stream=None),
+        **o}[k] for k in "rows c k bf16 x ldx w b out ldo state slots pieces n stream".split()])
+    assert conv(k=0) == 10 and conv(k=9) == 10 and conv(state=None) == 1 and conv(x=None) == 1 and conv(n=0) == 2
+    assert conv(ldo=4) == 2 and conv(c=0) == 2 and conv(pieces=P + 8) == 4
+    lora = lambda **o: lib.vmscan_lora_add(*[{**dict(  # noqa: E731
+        rows=4, di=8, do=8, r=4, ad=2, bf16=0, x=P, ldx=8, a=P, b=P, s=P, base=P, ldb=8, out=P, ldo=8, idx=P, ni=4,
+        tiles=P, nt=1, stream=None), **o}[k]
+        for k in "rows di do r ad bf16 x ldx a b s base ldb out ldo idx ni tiles nt stream".split()])
+    assert lora(r=0) == 2 and lora(r=129) == 2 and lora(rows=0) == 2 and lora(ni=5) == 2 and lora(nt=0) == 2
+    assert lora(x=None) == 1 and lora(s=None) == 1 and lora(tiles=P + 4) == 4 and lora(ldo=7) == 2

@@ -1,0 +1,476 @@
+"""Serving operators on the GPU against 64-bit references (serving_ref.py,
+whose bounds are derived there), at the lengths, slots, strides and sizes where
+they can go wrong, and MambaBlock.serve against the oracle's block."""
+
+import pytest
+import torch
+
+import serving_ref as ref
+from mlx_vision_mamba_b200 import (
+    LoraAdapters,
+    MambaBlock,
+    RequestBatch,
+    ResidualMambaBlock,
+    conv1d_silu_cached_cuda,
+    lora_add_cuda,
+    selective_scan_cached_cuda,
+)
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _scan_inputs(rows, dn, slots, dtype=F32, gate=True, seed=0, step=-3.0):
+    g = _gen(seed)
+    n = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    return dict(
+        x=n(rows, dn).to(dtype), delta=torch.nn.functional.softplus(0.5 * n(rows, dn) + step).to(dtype),
+        A=-torch.arange(1, 17, device="cuda") * torch.exp(0.1 * n(dn, 16)), B=n(rows, 16).to(dtype),
+        C=n(rows, 16).to(dtype), D=n(dn), state=0.3 * n(slots, dn, 16), z=n(rows, dn).to(dtype) if gate else None)
+
+
+def _scan_check(name, inp, batch):
+    want = ref.scan(batch=batch, **inp)
+    run = dict(inp, state=inp["state"].clone())
+    y = selective_scan_cached_cuda(batch=batch, **run)
+    again = inp["state"].clone()
+    y2 = selective_scan_cached_cuda(batch=batch, **dict(inp, state=again))
+    assert y.dtype == inp["x"].dtype and torch.equal(y, y2) and torch.equal(run["state"], again), f"{name}: not repeatable"
+    ref.check(f"{name} y", y, want[0], want[1])
+    ref.check(f"{name} state", run["state"], want[2], want[3])
+    return y, run["state"]
+
+
+def _mixed(lengths, **kw):
+    n = len(lengths)
+    return RequestBatch(lengths, slots=[n + (i * 7 + 3) % n for i in range(n)] if n % 7 else list(range(n, 2 * n)),
+                        sources=[-1 if i % 3 == 0 else i for i in range(n)], **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("dn", [1, 31, 64, 130])
+@pytest.mark.parametrize("lengths", [[1], [7], [8, 9, 1, 16], [0, 5, 33, 0, 1], [100]])
+def test_scan_prompts(lengths, dn, gate, dtype):
+    batch = _mixed(lengths)
+    _scan_check(f"scan {lengths} {dn}", _scan_inputs(batch.tokens, dn, 2 * len(lengths), dtype, gate, seed=dn), batch)
+
+
+@pytest.mark.parametrize("lengths,dn", [([1500], 40), ([2100, 3, 700], 33), ([0, 1200, 1], 260)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scan_split_prompts(lengths, dn, dtype):
+    """Prompts long enough to be scanned in several pieces, from and to the same slot and forked."""
+    n = len(lengths)
+    for batch in (RequestBatch(lengths), RequestBatch(lengths, slots=list(range(n, 2 * n)), sources=[0] * n)):
+        assert batch._build(("scan", dn))[1][2] > 0  # chains
+        _scan_check(f"scan {lengths} {dn}", _scan_inputs(batch.tokens, dn, 2 * n, dtype, seed=7), batch)
+
+
+def test_scan_long_memory():
+    """Small steps: the state at the end still holds the first rows'."""
+    batch = RequestBatch([1800], sources=[-1])
+    _scan_check("long memory", _scan_inputs(1800, 64, 1, seed=3, step=-8.0), batch)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dn", [1, 3, 32, 100, 771])
+@pytest.mark.parametrize("count", [1, 2, 37])
+def test_scan_tokens(count, dn, dtype):
+    slots = [count + i if i % 5 != 4 else -1 for i in range(count)]
+    sources = [-1 if i % 4 == 3 else i for i in range(count)]
+    batch = RequestBatch([1] * count, slots=slots, sources=sources)
+    assert batch.single_tokens
+    inp = _scan_inputs(count, dn, 2 * count, dtype, gate=dn != 100, seed=count)
+    y, _ = _scan_check(f"tokens {count} {dn}", inp, batch)
+    for i, s in enumerate(slots):
+        if s < 0:
+            assert (y[i] == 0).all()
+    _scan_check("in place", inp, RequestBatch([1] * count))
+
+
+def test_scan_single_tokens_equal_one_prompt_row_by_row():
+    """A prompt fed whole, in pieces and token by token ends in the same place."""
+    rows, dn = 41, 96
+    inp = _scan_inputs(rows, dn, 1, seed=5)
+    want = ref.scan(batch=RequestBatch([rows], sources=[-1]), **inp)
+    state = torch.full_like(inp["state"], float("nan"))  # a fresh prompt reads nothing
+    at, ys = 0, []
+    for k, length in enumerate([17, 1, 1, 8, 1, 13]):
+        part = {n: (t[at:at + length] if n in ("x", "delta", "B", "C", "z") else t) for n, t in inp.items()}
+        batch = RequestBatch([length], sources=[-1] if k == 0 else [0])
+        ys.append(selective_scan_cached_cuda(batch=batch, **dict(part, state=state)))
+        at += length
+    ref.check("y", torch.cat(ys), want[0], want[1])
+    ref.check("state", state, want[2], want[3])
+
+
+def test_scan_strided_rows():
+    """Column slices of wider rows at odd offsets, rows that repeat (stride 0),
+    columns with a stride, and types that have to be cast."""
+    rows, dn = 50, 37
+    inp = _scan_inputs(rows, dn, 4, seed=11)
+    wide = torch.randn(rows, 3 * dn + 5, device="cuda")
+    wide[:, 1:1 + dn], wide[:, 2 + dn:2 + 2 * dn] = inp["x"], inp["z"]
+    inp["x"], inp["z"] = wide[:, 1:1 + dn], wide[:, 2 + dn:2 + 2 * dn]
+    dbc = torch.randn(rows, 35, device="cuda")
+    inp["B"] = dbc[:, 3:19]
+    inp["C"] = inp["C"][:1].expand(rows, 16)
+    inp["delta"] = inp["delta"].t().contiguous().t()
+    inp["D"] = inp["D"].double()
+    for batch in (RequestBatch([20, 30], sources=[-1, 3], slots=[1, 2]), RequestBatch([1] * 4, slots=[3, 0, 1, 2])):
+        cut = {n: (t[:batch.tokens] if n in ("x", "delta", "B", "C", "z") else t) for n, t in inp.items()}
+        _scan_check("strided", cut, batch)
+
+
+def test_rows_behind_the_last_request_and_padding_requests():
+    inp = _scan_inputs(20, 40, 6, seed=2)
+    nan = torch.full((20, 40), float("nan"), device="cuda")
+    x = torch.where(torch.arange(20, device="cuda")[:, None] < 12, inp["x"], nan)  # rows 12..: never read
+    batch = RequestBatch([5, 4, 3], slots=[0, -1, 5])
+    x[5:9] = float("nan")  # the padding request's rows
+    state = inp["state"].clone()
+    y = selective_scan_cached_cuda(batch=batch, **dict(inp, x=x, state=state))
+    assert (y[12:] == 0).all() and (y[5:9] == 0).all()
+    want = ref.scan(batch=batch, **inp)
+    ref.check("y", y[:5], want[0][:5], want[1][:5])
+    ref.check("state", state, want[2], want[3])  # slots 1..4 bit for bit
+    w, b = torch.randn(40, 4, 1, device="cuda"), torch.randn(40, device="cuda")
+    cs = torch.randn(6, 3, 40, device="cuda")
+    new = cs.clone()
+    out = conv1d_silu_cached_cuda(x, w, b, new, batch)
+    assert (out[12:] == 0).all() and (out[5:9] == 0).all()
+    want = ref.conv(inp["x"], w, b, cs, batch)
+    ref.check("conv", out[:5], want[0][:5], want[1][:5])
+    ref.check("window", new, want[2], torch.zeros_like(want[2]))
+
+
+def test_one_request_does_not_reach_another():
+    """Non-finite values stay in their own request, and a fresh request does
+    not read its slot."""
+    lengths = [9, 1, 0, 700, 30]
+    inp = _scan_inputs(sum(lengths), 33, 5, seed=4)
+    batch = RequestBatch(lengths, sources=[0, -1, 2, 3, 4])
+    clean = inp["state"].clone()
+    y0 = selective_scan_cached_cuda(batch=batch, **dict(inp, state=clean))
+    bad = {k: (v.clone() if v is not None else None) for k, v in inp.items()}
+    bad["x"][9] = float("nan")
+    bad["x"][12:14] = float("inf")
+    bad["state"][1] = float("nan")
+    y1 = selective_scan_cached_cuda(batch=batch, **bad)
+    same = torch.ones(sum(lengths), dtype=torch.bool, device="cuda")
+    same[9:710] = False
+    assert torch.equal(y0[same], y1[same])
+    assert torch.isnan(y1[9]).all() and not torch.isfinite(y1[12:14]).any()
+    for s in (0, 2, 4):
+        assert torch.equal(clean[s], bad["state"][s])
+    inp["state"][1] = float("nan")
+    fresh = inp["state"].clone()
+    assert torch.equal(selective_scan_cached_cuda(batch=batch, **dict(inp, state=fresh)), y0)
+
+
+def test_extreme_steps():
+    """Steps of zero keep the state, huge steps clear it."""
+    inp = _scan_inputs(6, 32, 2, seed=9)
+    inp["delta"][0:2] = 0.0
+    inp["delta"][3] = 200.0
+    inp["x"][3] = 0.0
+    batch = RequestBatch([2, 4])
+    y, state = _scan_check("extreme", inp, batch)
+    assert torch.equal(state[0], inp["state"][0])
+
+
+def test_cache_offsets_beyond_32_bits():
+    dn = 1024
+    slots = 2 ** 31 // (dn * 16) + 6
+    state = torch.zeros(slots, dn, 16, device="cuda")
+    inp = _scan_inputs(12, dn, 4, seed=6)
+    lengths = [7, 1, 4]
+    at = [slots - 1, slots - 2, slots - 3]
+    for i, s in enumerate(at):
+        state[s] = inp["state"][i]
+    small = RequestBatch(lengths, slots=[0, 1, 2])
+    want = ref.scan(batch=small, **inp)
+    y = selective_scan_cached_cuda(batch=RequestBatch(lengths, slots=at), **dict(inp, state=state))
+    ref.check("y", y, want[0], want[1])
+    ref.check("state", state[at], want[2][:3], want[3][:3])
+    want = ref.scan(batch=RequestBatch([1] * 3), **{k: (v[:3] if k in "x delta B C z".split() else v) for k, v in inp.items()})
+    for i, s in enumerate(at):
+        state[s] = inp["state"][i]
+    y = selective_scan_cached_cuda(batch=RequestBatch([1] * 3, slots=at),
+                                   **{k: (v[:3] if k in "x delta B C z".split() else v) for k, v in dict(inp, state=state).items()})
+    ref.check("token y", y, want[0], want[1])
+    ref.check("token state", state[at], want[2][:3], want[3][:3])
+    assert state[:4].abs().max() == 0
+    del state
+    torch.cuda.empty_cache()
+    c, k = 4096, 8
+    slots = 2 ** 31 // (c * (k - 1)) + 6
+    win = torch.zeros(slots, k - 1, c, dtype=BF16, device="cuda")
+    x, w, b = torch.randn(9, c, device="cuda").to(BF16), torch.randn(c, k, 1, device="cuda"), torch.randn(c, device="cuda")
+    few = torch.randn(2, k - 1, c, device="cuda").to(BF16)
+    win[slots - 2:] = few
+    y = conv1d_silu_cached_cuda(x, w, b, win, RequestBatch([3, 6], slots=[slots - 2, slots - 1]))
+    want = ref.conv(x, w, b, few, RequestBatch([3, 6]))
+    ref.check("conv", y, want[0], want[1])
+    ref.check("window", win[slots - 2:], want[2], torch.zeros_like(want[2]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("k", [1, 2, 4, 5, 8])
+@pytest.mark.parametrize("c", [1, 64, 66, 771])
+@pytest.mark.parametrize("lengths", [[1], [1] * 9, [3, 0, 1, 2, 40], [31, 32, 33, 64, 100], [200]])
+def test_conv(lengths, c, k, dtype):
+    batch = _mixed(lengths)
+    g = _gen(c + k)
+    x = torch.randn(batch.tokens, c, generator=g, device="cuda").to(dtype)
+    w = torch.randn(c, k, 1, generator=g, device="cuda")
+    b = torch.randn(c, generator=g, device="cuda")
+    state = torch.randn(2 * len(lengths), k - 1, c, generator=g, device="cuda").to(dtype)
+    for bt in (batch, RequestBatch(lengths)):  # forked, and in place
+        want = ref.conv(x, w, b, state, bt)
+        new = state.clone()
+        y = conv1d_silu_cached_cuda(x, w, b, new, bt)
+        assert y.dtype == dtype
+        ref.check(f"conv {lengths} {c} {k}", y, want[0], want[1])
+        ref.check("window", new, want[2], torch.zeros_like(want[2]))  # copies: exact
+
+
+def test_conv_strided_rows():
+    x = torch.randn(40, 100, device="cuda")
+    w, b = torch.randn(64, 4, 1, device="cuda"), torch.randn(64, device="cuda")
+    state = torch.randn(2, 3, 64, device="cuda")
+    for off in (0, 4, 5):
+        v = x[:, off:off + 64]
+        bt = RequestBatch([30, 10])
+        want = ref.conv(v, w, b, state, bt)
+        new = state.clone()
+        ref.check(f"offset {off}", conv1d_silu_cached_cuda(v, w, b, new, bt), want[0], want[1])
+        ref.check("window", new, want[2], torch.zeros_like(want[2]))
+
+
+def _lora_inputs(batch, count, d_in, d_out, rank, dtype, seed=0, rows=None):
+    g = _gen(seed)
+    n = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    rows = batch.tokens if rows is None else rows
+    ads = LoraAdapters((n(count, rank, d_in) * d_in ** -0.5).to(dtype), (n(count, d_out, rank) * rank ** -0.5).to(dtype),
+                       [0.5 + i for i in range(count)])
+    return n(rows, d_out).to(dtype), n(rows, d_in).to(dtype), ads
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d_in,d_out,rank", [(1, 1, 1), (8, 8, 4), (33, 70, 5), (384, 520, 16), (130, 257, 64), (96, 64, 128)])
+@pytest.mark.parametrize("lengths", [[1], [1] * 21, [0, 40, 1, 17, 100], [16, 32]])
+def test_lora(lengths, d_in, d_out, rank, dtype):
+    n = len(lengths)
+    batch = RequestBatch(lengths, adapters=[(i * 5 + 2) % 4 - 1 for i in range(n)])
+    base, x, ads = _lora_inputs(batch, 3, d_in, d_out, rank, dtype, seed=d_in + n)
+    want = ref.lora(base, x, ads, batch)
+    y = lora_add_cuda(base, x, ads, batch)
+    ref.check(f"lora {lengths} {d_in} {d_out} {rank}", y, want[0], want[1])
+    assert torch.equal(y, lora_add_cuda(base, x, ads, batch))
+    inside = base.clone()
+    assert lora_add_cuda(inside, x, ads, batch, out=inside) is inside and torch.equal(inside, y)
+
+
+def test_lora_strides_and_rows_behind():
+    batch = RequestBatch([5, 20, 1], adapters=[1, -1, 0])
+    base, x, ads = _lora_inputs(batch, 2, 40, 30, 8, F32, rows=31)
+    wide = torch.randn(31, 100, device="cuda")
+    wide[:, 1:41], wide[:, 43:73] = x, base
+    want = ref.lora(base, x, ads, batch)
+    for xv, bv in ((wide[:, 1:41], wide[:, 43:73]), (x.t().contiguous().t(), base.t().contiguous().t())):
+        y = lora_add_cuda(bv, xv, ads, batch)
+        ref.check("strided", y, want[0], want[1])
+        assert torch.equal(y[26:], base[26:]) and torch.equal(y[5:25], base[5:25])
+    out = torch.zeros(31, 64, device="cuda")[:, 3:33]
+    assert torch.equal(lora_add_cuda(base, x, ads, batch, out=out), out)
+    ref.check("out", out, want[0], want[1])
+    view = wide[:, 43:73]  # a column slice beside x in the same rows, updated in place
+    lora_add_cuda(view, wide[:, 1:41], ads, batch, out=view)
+    ref.check("in place", view, want[0], want[1])
+    assert torch.equal(wide[:, 1:41], x)
+
+
+def test_refusals():
+    inp = _scan_inputs(4, 32, 2)
+    batch = RequestBatch([3, 1])
+    run = lambda b=batch, **kw: selective_scan_cached_cuda(batch=b, **dict(inp, **kw))  # noqa: E731
+    with pytest.raises(TypeError):
+        run(x=inp["x"].half())
+    with pytest.raises(ValueError):
+        run(b=RequestBatch([3, 2]))  # more rows than x has
+    with pytest.raises(ValueError):
+        run(b=RequestBatch([3, 1], slots=[0, 2]))  # slot outside the cache
+    with pytest.raises(ValueError):
+        run(b=RequestBatch([3, 1], sources=[0, 2], slots=[0, 1]))
+    with pytest.raises(ValueError):
+        run(state=inp["state"].to(BF16))
+    with pytest.raises(ValueError):
+        run(state=inp["state"].transpose(0, 1).contiguous().transpose(0, 1))
+    with pytest.raises(ValueError):
+        run(A=inp["A"][:, :8])
+    with pytest.raises(ValueError):
+        run(B=inp["B"][:3])
+    with pytest.raises(RuntimeError):
+        run(delta=inp["delta"].cpu())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        run(x=inp["x"].clone().requires_grad_(True))
+    with torch.no_grad():
+        run(x=inp["x"].clone().requires_grad_(True), state=inp["state"].clone())
+    w, b = torch.randn(32, 4, 1, device="cuda"), torch.randn(32, device="cuda")
+    with pytest.raises(ValueError):
+        conv1d_silu_cached_cuda(inp["x"], torch.randn(32, 9, 1, device="cuda"), b, torch.zeros(2, 8, 32, device="cuda"), batch)
+    with pytest.raises(ValueError):
+        conv1d_silu_cached_cuda(inp["x"], w, b, torch.zeros(2, 4, 32, device="cuda"), batch)
+    with pytest.raises(ValueError):
+        conv1d_silu_cached_cuda(inp["x"].to(BF16), w, b, torch.zeros(2, 3, 32, device="cuda"), batch)
+    lb = RequestBatch([3, 1], adapters=[0, 1])
+    base, x, ads = _lora_inputs(lb, 2, 24, 16, 4, F32)
+    with pytest.raises(ValueError):
+        lora_add_cuda(base, x, ads, batch)  # no adapters in the batch
+    with pytest.raises(ValueError):
+        lora_add_cuda(base, x, ads, RequestBatch([3, 1], adapters=[0, 2]))
+    with pytest.raises(TypeError):
+        lora_add_cuda(base.to(BF16), x.to(BF16), ads, lb)
+    with pytest.raises(ValueError):
+        lora_add_cuda(base, x, ads, lb, out=base[:1].expand(4, 16))
+    both = torch.randn(4, 30, device="cuda")
+    with pytest.raises(ValueError):
+        lora_add_cuda(base, both[:, :24], ads, lb, out=both[:, 10:26])
+    with pytest.raises(ValueError):
+        LoraAdapters(torch.zeros(1, 129, 4, device="cuda"), torch.zeros(1, 4, 129, device="cuda"))
+
+
+def test_other_streams_and_graphs():
+    """The same batch on two streams, captured, replayed with new inputs, and
+    replayed after its slots and adapters changed."""
+    dn, count = 48, 6
+    batch = RequestBatch([1] * count, slots=list(range(count)), adapters=[0] * count)
+    base, xl, ads = _lora_inputs(batch, 2, 24, 40, 4, F32, seed=1)
+    inp = _scan_inputs(count, dn, 2 * count, seed=8)
+    w, b = torch.randn(dn, 4, 1, device="cuda"), torch.randn(dn, device="cuda")
+    win = torch.randn(2 * count, 3, dn, device="cuda")
+
+    def step(state, window):
+        c = conv1d_silu_cached_cuda(inp["x"], w, b, window, batch)
+        return c, selective_scan_cached_cuda(batch=batch, **dict(inp, state=state)), lora_add_cuda(base, xl, ads, batch)
+
+    s0, w0 = inp["state"].clone(), win.clone()
+    first = step(s0, w0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s1, w1 = inp["state"].clone(), win.clone()
+        second = step(s1, w1)
+    torch.cuda.current_stream().wait_stream(side)
+    for p, q in zip(first + (s0, w0), second + (s1, w1)):
+        assert torch.equal(p, q)
+
+    state, window = inp["state"].clone(), win.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(state, window)
+    state.copy_(inp["state"])
+    window.copy_(win)
+    graph.replay()
+    for p, q in zip(first + (s0, w0), captured + (state, window)):
+        assert torch.equal(p, q)
+
+    batch.update(slots=[7, -1, 9, 2, 0, 1], sources=[3, 0, -1, 2, 0, 1], adapters=[1, 0, -1, 1, 1, 0])
+    state.copy_(inp["state"])
+    window.copy_(win)
+    graph.replay()
+    want = ref.scan(batch=batch, **inp)
+    ref.check("y", captured[1], want[0], want[1])
+    ref.check("state", state, want[2], want[3])
+    want = ref.conv(inp["x"], w, b, win, batch)
+    ref.check("conv", captured[0], want[0], want[1])
+    ref.check("window", window, want[2], torch.zeros_like(want[2]))
+    want = ref.lora(base, xl, ads, batch)
+    ref.check("lora", captured[2], want[0], want[1])
+    s2, w2 = inp["state"].clone(), win.clone()
+    for p, q in zip(step(s2, w2) + (s2, w2), captured + (state, window)):
+        assert torch.equal(p, q)
+
+
+def test_capture_needs_an_eager_call():
+    inp = _scan_inputs(3, 32, 1)
+    batch = RequestBatch([3])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="once"):
+        with torch.cuda.graph(graph):
+            selective_scan_cached_cuda(batch=batch, **inp)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("d_model", [64, 20])
+def test_block_serves_what_it_computes(d_model):
+    """MambaBlock.serve over prompts and single tokens, against the oracle's
+    block on each request's whole sequence in 64 bits (and the oracle in 32
+    bits for the reference's own rounding)."""
+    from oracle.model_ref import MambaBlockRef
+    from parity import assert_parity
+
+    torch.manual_seed(d_model)
+    block = MambaBlock(d_model=d_model).cuda()
+    res = ResidualMambaBlock(d_model=d_model).cuda()
+    oracle = {}
+    for dt in (torch.float64, F32):
+        oracle[dt] = MambaBlockRef(d_model=d_model)
+        oracle[dt].load_state_dict({k: v.cpu() for k, v in block.state_dict().items()})
+        oracle[dt].to(dt)
+    totals = [40, 7, 90]
+    seqs = [torch.randn(t, d_model) for t in totals]
+    fed, outs = [0, 0, 0], [[], [], []]
+    cache = block.new_cache(4)
+    for lengths in ([17, 2, 64], [1, 1, 1], [1, 1, 1], [5, 0, 20], [16, 3, 4]):
+        rows = torch.cat([s[f:f + l] for s, f, l in zip(seqs, fed, lengths)]).cuda()
+        batch = RequestBatch(lengths, slots=[2, 0, 3], sources=[-1] * 3 if fed == [0, 0, 0] else None)
+        y = block.serve(rows, cache, batch).cpu()
+        at = 0
+        for i, l in enumerate(lengths):
+            outs[i].append(y[at:at + l])
+            at += l
+            fed[i] += l
+    assert fed == totals
+    with torch.no_grad():
+        for i, s in enumerate(seqs):
+            exact, ref32 = oracle[torch.float64](s[None].double())[0], oracle[F32](s[None])[0]
+            assert_parity(f"serve {d_model} request {i}", torch.cat(outs[i]), exact, ref32)
+        rows = torch.randn(30, d_model, device="cuda")
+        got = res.serve(rows, res.new_cache(1), RequestBatch([30], sources=[-1]))
+        want = res(rows[None])[0]
+        assert (got - want).abs().max() <= 1e-5 * want.abs().max()
+    assert (cache.ssm[1] == 0).all() and (cache.conv[1] == 0).all()
+
+
+def test_block_serves_adapters():
+    """Adapters on in_proj and out_proj are those projections with W + scale B A."""
+    torch.manual_seed(1)
+    d = 64
+    block = MambaBlock(d_model=d).cuda()
+    g = _gen(2)
+    n = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    ain = LoraAdapters(n(2, 8, d) * d ** -0.5, n(2, 4 * d, 8) * 0.1, [1.0, 2.0])
+    aout = LoraAdapters(n(2, 4, 2 * d) * d ** -0.5, n(2, d, 4) * 0.1)
+    lengths, picks = [20, 1, 33], [1, -1, 0]
+    x = n(sum(lengths), d)
+    batch = RequestBatch(lengths, sources=[-1] * 3, adapters=picks)
+    y = block.serve(x, block.new_cache(3), batch, ain, aout)
+    at = 0
+    for l, k in zip(lengths, picks):
+        merged = MambaBlock(d_model=d).cuda()
+        merged.load_state_dict(block.state_dict())
+        with torch.no_grad():
+            if k >= 0:
+                merged.in_proj.weight += ain.scale[k] * (ain.b[k] @ ain.a[k])
+                merged.out_proj.weight += aout.scale[k] * (aout.b[k] @ aout.a[k])
+            want = merged.serve(x[at:at + l], merged.new_cache(1), RequestBatch([l], sources=[-1]))
+        # the two orders of the same products differ by fp32 roundings of sums of at most 256 terms through
+        # a block whose gains are of order one
+        assert (y[at:at + l] - want).abs().max() <= 2e-5 * want.abs().max()
+        at += l
