@@ -1317,6 +1317,12 @@ int cached_scan_args(CachedScanArgs& a, int64_t rows, int64_t d_inner, int64_t d
   return VMSCAN_OK;
 }
 
+// Whether rows of four-element groups can be read with one load each.
+template <typename T>
+bool four_wide(const void* p, int64_t ld) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && ld % 4 == 0;
+}
+
 struct CachedScanPlan {
   int groups;       // CTAs per piece
   size_t carry, sums, total;
@@ -1331,7 +1337,35 @@ CachedScanPlan cached_scan_plan(int64_t d_inner, int64_t carry_rows) {
   return p;
 }
 
+// Widest copy (16, 4 or 2 bytes) that takes rows of a multiple of its
+// elements at this address and stride.
 template <typename T>
+int row_grain(const void* p, int64_t ld, int64_t cols) {
+  for (int g : {16, 4})
+    if (reinterpret_cast<uintptr_t>(p) % g == 0 && ld * int64_t(sizeof(T)) % g == 0 && cols * int64_t(sizeof(T)) % g == 0)
+      return g;
+  return 2;
+}
+
+template <typename T>
+int cached_scan_grain(const CachedScanArgs& a) {
+  const int g = std::min(row_grain<T>(a.u, a.ldu, a.dn), row_grain<T>(a.delta, a.ldd, a.dn));
+  return a.z != nullptr ? std::min(g, row_grain<T>(a.z, a.ldz, a.dn)) : g;
+}
+
+template <typename T, int G, bool HAS_Z, bool CARRY>
+int launch_scan_pass(const CachedScanArgs& a, const int32_t* pieces, int64_t n, int groups, const float* h_start,
+                     float* carry_h, float* carry_s, cudaStream_t s) {
+  constexpr size_t smem = cached_scan_smem<T>();
+  auto kern = cached_scan_kernel<T, G, HAS_Z, CARRY>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    return fail(VMSCAN_ERR_LAUNCH, "cudaFuncSetAttribute(cached_scan_kernel) failed");
+  const int bc = std::min(row_grain<T>(a.B, a.ldb, NS), row_grain<T>(a.C, a.ldc, NS));
+  kern<<<unsigned(n * groups), CSC_WARPS * 32, smem, s>>>(a, pieces, groups, bc, h_start, carry_h, carry_s);
+  return check_launch();
+}
+
+template <typename T, int G>
 int launch_cached_scan(const CachedScanArgs& a, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
                        const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* ws, cudaStream_t s) {
   const CachedScanPlan p = cached_scan_plan(a.dn, carry_rows);
@@ -1340,19 +1374,25 @@ int launch_cached_scan(const CachedScanArgs& a, const int32_t* pieces, int64_t n
   float* h_start = reinterpret_cast<float*>(w + p.carry);
   float* carry_s = reinterpret_cast<float*>(w + 2 * p.carry);
   if (n_chains > 0) {
-    cached_scan_kernel<T, false, true><<<unsigned(n_carry * p.groups), CSC_WARPS * 32, 0, s>>>(
-        a, pieces, p.groups, nullptr, carry_h, carry_s);
-    VM_TRY(check_launch());
+    VM_TRY((launch_scan_pass<T, G, false, true>(a, pieces, n_carry, p.groups, nullptr, carry_h, carry_s, s)));
     cached_chain_kernel<<<dim3(unsigned((int64_t(a.dn) * NS + 127) / 128), unsigned(n_chains)), 128, 0, s>>>(
         chains, a.A, a.state, a.n_slots, carry_h, carry_s, h_start, a.dn);
     VM_TRY(check_launch());
   }
-  const unsigned grid = unsigned(n_pieces * p.groups);
   if (a.z != nullptr)
-    cached_scan_kernel<T, true, false><<<grid, CSC_WARPS * 32, 0, s>>>(a, pieces, p.groups, h_start, nullptr, nullptr);
-  else
-    cached_scan_kernel<T, false, false><<<grid, CSC_WARPS * 32, 0, s>>>(a, pieces, p.groups, h_start, nullptr, nullptr);
-  return check_launch();
+    return launch_scan_pass<T, G, true, false>(a, pieces, n_pieces, p.groups, h_start, nullptr, nullptr, s);
+  return launch_scan_pass<T, G, false, false>(a, pieces, n_pieces, p.groups, h_start, nullptr, nullptr, s);
+}
+
+template <typename T>
+int run_cached_scan(const CachedScanArgs& a, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
+                    const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* ws, cudaStream_t s) {
+  const int g = cached_scan_grain<T>(a);
+  if (g == 16) return launch_cached_scan<T, 16>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, ws, s);
+  if constexpr (sizeof(T) == 2) {
+    if (g == 2) return launch_cached_scan<T, 2>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, ws, s);
+  }
+  return launch_cached_scan<T, 4>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, ws, s);
 }
 
 template <typename T>
@@ -1368,18 +1408,38 @@ int launch_cached_step(const CachedScanArgs& a, const int32_t* slots, const int3
 
 template <typename T>
 int launch_cached_conv(const CachedConvArgs& a, const int32_t* pieces, int64_t n_pieces, cudaStream_t s) {
-  const size_t q = 4 * sizeof(T);  // bytes of a four-channel access
-  const auto fits = [&](const void* p, int64_t ld) {
-    return reinterpret_cast<uintptr_t>(p) % q == 0 && (ld * int64_t(sizeof(T))) % int64_t(q) == 0;
-  };
-  const bool wide = a.channels % 4 == 0 && fits(a.x, a.ldx) && fits(a.out, a.ldo) && fits(a.state, a.channels);
+  const bool wide = a.channels % 4 == 0 && four_wide<T>(a.x, a.ldx) && four_wide<T>(a.out, a.ldo) &&
+                    four_wide<T>(a.state, a.channels);
   const int groups = (a.channels + CCV_THREADS * (wide ? 4 : 1) - 1) / (CCV_THREADS * (wide ? 4 : 1));
   if (n_pieces * groups > INT32_MAX) return fail(VMSCAN_ERR_SHAPE, "cached conv: %lld pieces", (long long)n_pieces);
   const unsigned grid = unsigned(n_pieces * groups);
-  if (wide)
-    cached_conv_kernel<T, 4><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+  if (wide && a.K <= 4)
+    cached_conv_kernel<T, 4, 4><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+  else if (wide)
+    cached_conv_kernel<T, 4, 8><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+  else if (a.K <= 4)
+    cached_conv_kernel<T, 1, 4><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
   else
-    cached_conv_kernel<T, 1><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+    cached_conv_kernel<T, 1, 8><<<grid, CCV_THREADS, 0, s>>>(a, pieces, groups);
+  return check_launch();
+}
+
+template <typename T>
+int launch_lora(LoraArgs& l, int n_tiles, cudaStream_t s) {
+  l.wide_in = row_grain<T>(l.x, l.ldx, l.d_in) == 16 && row_grain<T>(l.a, l.d_in, l.d_in) == 16;
+  l.wide_rank = l.rank % 4 == 0 && four_wide<T>(l.b, l.rank);
+  l.wide_out = l.d_out % 4 == 0 && four_wide<T>(l.base, l.ldbase) && four_wide<T>(l.out, l.ldout);
+  // column shares (of whole 64-column rounds of the CTA's warps): enough that
+  // a few tiles still occupy the SMs; each share forms the rank-wide products
+  // of its tile again
+  const int rounds = (l.d_out + 16 * LORA_WARPS - 1) / (16 * LORA_WARPS);
+  const int shares = std::max(1, std::min(rounds, 2 * sm_count() / n_tiles));
+  const int cols = (rounds + shares - 1) / shares * 16 * LORA_WARPS;
+  const size_t smem = lora_smem<T>(l.rank);
+  if (cudaFuncSetAttribute(lora_add_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(lora_smem<T>(LORA_RMAX))) != cudaSuccess)
+    return fail(VMSCAN_ERR_LAUNCH, "cudaFuncSetAttribute(lora_add_kernel) failed");
+  lora_add_kernel<T><<<dim3(unsigned(n_tiles), unsigned((l.d_out + cols - 1) / cols)), LORA_WARPS * 32, smem, s>>>(l, cols);
   return check_launch();
 }
 
@@ -1490,8 +1550,8 @@ int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16,
   VM_TRY(ensure_context(state));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (bf16)
-    return launch_cached_scan<__nv_bfloat16>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
-  return launch_cached_scan<float>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
+    return run_cached_scan<__nv_bfloat16>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
+  return run_cached_scan<float>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
 }
 
 int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
@@ -1520,7 +1580,8 @@ int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int
   if (weight == nullptr || bias == nullptr || pieces == nullptr || (ksize > 1 && state == nullptr) ||
       (rows > 0 && (x == nullptr || out == nullptr)))
     return VMSCAN_ERR_NULL;
-  if (!aligned16(pieces)) return fail(VMSCAN_ERR_ALIGN, "pieces must be 16-byte aligned");
+  if (!aligned16(pieces) || !aligned16(weight))
+    return fail(VMSCAN_ERR_ALIGN, "pieces and weight must be 16-byte aligned");
   VM_TRY(check_row_stride("x", ldx, rows));
   VM_TRY(check_out_stride("out", ldo, channels, rows));
   VM_TRY(ensure_context(pieces));
@@ -1598,18 +1659,11 @@ int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int
   VM_TRY(check_row_stride("base", ldbase, rows));
   VM_TRY(check_out_stride("out", ldout, d_out, rows));
   VM_TRY(ensure_context(out));
-  const LoraArgs l{x, a, b, base, out, scale, row_index, tiles, ldx, ldbase, ldout, int(rows), int(d_in), int(d_out),
-                   int(rank), int(n_adapters), int(n_index)};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // enough column shares to give every SM a CTA
-  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>((d_out + 127) / 128, sm_count() * 2 / n_tiles));
-  const int cols = int((d_out + shares - 1) / shares);
-  const dim3 grid(unsigned(n_tiles), unsigned((d_out + cols - 1) / cols));
-  if (bf16)
-    lora_add_kernel<__nv_bfloat16><<<grid, LORA_THREADS, 0, s>>>(l, cols);
-  else
-    lora_add_kernel<float><<<grid, LORA_THREADS, 0, s>>>(l, cols);
-  return check_launch();
+  LoraArgs l{x, a, b, base, out, scale, row_index, tiles, ldx, ldbase, ldout, int(rows), int(d_in), int(d_out),
+             int(rank), int(n_adapters), int(n_index), 0, 0, 0};
+  if (bf16) return launch_lora<__nv_bfloat16>(l, int(n_tiles), s);
+  return launch_lora<float>(l, int(n_tiles), s);
 }
 
 }  // extern "C"

@@ -73,119 +73,287 @@ struct CachedScanArgs {
 };
 
 // ---------------------------------------------------------------------------
-// Prompts: a warp owns 32 channels of one piece, a lane one channel and its 16
-// states.  B and C of CSC_ROWS rows are staged in the warp's shared memory.
+// Prompts: a warp owns 32 channels of one piece.  A lane pair owns two adjacent
+// channels and each lane 8 of the 16 states of both, so a B / C value read from
+// shared memory serves two channels.  The rows travel through a ring of
+// CSC_STAGES blocks of CSC_ROWS rows in the warp's own shared memory, filled by
+// asynchronous copies: a warp needs no other warp and no barrier, and one warp
+// alone on its scheduler still has 3 blocks in flight.
+// G: bytes of one copy, the widest that the rows' alignment allows
+// (cached_scan_grain): 16, 4 (two bf16 or one fp32) or 2 (odd bf16 rows: plain
+// loads, kept in registers while the block before is computed).  bc_grain: the
+// same for B and C.
 // CARRY: only the state at the piece's end from a zero state and the sum of
 // delta (the piece maps h to exp(A sum delta) h + carry_h).
 // ---------------------------------------------------------------------------
 constexpr int CSC_WARPS = 4;
 constexpr int CSC_ROWS = 8;
+constexpr int CSC_STAGES = 3;
 
-template <typename T, bool HAS_Z, bool CARRY>
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// First column (of 32) that a lane copies, and the copies of CSC_ROWS rows
+// into dst[row][32].  p: that column of row 0; rows past `last` repeat it.
+template <typename T, int G>
+__device__ __forceinline__ int copy_col(int lane) {
+  constexpr int E = G / int(sizeof(T));
+  return lane % (32 / E) * E;
+}
+template <typename T, int G>
+__device__ __forceinline__ void copy_rows(T* dst, const T* p, int64_t ld, int t0, int last, int lane) {
+  constexpr int E = G / int(sizeof(T)), LPR = 32 / E;  // E rows at a time
+  static_assert(CSC_ROWS % E == 0, "a copy must not reach past the block's rows");
+#pragma unroll
+  for (int r0 = 0; r0 < CSC_ROWS; r0 += E) {
+    const int r = r0 + lane / LPR;
+    cp_async<G>(dst + r * 32 + lane % LPR * E, p + min(t0 + r, last) * ld);
+  }
+}
+
+// One stage of a warp's ring.
+template <typename T>
+struct ScanStage {
+  T u[CSC_ROWS][32], dl[CSC_ROWS][32], z[CSC_ROWS][32], bc[CSC_ROWS][32];
+};
+template <typename T>
+struct ScanRing {
+  ScanStage<T> st[CSC_STAGES];
+  float wide[sizeof(T) == 4 ? 1 : CSC_ROWS][32];  // bf16: the block's B | C as fp32
+};
+template <typename T>
+constexpr size_t cached_scan_smem() {
+  return sizeof(ScanRing<T>) * CSC_WARPS;
+}
+
+template <typename T, int G, bool HAS_Z, bool CARRY>
 __global__ void __launch_bounds__(CSC_WARPS * 32)
-    cached_scan_kernel(const CachedScanArgs a, const int32_t* __restrict__ pieces, int groups,
+    cached_scan_kernel(const CachedScanArgs a, const int32_t* __restrict__ pieces, int groups, int bc_grain,
                        const float* __restrict__ h_start, float* __restrict__ carry_h, float* __restrict__ carry_s) {
-  __shared__ float bc[CSC_WARPS][CSC_ROWS][2 * NS];
+  constexpr bool LOAD_Z = HAS_Z && !CARRY;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ScanRing<T>& ring = reinterpret_cast<ScanRing<T>*>(smem_raw)[warp];
   const Piece p = load_piece(pieces, blockIdx.x / groups, a.rows, a.n_slots);
-  const int d = ((blockIdx.x % groups) * CSC_WARPS + warp) * 32 + lane;
-  if (d - lane >= a.dn) return;  // whole warps only: the rest of the kernel shuffles and syncs by warp
-  const bool ok = d < a.dn;
-  const int dc = ok ? d : a.dn - 1;
-  const T* __restrict__ u = static_cast<const T*>(a.u) + dc;
-  const T* __restrict__ dl = static_cast<const T*>(a.delta) + dc;
-  const T* __restrict__ z = static_cast<const T*>(a.z) + (HAS_Z ? dc : 0);
-  T* __restrict__ y = static_cast<T*>(a.y) + dc;
+  const int d0 = ((blockIdx.x % groups) * CSC_WARPS + warp) * 32;
+  if (d0 >= a.dn) return;  // whole warps: the rest shuffles and syncs by warp only
+  const int hb = lane & 1, pc = lane & ~1;
+  const int own = d0 + lane, dp = d0 + pc;
+  const bool ok = own < a.dn;
+  T* __restrict__ y = static_cast<T*>(a.y) + min(own, a.dn - 1);
   if (p.slot < 0) {  // padding request
     if (!CARRY && ok)
       for (int t = p.t0; t < p.t1; ++t) y[t * a.ldy] = from_f<T>(0.f);
     return;
   }
-  float2 A2[8], h[8];
+  // what this lane copies: columns past the last channel repeat the last ones
+  const int last = p.t1 - 1;
+  constexpr int E = G / int(sizeof(T));
+  const int col = min(d0 + copy_col<T, G>(lane), a.dn - E);
+  const T* __restrict__ pu = static_cast<const T*>(a.u) + col;
+  const T* __restrict__ pd = static_cast<const T*>(a.delta) + col;
+  const T* __restrict__ pz = static_cast<const T*>(a.z) + (LOAD_Z ? col : 0);
+  const int bcol = bc_grain == 16 ? copy_col<T, 16>(lane) : bc_grain == 4 ? copy_col<T, 4>(lane) : lane;
+  const bool is_b = bcol < NS;
+  const T* __restrict__ pbc = is_b ? static_cast<const T*>(a.B) + bcol : static_cast<const T*>(a.C) + bcol - NS;
+  const int64_t ldbc = is_b ? a.ldb : a.ldc;
+  T ru[G == 2 ? CSC_ROWS : 1], rd[G == 2 ? CSC_ROWS : 1], rz[G == 2 ? CSC_ROWS : 1], rbc[sizeof(T) == 2 ? CSC_ROWS : 1];
+
+  auto issue = [&](int t0, ScanStage<T>& st) {
+    if (t0 < p.t1) {
+      if constexpr (G == 2) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float4 v = *reinterpret_cast<const float4*>(a.A + int64_t(dc) * NS + 4 * j);
-    A2[2 * j] = make_float2(v.x, v.y);
-    A2[2 * j + 1] = make_float2(v.z, v.w);
+        for (int r = 0; r < CSC_ROWS; ++r) {
+          const int64_t t = min(t0 + r, last);
+          ru[r] = pu[t * a.ldu];
+          rd[r] = pd[t * a.ldd];
+          if (LOAD_Z) rz[r] = pz[t * a.ldz];
+        }
+      } else {
+        copy_rows<T, G>(&st.u[0][0], pu, a.ldu, t0, last, lane);
+        copy_rows<T, G>(&st.dl[0][0], pd, a.ldd, t0, last, lane);
+        if (LOAD_Z) copy_rows<T, G>(&st.z[0][0], pz, a.ldz, t0, last, lane);
+      }
+      if (!CARRY || is_b) {
+        if (bc_grain == 16) {
+          copy_rows<T, 16>(&st.bc[0][0], pbc, ldbc, t0, last, lane);
+        } else if (bc_grain == 4) {
+          copy_rows<T, 4>(&st.bc[0][0], pbc, ldbc, t0, last, lane);
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int r = 0; r < CSC_ROWS; ++r) rbc[r] = pbc[min(t0 + r, last) * ldbc];
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  // what `issue` left in registers, into its stage
+  auto settle = [&](int t0, ScanStage<T>& st) {
+    if (t0 >= p.t1) return;
+    if constexpr (G == 2) {
+#pragma unroll
+      for (int r = 0; r < CSC_ROWS; ++r) {
+        st.u[r][lane] = ru[r];
+        st.dl[r][lane] = rd[r];
+        if (LOAD_Z) st.z[r][lane] = rz[r];
+      }
+    }
+    if constexpr (sizeof(T) == 2) {
+      if (bc_grain == 2 && (!CARRY || is_b)) {
+#pragma unroll
+        for (int r = 0; r < CSC_ROWS; ++r) st.bc[r][lane] = rbc[r];
+      }
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < CSC_STAGES - 1; ++k) {
+    issue(p.t0 + k * CSC_ROWS, ring.st[k]);
+    settle(p.t0 + k * CSC_ROWS, ring.st[k]);
   }
+
+  float2 A2[2][4], h[2][4];
   const float* src = nullptr;
   if (!CARRY) {
     if (p.carry >= 0)  // also for a first piece: another piece may write the source's slot meanwhile
-      src = h_start + (int64_t(p.carry) * a.dn + dc) * NS;
+      src = h_start + int64_t(p.carry) * a.dn * NS;
     else if (p.source >= 0)
-      src = a.state + (int64_t(p.source) * a.dn + dc) * NS;
+      src = a.state + int64_t(p.source) * a.dn * NS;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float4 v = src != nullptr ? *reinterpret_cast<const float4*>(src + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-    h[2 * j] = make_float2(v.x, v.y);
-    h[2 * j + 1] = make_float2(v.z, v.w);
+  for (int c = 0; c < 2; ++c) {
+    const int64_t off = int64_t(min(dp + c, a.dn - 1)) * NS + 8 * hb;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float4 v = *reinterpret_cast<const float4*>(a.A + off + 4 * j);
+      A2[c][2 * j] = make_float2(v.x, v.y);
+      A2[c][2 * j + 1] = make_float2(v.z, v.w);
+      const float4 g = src != nullptr ? *reinterpret_cast<const float4*>(src + off + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      h[c][2 * j] = make_float2(g.x, g.y);
+      h[c][2 * j + 1] = make_float2(g.z, g.w);
+    }
   }
-  const float Dd = a.D[dc];
-  float dsum = 0.f;
-  const int brow = lane >> 2, bcol = (lane & 3) * 4;  // B / C values this lane stages
+  const float Dd = a.D[min(own, a.dn - 1)];
+  float2 dsum = make_float2(0.f, 0.f);
+
+  int stage = 0;
   for (int t0 = p.t0; t0 < p.t1; t0 += CSC_ROWS) {
+    cp_async_wait<CSC_STAGES - 2>();
+    __syncwarp();  // this block has arrived for every lane, and every lane has left the one before
+    const ScanStage<T>& st = ring.st[stage];
+    const float* bc;
+    if constexpr (sizeof(T) == 4) {
+      bc = &st.bc[0][0];
+    } else {
+      const uint4 q = *reinterpret_cast<const uint4*>(&st.bc[lane >> 2][(lane & 3) * 8]);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      float2 f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      float* o = &ring.wide[lane >> 2][(lane & 3) * 8];
+      *reinterpret_cast<float4*>(o) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+      *reinterpret_cast<float4*>(o + 4) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+      __syncwarp();
+      bc = &ring.wide[0][0];
+    }
+    const int ahead = t0 + (CSC_STAGES - 1) * CSC_ROWS;
+    ScanStage<T>& free_stage = ring.st[stage == 0 ? CSC_STAGES - 1 : stage - 1];
+    issue(ahead, free_stage);
+    // decays of a row; computed one row ahead of their use, so that the exp
+    // unit works while the row before is summed
+    struct Decay {
+      float2 e[2][4];
+      float2 u, d;
+    };
+    auto decay = [&](int r, Decay& k) {
+      k.u = ld_pair(&st.u[r][pc]);
+      k.d = ld_pair(&st.dl[r][pc]);
+      const float2 dlog = mul2(k.d, bcast2(kLog2e)), off = bcast2(kEx2ArgBias);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float2 dg = bcast2(c ? dlog.y : dlog.x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 arg = fma2(dg, A2[c][j], off);
+          k.e[c][j] = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+        }
+      }
+    };
+    auto row = [&](int r, const Decay& k) {
+      const float2 du = mul2(k.d, k.u);
+      if (CARRY) dsum = add2(dsum, k.d);
+      const float* s = bc + r * 32 + 8 * hb;
+      const float4 b0 = lds4(s), b1 = lds4(s + 4);
+      const float2 B2[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y),
+                            make_float2(b1.z, b1.w)};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float2 db = bcast2(c ? du.y : du.x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[c][j] = fma2(k.e[c][j], h[c][j], mul2(db, B2[j]));
+      }
+      if (!CARRY) {
+        const float4 e0 = lds4(s + NS), e1 = lds4(s + NS + 4);
+        const float2 C2[4] = {make_float2(e0.x, e0.y), make_float2(e0.z, e0.w), make_float2(e1.x, e1.y),
+                              make_float2(e1.z, e1.w)};
+        float part[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float2 acc =
+              add2(fma2(C2[1], h[c][1], mul2(C2[0], h[c][0])), fma2(C2[3], h[c][3], mul2(C2[2], h[c][2])));
+          part[c] = acc.x + acc.y;
+        }
+        float yy = fmaf(hb ? k.u.y : k.u.x, Dd, pair_scatter(part[0], part[1], hb));
+        if (HAS_Z) yy *= silu_f(ld_one(&st.z[r][lane]));
+        // an explicit global store: a generic one could alias the ring, and would keep the next row's
+        // shared loads behind it
+        stg_if_t<T>(y + (t0 + r) * a.ldy, yy, ok);
+      }
+    };
     const int nr = min(CSC_ROWS, p.t1 - t0);
-    float uv[CSC_ROWS], dv[CSC_ROWS], zv[CSC_ROWS];
+    Decay ka, kb;
+    decay(0, ka);
+    if (nr == CSC_ROWS) {
 #pragma unroll
-    for (int r = 0; r < CSC_ROWS; ++r) {
-      const int64_t t = min(t0 + r, p.t1 - 1);
-      uv[r] = ld_one(u + t * a.ldu);
-      dv[r] = ld_one(dl + t * a.ldd);
-      if (HAS_Z && !CARRY) zv[r] = ld_one(z + t * a.ldz);
-    }
-    __syncwarp();
-    if (brow < nr) {
-      const T* pb = static_cast<const T*>(a.B) + (t0 + brow) * a.ldb + bcol;
-      const T* pc = static_cast<const T*>(a.C) + (t0 + brow) * a.ldc + bcol;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        bc[warp][brow][bcol + k] = ld_one(pb + k);
-        if (!CARRY) bc[warp][brow][NS + bcol + k] = ld_one(pc + k);
+      for (int r = 0; r < CSC_ROWS; ++r) {
+        if (r + 1 < CSC_ROWS) decay(r + 1, kb);
+        row(r, ka);
+        ka = kb;
+      }
+    } else {
+      for (int r = 0; r < nr; ++r) {
+        row(r, ka);
+        if (r + 1 < nr) decay(r + 1, ka);
       }
     }
-    __syncwarp();
-#pragma unroll
-    for (int r = 0; r < CSC_ROWS; ++r) {
-      if (r < nr) {
-        const float2 du = bcast2(dv[r] * uv[r]), dlog = bcast2(dv[r] * kLog2e), off = bcast2(kEx2ArgBias);
-        if (CARRY) dsum += dv[r];
-        float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 arg = fma2(dlog, A2[j], off);
-          const float2 e = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
-          h[j] = fma2(e, h[j], mul2(du, lds2(&bc[warp][r][2 * j])));
-          if (!CARRY) {
-            const float2 c2 = lds2(&bc[warp][r][NS + 2 * j]);
-            if (j & 1)
-              acc1 = fma2(c2, h[j], acc1);
-            else
-              acc0 = fma2(c2, h[j], acc0);
-          }
-        }
-        if (!CARRY) {
-          const float2 acc = add2(acc0, acc1);
-          float yy = fmaf(uv[r], Dd, acc.x + acc.y);
-          if (HAS_Z) yy *= silu_f(zv[r]);
-          if (ok) y[(t0 + r) * a.ldy] = from_f<T>(yy);
-        }
-      }
-    }
+    settle(ahead, free_stage);
+    stage = stage + 1 == CSC_STAGES ? 0 : stage + 1;
   }
-  if (!ok) return;
   float* dst = nullptr;
   if (CARRY) {
-    dst = carry_h + (int64_t(p.carry) * a.dn + d) * NS;
-    carry_s[int64_t(p.carry) * a.dn + d] = dsum;
+    dst = carry_h + int64_t(p.carry) * a.dn * NS;
+    if (ok) carry_s[int64_t(p.carry) * a.dn + own] = hb ? dsum.y : dsum.x;
   } else if (p.t1 == p.end) {
-    dst = a.state + (int64_t(p.slot) * a.dn + d) * NS;
+    dst = a.state + int64_t(p.slot) * a.dn * NS;
   }
-  if (dst != nullptr) {
+  if (dst == nullptr) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4*>(dst + 4 * j) = make_float4(h[2 * j].x, h[2 * j].y, h[2 * j + 1].x, h[2 * j + 1].y);
-  }
+  for (int c = 0; c < 2; ++c)
+    if (dp + c < a.dn) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<float4*>(dst + int64_t(dp + c) * NS + 8 * hb + 4 * j) =
+            make_float4(h[c][2 * j].x, h[c][2 * j].y, h[c][2 * j + 1].x, h[c][2 * j + 1].y);
+    }
 }
 
 // State entering every piece of the split requests: chain i =
@@ -286,6 +454,7 @@ __global__ void __launch_bounds__(CST_WARPS * 32)
 constexpr int CCV_ROWS = 32;
 constexpr int CCV_THREADS = 64;
 constexpr int CCV_KMAX = 8;
+constexpr int CCV_AHEAD = 8;  // rows whose loads are issued together
 
 template <typename T, int VEC>
 __device__ __forceinline__ void ldv(const T* p, float v[VEC]) {
@@ -326,39 +495,48 @@ struct CachedConvArgs {
   int rows, channels, K;
 };
 
-template <typename T, int VEC>
+// KW: window slots (4 or 8, at least K); the K taps sit at the newest end.
+template <typename T, int VEC, int KW>
 __global__ void __launch_bounds__(CCV_THREADS)
     cached_conv_kernel(const CachedConvArgs a, const int32_t* __restrict__ pieces, int groups) {
   const Piece p = load_piece(pieces, blockIdx.x / groups, a.rows, a.n_slots);
   const int c = ((blockIdx.x % groups) * CCV_THREADS + threadIdx.x) * VEC;
   if (c >= a.channels) return;
   const int K = a.K;
-  T* out = static_cast<T*>(a.out) + c;
+  T* __restrict__ out = static_cast<T*>(a.out) + c;
   if (p.slot < 0) {
     const float zero[VEC] = {};
     for (int t = p.t0; t < p.t1; ++t) stv<T, VEC>(out + t * a.ldo, zero);
     return;
   }
-  const T* x = static_cast<const T*>(a.x) + c;
+  const T* __restrict__ x = static_cast<const T*>(a.x) + c;
   T* state = static_cast<T*>(a.state) + c;
   const int64_t C = a.channels;
-  float w[CCV_KMAX][VEC], win[CCV_KMAX][VEC], bias[VEC];
-#pragma unroll
-  for (int m = 0; m < CCV_KMAX; ++m) {
-    const int k = m - (CCV_KMAX - K);  // tap of window slot m: the K taps sit at the newest end
+  float w[KW][VEC], win[KW][VEC], bias[VEC];
+  if (KW == 4 && K == 4) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      w[m][v] = k >= 0 ? a.w[int64_t(c + v) * K + k] : 0.f;
-      win[m][v] = 0.f;
+      const float4 q = *reinterpret_cast<const float4*>(a.w + int64_t(c + v) * 4);
+      w[0][v] = q.x, w[1][v] = q.y, w[KW - 2][v] = q.z, w[KW - 1][v] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < KW; ++m) {
+      const int k = m - (KW - K);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) w[m][v] = k >= 0 ? a.w[int64_t(c + v) * K + k] : 0.f;
     }
   }
 #pragma unroll
   for (int v = 0; v < VEC; ++v) bias[v] = a.bias[c + v];
-  // rows before the piece: rows of the request, or of the stored window
+  // rows before the piece: rows of the request, or of the stored window.  Slot
+  // m is row t0 - (KW - m) before the first shift.
 #pragma unroll
-  for (int m = 1; m < CCV_KMAX; ++m) {
-    const int t = p.t0 - (CCV_KMAX - m);  // row of window slot m before the first shift
-    if (CCV_KMAX - m < K) {
+  for (int m = 0; m < KW; ++m) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) win[m][v] = 0.f;
+    const int t = p.t0 - (KW - m);
+    if (m > 0 && KW - m < K) {
       if (t >= p.begin)
         ldv<T, VEC>(x + t * a.ldx, win[m]);
       else if (p.source >= 0)
@@ -367,43 +545,50 @@ __global__ void __launch_bounds__(CCV_THREADS)
   }
   if (p.t0 == p.begin) {
     // the new window: its row j is row end - (K - 1) + j of the request, and
-    // where that lies before the request, the old window's row j + length
-    // (read above: slot m of win is row begin - (CCV_KMAX - m))
+    // where that lies before the request, the old window's (read above: slot s
+    // is row begin - (KW - s))
     const int len = p.end - p.begin;
 #pragma unroll
-    for (int m = 1; m < CCV_KMAX; ++m) {
-      const int j = K - 1 - (CCV_KMAX - m);
+    for (int m = 1; m < KW; ++m) {
+      const int j = K - 1 - (KW - m);
       if (j >= 0) {
         float v[VEC] = {};
-        const int t = p.end - (CCV_KMAX - m);
+        const int t = p.end - (KW - m);
         if (t >= p.begin) {
           ldv<T, VEC>(x + t * a.ldx, v);
         } else {
 #pragma unroll
-          for (int s = 1; s < CCV_KMAX; ++s)
-            if (s == m + len)
+          for (int s = m; s < KW; ++s)
+            if (s == m + len) {
 #pragma unroll
               for (int q = 0; q < VEC; ++q) v[q] = win[s][q];
+            }
         }
         stv<T, VEC>(state + (int64_t(p.slot) * (K - 1) + j) * C, v);
       }
     }
   }
-  for (int t = p.t0; t < p.t1; ++t) {
+  for (int t0 = p.t0; t0 < p.t1; t0 += CCV_AHEAD) {
+    float xs[CCV_AHEAD][VEC];
 #pragma unroll
-    for (int m = 0; m < CCV_KMAX - 1; ++m)
+    for (int u = 0; u < CCV_AHEAD; ++u) ldv<T, VEC>(x + min(t0 + u, p.t1 - 1) * a.ldx, xs[u]);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) win[m][v] = win[m + 1][v];
-    ldv<T, VEC>(x + t * a.ldx, win[CCV_KMAX - 1]);
-    float acc[VEC];
+    for (int u = 0; u < CCV_AHEAD; ++u) {
+      if (t0 + u < p.t1) {
+        float acc[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      acc[v] = bias[v];
+        for (int v = 0; v < VEC; ++v) {
 #pragma unroll
-      for (int m = 0; m < CCV_KMAX; ++m) acc[v] = fmaf(w[m][v], win[m][v], acc[v]);
-      acc[v] = silu_f(acc[v]);
+          for (int m = 0; m < KW - 1; ++m) win[m][v] = win[m + 1][v];
+          win[KW - 1][v] = xs[u][v];
+          acc[v] = bias[v];
+#pragma unroll
+          for (int m = 0; m < KW; ++m) acc[v] = fmaf(w[m][v], win[m][v], acc[v]);
+          acc[v] = silu_f(acc[v]);
+        }
+        stv<T, VEC>(out + (t0 + u) * a.ldo, acc);
+      }
     }
-    stv<T, VEC>(out + t * a.ldo, acc);
   }
 }
 

@@ -4,17 +4,32 @@
 //
 // The host sorts the rows by adapter and cuts them into tiles of at most
 // LORA_ROWS rows of one adapter (int32[4] records: first entry of the row
-// list, entries, adapter or -1, 0).  A CTA forms the tile's rank-wide products
-// in fp32 in shared memory and expands them into its share of the columns.
+// list, entries, adapter or -1, 0).  One CTA owns a tile and a share of the
+// output columns: its warps split d_in and form partial products
+// S = x A^T (rows x rank), which are added in shared memory in a fixed order,
+// and then split the columns for out = base + S B^T.  Nothing but base, x and
+// out crosses HBM; the rank-wide S never leaves the SM.
+//
+// Both products run on mma.sync (a tile has a few rows of one adapter and a
+// rank of 4 to 64: far too little work per operand byte for tcgen05 to matter;
+// the kernel is bound by the bytes of base and out).  Operands go from global
+// memory straight to fragments: the order of a product's inner index is free,
+// so a lane's four (fp32) or eight (bf16) adjacent elements stand for the
+// inner indices that its fragment registers hold, on both operands alike, and
+// every access is a 16-byte one.
+//   fp32: TF32 hi / lo parts, hi hi + hi lo + lo hi, fp32 accumulators.
+//   bf16: x, A, B are exact operands; S enters the second product as three
+//         bf16 parts (24 bits).  The output is rounded once.
 #pragma once
 
 #include "vmscan_common.cuh"
 
 namespace vmscan {
 
-constexpr int LORA_ROWS = 16;
-constexpr int LORA_THREADS = 128;
+constexpr int LORA_ROWS = 32;
+constexpr int LORA_WARPS = 4;
 constexpr int LORA_RMAX = 128;
+constexpr int LORA_RCHUNK = 32;  // rank columns whose partial products a warp holds at a time
 
 struct LoraArgs {
   const void* x;
@@ -27,60 +42,346 @@ struct LoraArgs {
   const int32_t* tiles;
   int64_t ldx, ldbase, ldout;
   int rows, d_in, d_out, rank, adapters, n_index;
+  int wide_in, wide_rank, wide_out;  // 16-byte (x, A), 4-element (B), 4-element (base, out) accesses fit
 };
 
+__device__ __forceinline__ void mma_tf32(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Sixteen bytes of a row from column c on, zero past `limit`.
 template <typename T>
-__global__ void __launch_bounds__(LORA_THREADS) lora_add_kernel(const LoraArgs a, int cols_per_cta) {
-  __shared__ float s[LORA_ROWS][LORA_RMAX];
+struct Chunk {
+  static constexpr int N = 16 / int(sizeof(T));
+  uint32_t w[4];
+};
+template <typename T>
+__device__ __forceinline__ Chunk<T> ld_chunk(const T* row, int c, int limit, bool wide) {
+  Chunk<T> k;
+  if (wide) {  // limit is a multiple of N: a chunk is inside or outside
+    const uint4 q = c < limit ? __ldg(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
+    k.w[0] = q.x, k.w[1] = q.y, k.w[2] = q.z, k.w[3] = q.w;
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k.w[i] = c + i < limit ? __float_as_uint(row[c + i]) : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = c + 2 * i < limit ? __bfloat16_as_ushort(row[c + 2 * i]) : 0;
+      const uint32_t hi = c + 2 * i + 1 < limit ? __bfloat16_as_ushort(row[c + 2 * i + 1]) : 0;
+      k.w[i] = lo | hi << 16;
+    }
+  }
+  return k;
+}
+
+// Four elements of a row from column c on as they lie in memory (fp32: 4
+// words, bf16: 2), zero past `limit`.
+template <typename T>
+struct Four {
+  uint32_t w[sizeof(T)];
+};
+// Ordinary loads (base may be the output: no read-only path), which the
+// compiler may still move across the stores of other columns.
+template <typename T>
+__device__ __forceinline__ Four<T> ld_quad(const T* row, int c, int limit, bool wide) {
+  Four<T> k;
+  if constexpr (sizeof(T) == 4) {
+    if (wide) {
+      k.w[0] = k.w[1] = k.w[2] = k.w[3] = 0;
+      if (c < limit)
+        asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+            : "=r"(k.w[0]), "=r"(k.w[1]), "=r"(k.w[2]), "=r"(k.w[3])
+            : "l"(row + c));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k.w[i] = c + i < limit ? __float_as_uint(row[c + i]) : 0u;
+    }
+  } else {
+    if (wide) {
+      k.w[0] = k.w[1] = 0;
+      if (c < limit) asm("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(k.w[0]), "=r"(k.w[1]) : "l"(row + c));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t lo = c + 2 * i < limit ? __bfloat16_as_ushort(row[c + 2 * i]) : 0;
+        const uint32_t hi = c + 2 * i + 1 < limit ? __bfloat16_as_ushort(row[c + 2 * i + 1]) : 0;
+        k.w[i] = lo | hi << 16;
+      }
+    }
+  }
+  return k;
+}
+
+template <typename T>
+__device__ __forceinline__ float4 four_f(const Four<T>& k) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float4(__uint_as_float(k.w[0]), __uint_as_float(k.w[1]), __uint_as_float(k.w[2]),
+                       __uint_as_float(k.w[3]));
+  } else {
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&k.w[0]));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&k.w[1]));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void st_quad(T* row, int c, int limit, bool wide, const float4& v) {
+  if constexpr (sizeof(T) == 4) {
+    if (wide) {
+      if (c < limit) *reinterpret_cast<float4*>(row + c) = v;
+      return;
+    }
+    if (c < limit) row[c] = v.x;
+    if (c + 1 < limit) row[c + 1] = v.y;
+    if (c + 2 < limit) row[c + 2] = v.z;
+    if (c + 3 < limit) row[c + 3] = v.w;
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    if (wide) {
+      uint2 q;
+      q.x = *reinterpret_cast<const uint32_t*>(&a);
+      q.y = *reinterpret_cast<const uint32_t*>(&b);
+      if (c < limit) *reinterpret_cast<uint2*>(row + c) = q;
+      return;
+    }
+    if (c < limit) row[c] = a.x;
+    if (c + 1 < limit) row[c + 1] = a.y;
+    if (c + 2 < limit) row[c + 2] = b.x;
+    if (c + 3 < limit) row[c + 3] = b.y;
+  }
+}
+
+__device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return (x + 0x1000u) & 0xFFFFE000u; }
+__device__ __forceinline__ uint32_t tf32_lo(uint32_t x, uint32_t hi) {
+  return __float_as_uint(tf32_round(__uint_as_float(x) - __uint_as_float(hi)));
+}
+
+// Fragments of S for 16 rank columns and one 16-row block, as groups of four
+// words a lane: fp32 two steps of hi and two of lo, bf16 three parts.
+template <typename T>
+struct LoraFrag {
+  static constexpr int GROUPS = sizeof(T) == 4 ? 4 : 3;
+};
+template <typename T>
+constexpr size_t lora_smem(int rank) {
+  return (size_t(LORA_WARPS) * LORA_ROWS * (LORA_RCHUNK + 1) +
+          size_t(2) * ((rank + 15) / 16) * 32 * 4 * LoraFrag<T>::GROUPS) * 4;
+}
+
+// MT: 16-row blocks of the tile in use.
+template <typename T, int MT>
+__device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int n, int ad, int c_begin, int c_end,
+                                          float* part, uint32_t* frag) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int CN = Chunk<T>::N;
+  int r[2 * MT];  // rows g, g + 8, ... of the tile; those past the last repeat it
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) r[i] = row[min(g + 8 * i, n - 1)];
+  const int steps = (a.rank + 15) / 16;
+  if (ad >= 0) {
+    const T* A = static_cast<const T*>(a.a) + int64_t(ad) * a.rank * a.d_in;
+    const float scale = a.scale[ad];
+    for (int rc = 0; rc < a.rank; rc += LORA_RCHUNK) {
+      float acc[MT][4][4] = {};
+      const int nt = min(4, (a.rank - rc + 7) / 8);  // 8-column blocks of this chunk
+#pragma unroll 2
+      for (int c = (warp * 4 + t) * CN; c - t * CN < a.d_in; c += LORA_WARPS * 4 * CN) {
+        Chunk<T> x[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)
+          x[i] = ld_chunk(static_cast<const T*>(a.x) + r[i] * a.ldx, c, a.d_in, a.wide_in != 0);
+        uint32_t xl[2 * MT][4];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t hi = tf32_hi(x[i].w[k]);
+              xl[i][k] = tf32_lo(x[i].w[k], hi);
+              x[i].w[k] = hi;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j < nt) {
+            const int k = rc + 8 * j + g;
+            Chunk<T> b{};
+            if (k < a.rank) b = ld_chunk(A + int64_t(k) * a.d_in, c, a.d_in, a.wide_in != 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // words 2h and 2h + 1 of the chunk are one step of the product
+              uint32_t bh[2] = {b.w[2 * h], b.w[2 * h + 1]}, bl[2];
+              if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const uint32_t hi = tf32_hi(bh[q]);
+                  bl[q] = tf32_lo(bh[q], hi);
+                  bh[q] = hi;
+                }
+              }
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const uint32_t xa[4] = {x[2 * m].w[2 * h], x[2 * m + 1].w[2 * h], x[2 * m].w[2 * h + 1],
+                                        x[2 * m + 1].w[2 * h + 1]};
+                if constexpr (sizeof(T) == 4) {
+                  const uint32_t la[4] = {xl[2 * m][2 * h], xl[2 * m + 1][2 * h], xl[2 * m][2 * h + 1],
+                                          xl[2 * m + 1][2 * h + 1]};
+                  mma_tf32(acc[m][j], la, bh[0], bh[1]);
+                  mma_tf32(acc[m][j], xa, bl[0], bl[1]);
+                  mma_tf32(acc[m][j], xa, bh[0], bh[1]);
+                } else {
+                  mma_bf16(acc[m][j], xa, bh[0], bh[1]);
+                }
+              }
+            }
+          }
+        }
+      }
+      // partial products of the warps, then their sum in a fixed order as the
+      // fragments of the second product
+      constexpr int LD = LORA_RCHUNK + 1;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < nt) {
+            float* p = part + (warp * LORA_ROWS + 16 * m + g) * LD + 8 * j + 2 * t;
+            p[0] = acc[m][j][0];
+            p[1] = acc[m][j][1];
+            p[8 * LD] = acc[m][j][2];
+            p[8 * LD + 1] = acc[m][j][3];
+          }
+      __syncthreads();
+      const int here = min(2, steps - rc / 16);  // 16-column steps of this chunk
+      for (int e = threadIdx.x; e < MT * here * 32; e += LORA_WARPS * 32) {
+        const int fl = e & 31, s = (e >> 5) % here, m = (e >> 5) / here;
+        const int fr = 16 * m + (fl >> 2), fc = 16 * s + 4 * (fl & 3);
+        float v[2][4];  // rows fr, fr + 8; columns fc .. fc + 3
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float sum = 0.f;
+            if (rc + fc + q < a.rank) {
+#pragma unroll
+              for (int w = 0; w < LORA_WARPS; ++w) sum += part[(w * LORA_ROWS + fr + 8 * i) * LD + fc + q];
+            }
+            v[i][q] = scale * sum;
+          }
+        uint32_t* f = frag + (size_t(m * steps + rc / 16 + s) * LoraFrag<T>::GROUPS * 32 + fl) * 4;
+        if constexpr (sizeof(T) == 4) {
+          // groups 0, 1: hi of step h = 0, 1 (columns fc + 2h, fc + 2h + 1); 2, 3: lo
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t x = __float_as_uint(v[q & 1][2 * h + (q >> 1)]), hi = tf32_hi(x);
+              f[128 * h + q] = hi;
+              f[128 * (2 + h) + q] = tf32_lo(x, hi);
+            }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float x0 = v[q & 1][2 * (q >> 1)], x1 = v[q & 1][2 * (q >> 1) + 1];
+#pragma unroll
+            for (int w = 0; w < 3; ++w) {
+              const __nv_bfloat162 b2 = __floats2bfloat162_rn(x0, x1);
+              f[128 * w + q] = *reinterpret_cast<const uint32_t*>(&b2);
+              const float2 back = __bfloat1622float2(b2);
+              x0 -= back.x;
+              x1 -= back.y;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  // columns in groups of 16: lane t of a quad owns columns 4t .. 4t + 3 of its
+  // rows, which are columns 2t, 2t + 1 of the group's two 8-column blocks
+  const T* B = static_cast<const T*>(a.b) + int64_t(max(ad, 0)) * a.d_out * a.rank;
+#pragma unroll 2
+  for (int c0 = c_begin + 16 * warp; c0 < c_end; c0 += 16 * LORA_WARPS) {
+    Four<T> base[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i)
+      base[i] = ld_quad(static_cast<const T*>(a.base) + r[i] * a.ldbase, c0 + 4 * t, a.d_out, a.wide_out != 0);
+    float acc[MT][2][4] = {};
+    if (ad >= 0) {
+      for (int s = 0; s < steps; ++s) {
+        Four<T> b[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = c0 + 4 * (g >> 1) + (g & 1) + 2 * j;
+          b[j] = Four<T>{};
+          if (col < a.d_out) b[j] = ld_quad(B + int64_t(col) * a.rank, 16 * s + 4 * t, a.rank, a.wide_rank != 0);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint4* f = reinterpret_cast<const uint4*>(frag) + size_t(m * steps + s) * LoraFrag<T>::GROUPS * 32 + lane;
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 fh = f[32 * h], fl = f[32 * (2 + h)];
+              const uint32_t sh[4] = {fh.x, fh.y, fh.z, fh.w}, sl[4] = {fl.x, fl.y, fl.z, fl.w};
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t h0 = tf32_hi(b[j].w[2 * h]), h1 = tf32_hi(b[j].w[2 * h + 1]);
+                mma_tf32(acc[m][j], sl, h0, h1);
+                mma_tf32(acc[m][j], sh, tf32_lo(b[j].w[2 * h], h0), tf32_lo(b[j].w[2 * h + 1], h1));
+                mma_tf32(acc[m][j], sh, h0, h1);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int w = 2; w >= 0; --w) {
+              const uint4 fw = f[32 * w];
+              const uint32_t sw[4] = {fw.x, fw.y, fw.z, fw.w};
+#pragma unroll
+              for (int j = 0; j < 2; ++j) mma_bf16(acc[m][j], sw, b[j].w[0], b[j].w[1]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const float4 v = four_f(base[i]);
+      const float* p0 = &acc[i >> 1][0][2 * (i & 1)];
+      const float* p1 = &acc[i >> 1][1][2 * (i & 1)];
+      if (g + 8 * i < n)
+        st_quad(static_cast<T*>(a.out) + r[i] * a.ldout, c0 + 4 * t, a.d_out, a.wide_out != 0,
+                make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]));
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LORA_WARPS * 32) lora_add_kernel(const LoraArgs a, int cols_per_cta) {
+  extern __shared__ __align__(16) unsigned char lora_raw[];
   __shared__ int row[LORA_ROWS];
+  float* part = reinterpret_cast<float*>(lora_raw);
+  uint32_t* frag = reinterpret_cast<uint32_t*>(part + LORA_WARPS * LORA_ROWS * (LORA_RCHUNK + 1));
   const int4 tile = reinterpret_cast<const int4*>(a.tiles)[blockIdx.x];
   const int first = max(tile.x, 0);
   const int n = min(min(tile.y, LORA_ROWS), a.n_index - first);
   if (n <= 0) return;
   const int ad = tile.z < a.adapters ? tile.z : -1;
   if (ad < 0 && a.out == a.base) return;
-  for (int i = threadIdx.x; i < n; i += LORA_THREADS) row[i] = min(max(a.row_index[first + i], 0), a.rows - 1);
+  for (int i = threadIdx.x; i < n; i += LORA_WARPS * 32) row[i] = min(max(a.row_index[first + i], 0), a.rows - 1);
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = blockIdx.y * cols_per_cta, c1 = min(c0 + cols_per_cta, a.d_out);
-  if (ad >= 0) {
-    const T* A = static_cast<const T*>(a.a) + int64_t(ad) * a.rank * a.d_in;
-    const float scale = a.scale[ad];
-    for (int i = warp; i < n * a.rank; i += LORA_THREADS / 32) {
-      const int r = i / a.rank, k = i % a.rank;
-      const T* x = static_cast<const T*>(a.x) + row[r] * a.ldx;
-      float acc = 0.f;
-      for (int j = lane; j < a.d_in; j += 32) acc = fmaf(ld_one(x + j), ld_one(A + int64_t(k) * a.d_in + j), acc);
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-      if (lane == 0) s[r][k] = scale * acc;
-    }
-  }
-  __syncthreads();
-  for (int c = c0 + threadIdx.x; c < c1; c += LORA_THREADS) {
-    float acc[LORA_ROWS];
-#pragma unroll
-    for (int r = 0; r < LORA_ROWS; ++r)
-      acc[r] = r < n ? ld_one(static_cast<const T*>(a.base) + row[r] * a.ldbase + c) : 0.f;
-    if (ad >= 0) {
-      const T* B = static_cast<const T*>(a.b) + (int64_t(ad) * a.d_out + c) * a.rank;
-      for (int k = 0; k < a.rank; ++k) {
-        const float bk = ld_one(B + k);
-#pragma unroll
-        for (int r = 0; r < LORA_ROWS; ++r)
-          if (r < n) acc[r] = fmaf(s[r][k], bk, acc[r]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < LORA_ROWS; ++r)
-      if (r < n) {
-        T* o = static_cast<T*>(a.out) + row[r] * a.ldout + c;
-        if constexpr (sizeof(T) == 4)
-          *o = acc[r];
-        else
-          *o = __float2bfloat16_rn(acc[r]);
-      }
-  }
+  if (n > 16)
+    lora_tile<T, 2>(a, row, n, ad, c0, c1, part, frag);
+  else
+    lora_tile<T, 1>(a, row, n, ad, c0, c1, part, frag);
 }
 
 }  // namespace vmscan

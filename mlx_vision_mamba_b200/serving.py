@@ -26,7 +26,6 @@ There is no CPU path: inputs must be CUDA tensors and libvmscan.so must load.
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Sequence
 
 import numpy as np
@@ -100,6 +99,7 @@ class RequestBatch:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device() if torch.cuda.is_available() else 0)
+        self.index = -2 if self.device.type != "cuda" else self.device.index
         self.single_tokens = bool((self.lengths == 1).all())
         self._tables = {}
         self._set(slots if slots is not None else np.arange(self.count), sources, adapters)
@@ -162,9 +162,7 @@ class RequestBatch:
                              "vmscan_lora_tiles")
             return _pinned(table), (int(most),)
         if kind == "scan":
-            with _device_guard(self.device):
-                rows = lib.vmscan_cached_scan_rows(self.count, ptr(self.lengths), arg)
-            by_length = 1
+            rows, by_length = lib.vmscan_cached_scan_rows(self.count, ptr(self.lengths), arg), 1
         else:
             rows, by_length = lib.vmscan_cached_conv_rows(), 0
         if rows < 0:
@@ -176,11 +174,12 @@ class RequestBatch:
         _check_count(lib.vmscan_request_pieces(*args, ptr(table), table.size, ptr(info)), "vmscan_request_pieces")
         return _pinned(table), (int(n), int(info[0]), int(info[1]), int(info[2]))
 
-    def _table(self, kind: str, arg: int = 0) -> _Table:
-        """The device table of a kind for the current stream."""
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+    def _table(self, kind: str, stream: int, arg: int = 0) -> _Table:
+        """The device table of a kind for a stream (the current one)."""
         key = (kind, arg, stream)
         table = self._tables.get(key)
+        if table is not None and not (table.captured or _capturing()):
+            return table
         if _capturing():
             # any stream's table will do: capture starts after a device-wide
             # synchronisation, so its upload has completed
@@ -189,8 +188,7 @@ class RequestBatch:
             if table is None:
                 raise RuntimeError("RequestBatch: call the operator once with this batch before capturing it")
             table.captured = True
-            return table
-        if table is None:
+        elif table is None:
             host, info = self._build(key)
             table = _Table(host.to(self.device, non_blocking=True), host, info)
             self._tables[key] = table
@@ -203,31 +201,22 @@ def _check_count(n: int, where: str) -> int:
     return int(n)
 
 
+_CUDA_BUILD = hasattr(torch._C, "_cuda_isCurrentStreamCapturing")
+
+
 def _capturing() -> bool:
-    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+    return _CUDA_BUILD and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _stream_of(index: int) -> int:
+    """The current stream of a device as an integer handle.  (The Stream object
+    of torch.cuda.current_stream takes 3 us to make, a quarter of a small call.)"""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _pinned(a: np.ndarray) -> torch.Tensor:
     t = torch.from_numpy(a)
     return t.pin_memory() if torch.cuda.is_available() and a.size else t
-
-
-class _device_guard:
-    """Makes `device` current for the calls inside (launches and workspaces go
-    to the device that owns the tensors); nothing when it already is."""
-
-    def __init__(self, device: torch.device):
-        self.index = device.index if device.type == "cuda" else None
-        self.previous = None
-
-    def __enter__(self):
-        if self.index is not None and torch.cuda.is_available() and torch.cuda.current_device() != self.index:
-            self.previous = torch.cuda.current_device()
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.previous is not None:
-            torch.cuda.set_device(self.previous)
 
 
 class LoraAdapters:
@@ -262,12 +251,13 @@ class LoraAdapters:
         self.scale = scale.detach().to(a.device).contiguous()
 
 
-def _refuse_grad(where: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{where}: a serving operator has no gradient; call it under torch.no_grad()")
+# The operators' small calls are bound by the host, so each tests all that a good
+# call satisfies in one expression; only when that fails are the conditions gone
+# through one by one to say which it was.
 
 
-def _check_batch(where: str, batch: RequestBatch, x: torch.Tensor) -> None:
+def _refuse_batch(where: str, batch, x) -> None:
+    """Raises what is wrong with a batch and the rows it is used on."""
     if not isinstance(batch, RequestBatch):
         raise TypeError(f"{where}: `batch` must be a RequestBatch, got {type(batch).__name__}")
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
@@ -280,48 +270,66 @@ def _check_batch(where: str, batch: RequestBatch, x: torch.Tensor) -> None:
         raise TypeError(f"{where}: x must be fp32 or bf16, got {x.dtype}")
     if x.shape[0] < batch.tokens:
         raise ValueError(f"{where}: x has {x.shape[0]} rows, the batch's requests have {batch.tokens}")
-    if x.shape[0] > _MAX_ROWS:
-        raise ValueError(f"{where}: x has {x.shape[0]} rows (at most {_MAX_ROWS})")
+    raise ValueError(f"{where}: x has {x.shape[0]} rows (at most {_MAX_ROWS})")
+
+
+def _batch_ok(batch, x) -> bool:
+    return (isinstance(batch, RequestBatch) and isinstance(x, torch.Tensor) and x.is_cuda
+            and x.get_device() == batch.index and x.dim() == 2 and x.dtype in _DTYPES
+            and batch.tokens <= x.shape[0] <= _MAX_ROWS)
+
+
+def _refuse_tensors(where: str, x, named) -> None:
+    """Raises for the first of (name, tensor, shape) that is no CUDA tensor of
+    that shape on x's device."""
+    for name, t, shape in named:
+        if not isinstance(t, torch.Tensor) or t.device != x.device:
+            raise RuntimeError(f"{where}: `{name}` must be a CUDA tensor on x's device (there is no CPU path)")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{where}: {name} must be {shape}, got {tuple(t.shape)}")
+
+
+def _refuse_grad(where: str) -> None:
+    raise RuntimeError(f"{where}: a serving operator has no gradient; call it under torch.no_grad()")
+
+
+def _check_state(where: str, state, tail, dtype: torch.dtype, batch: RequestBatch) -> None:
+    if (isinstance(state, torch.Tensor) and state.get_device() == batch.index and state.dim() == 3
+            and state.shape[1:] == tail and state.dtype is dtype and state.is_contiguous()
+            and batch.max_slot < state.shape[0] and state.data_ptr() % 16 == 0):
+        return
+    if not isinstance(state, torch.Tensor) or state.device != batch.device:
+        raise RuntimeError(f"{where}: `state` must be a CUDA tensor on x's device")
+    if state.dim() != 3 or tuple(state.shape[1:]) != tail or state.dtype != dtype:
+        raise ValueError(f"{where}: state must be (slots, {tail[0]}, {tail[1]}) {dtype}, got {tuple(state.shape)} "
+                         f"{state.dtype}")
+    if batch.max_slot >= state.shape[0]:
+        raise ValueError(f"{where}: the batch uses slot {batch.max_slot}, the state has {state.shape[0]} slots")
+    raise ValueError(f"{where}: state must be contiguous and 16-byte aligned (it is updated in place)")
 
 
 def _rows(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """t (rows, columns) in `dtype` with unit column stride (a view when it is so)."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         t = t.to(dtype)
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def _param(t: torch.Tensor) -> torch.Tensor:
-    """An fp32 parameter, contiguous and 16-byte aligned."""
-    t = t.detach()
-    if t.dtype != torch.float32:
-        t = t.float()
-    t = t.contiguous()
+    """A parameter as contiguous, 16-byte aligned fp32."""
+    if t.dtype is torch.float32 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    t = t.detach().float().contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _check_state(where: str, state, x: torch.Tensor, tail, dtype: torch.dtype, batch: RequestBatch) -> None:
-    if not isinstance(state, torch.Tensor) or state.device != x.device:
-        raise RuntimeError(f"{where}: `state` must be a CUDA tensor on x's device")
-    if state.dim() != 3 or tuple(state.shape[1:]) != tail or state.dtype != dtype:
-        raise ValueError(f"{where}: state must be (slots, {tail[0]}, {tail[1]}) {dtype}, got {tuple(state.shape)} "
-                         f"{state.dtype}")
-    if not state.is_contiguous() or (state.numel() and state.data_ptr() % 16):
-        raise ValueError(f"{where}: state must be contiguous and 16-byte aligned (it is updated in place)")
-    if batch.max_slot >= state.shape[0]:
-        raise ValueError(f"{where}: the batch uses slot {batch.max_slot}, the state has {state.shape[0]} slots")
 
 
 def _out_rows(x: torch.Tensor, columns: int, batch: RequestBatch) -> torch.Tensor:
     """Output rows; those behind the last request are zero."""
-    y = torch.empty((x.shape[0], columns), dtype=x.dtype, device=x.device)
-    if x.shape[0] > batch.tokens:
+    rows = x.shape[0]
+    y = x.new_empty((rows, columns))
+    if rows > batch.tokens:
         y[batch.tokens:].zero_()
     return y
-
-
-def _p(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
 
 
 def selective_scan_cached_cuda(x, delta, A, B, C, D, state, batch: RequestBatch,
@@ -342,46 +350,63 @@ def selective_scan_cached_cuda(x, delta, A, B, C, D, state, batch: RequestBatch,
     rounding where a long prompt is split for speed.
     """
     where = "selective_scan_cached_cuda"
-    _check_batch(where, batch, x)
+    if not _batch_ok(batch, x):
+        _refuse_batch(where, batch, x)
     rows, dn = x.shape
-    for name, t, shape in (("delta", delta, (rows, dn)), ("A", A, (dn, D_STATE)), ("B", B, (rows, D_STATE)),
-                           ("C", C, (rows, D_STATE)), ("D", D, (dn,)), ("z", z, (rows, dn))):
-        if t is None and name == "z":
-            continue
-        if not isinstance(t, torch.Tensor) or t.device != x.device:
-            raise RuntimeError(f"{where}: `{name}` must be a CUDA tensor on x's device (there is no CPU path)")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{where}: {name} must be {shape}, got {tuple(t.shape)}")
-    _check_state(where, state, x, (dn, D_STATE), torch.float32, batch)
-    _refuse_grad(where, x, delta, A, B, C, D, state, z)
+    index, shape, bc = batch.index, x.shape, (rows, D_STATE)
+    try:
+        good = (delta.shape == shape and A.shape == (dn, D_STATE) and B.shape == bc and C.shape == bc
+                and D.shape == (dn,) and (z is None or (z.shape == shape and z.get_device() == index))
+                and delta.get_device() == A.get_device() == B.get_device() == C.get_device() == D.get_device() == index)
+    except AttributeError:
+        good = False
+    if not good:
+        named = [("delta", delta, (rows, dn)), ("A", A, (dn, D_STATE)), ("B", B, bc), ("C", C, bc), ("D", D, (dn,))]
+        _refuse_tensors(where, x, named + ([("z", z, (rows, dn))] if z is not None else []))
+    _check_state(where, state, (dn, D_STATE), torch.float32, batch)
+    if torch.is_grad_enabled() and (x.requires_grad or delta.requires_grad or A.requires_grad or B.requires_grad
+                                    or C.requires_grad or D.requires_grad or state.requires_grad
+                                    or (z is not None and z.requires_grad)):
+        _refuse_grad(where)
     if dn == 0:
         return torch.zeros_like(x)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _scan_cached(x, delta, A, B, C, D, state, batch, z)
+    return _scan_cached(x, delta, A, B, C, D, state, batch, z)
+
+
+def _scan_cached(x, delta, A, B, C, D, state, batch, z):
     sd = x.dtype
     lib = _native.load()
-    with _device_guard(x.device):
-        x, delta, B, C = _rows(x, sd), _rows(delta, sd), _rows(B, sd), _rows(C, sd)
-        z = _rows(z, sd) if z is not None else None
-        A, D = _param(A), _param(D)
-        y = _out_rows(x, dn, batch)
-        stream = torch.cuda.current_stream().cuda_stream
-        head = (dn, D_STATE, int(sd == torch.bfloat16), _p(x), x.stride(0), _p(delta), delta.stride(0), _p(A), _p(B),
-                B.stride(0), _p(C), C.stride(0), _p(D), _p(z), z.stride(0) if z is not None else 0, _p(y), dn,
-                _p(state), state.shape[0])
-        if batch.single_tokens:
-            table = batch._table("step").tensor
-            _native.check(lib.vmscan_cached_step(batch.tokens, *head, _p(table), _p(table) + 4 * batch.count, stream),
-                          "vmscan_cached_step")
-            return y
-        table = batch._table("scan", dn)
-        n, n_carry, n_chains, carry_rows = table.info
-        ws, ws_n = None, 0
-        if carry_rows:
-            ws_n = _check_count(lib.vmscan_cached_scan_workspace_bytes(dn, carry_rows),
-                                "vmscan_cached_scan_workspace_bytes")
-            ws = torch.empty(ws_n, dtype=torch.uint8, device=x.device)
-        pieces = _p(table.tensor)
-        _native.check(lib.vmscan_cached_scan(rows, *head, pieces, n, n_carry, pieces + 32 * n if n_chains else None,
-                                             n_chains, carry_rows, _p(ws), ws_n, stream), "vmscan_cached_scan")
+    rows, dn = x.shape
+    x, delta, B, C = _rows(x, sd), _rows(delta, sd), _rows(B, sd), _rows(C, sd)
+    A, D = _param(A), _param(D)
+    zp, ldz = None, 0
+    if z is not None:
+        z = _rows(z, sd)
+        zp, ldz = z.data_ptr(), z.stride(0)
+    y = _out_rows(x, dn, batch)
+    stream = _stream_of(batch.index)
+    args = (dn, D_STATE, sd is torch.bfloat16, x.data_ptr(), x.stride(0), delta.data_ptr(), delta.stride(0),
+            A.data_ptr(), B.data_ptr(), B.stride(0), C.data_ptr(), C.stride(0), D.data_ptr(), zp, ldz, y.data_ptr(), dn,
+            state.data_ptr(), state.shape[0])
+    if batch.single_tokens:
+        table = batch._table("step", stream).tensor.data_ptr()
+        _native.check(lib.vmscan_cached_step(batch.tokens, *args, table, table + 4 * batch.count, stream),
+                      "vmscan_cached_step")
+        return y
+    table = batch._table("scan", stream, dn)
+    n, n_carry, n_chains, carry_rows = table.info
+    ws, ws_n = None, 0
+    if carry_rows:
+        ws_n = _check_count(lib.vmscan_cached_scan_workspace_bytes(dn, carry_rows),
+                            "vmscan_cached_scan_workspace_bytes")
+        ws = torch.empty(ws_n, dtype=torch.uint8, device=x.device)
+    pieces = table.tensor.data_ptr()
+    _native.check(lib.vmscan_cached_scan(rows, *args, pieces, n, n_carry, pieces + 32 * n if n_chains else None,
+                                         n_chains, carry_rows, None if ws is None else ws.data_ptr(), ws_n, stream),
+                  "vmscan_cached_scan")
     return y
 
 
@@ -396,30 +421,41 @@ def conv1d_silu_cached_cuda(x, weight, bias, state, batch: RequestBatch) -> torc
     requests and behind the last request.
     """
     where = "conv1d_silu_cached_cuda"
-    _check_batch(where, batch, x)
+    if not _batch_ok(batch, x):
+        _refuse_batch(where, batch, x)
     rows, c = x.shape
+    index = batch.index
     for name, t in (("weight", weight), ("bias", bias)):
-        if not isinstance(t, torch.Tensor) or t.device != x.device:
+        if not isinstance(t, torch.Tensor) or t.get_device() != index:
             raise RuntimeError(f"{where}: `{name}` must be a CUDA tensor on x's device (there is no CPU path)")
-    if weight.dim() != 3 or weight.shape[0] != c or weight.shape[2] != 1 or tuple(bias.shape) != (c,):
+    if weight.dim() != 3 or weight.shape[0] != c or weight.shape[2] != 1 or bias.shape != (c,):
         raise ValueError(f"{where}: bad shapes x={tuple(x.shape)} weight={tuple(weight.shape)} bias={tuple(bias.shape)}")
     k = weight.shape[1]
     if not 1 <= k <= 8:
         raise ValueError(f"{where}: kernel size {k} (1 to 8)")
-    _check_state(where, state, x, (k - 1, c), x.dtype, batch)
-    _refuse_grad(where, x, weight, bias, state)
+    _check_state(where, state, (k - 1, c), x.dtype, batch)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad
+                                    or state.requires_grad):
+        _refuse_grad(where)
     if c == 0:
         return torch.zeros_like(x)
-    lib = _native.load()
-    with _device_guard(x.device):
-        x = _rows(x, x.dtype)
-        weight, bias = _param(weight), _param(bias)
-        out = _out_rows(x, c, batch)
-        table = batch._table("conv")
-        _native.check(lib.vmscan_cached_conv1d_silu(
-            rows, c, k, int(x.dtype == torch.bfloat16), _p(x), x.stride(0), _p(weight), _p(bias), _p(out), c, _p(state),
-            state.shape[0], _p(table.tensor), table.info[0], torch.cuda.current_stream().cuda_stream),
-            "vmscan_cached_conv1d_silu")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _conv_cached(x, weight, bias, state, batch, k)
+    return _conv_cached(x, weight, bias, state, batch, k)
+
+
+def _conv_cached(x, weight, bias, state, batch, k):
+    rows, c = x.shape
+    x = _rows(x, x.dtype)
+    weight, bias = _param(weight), _param(bias)
+    out = _out_rows(x, c, batch)
+    stream = _stream_of(batch.index)
+    table = batch._table("conv", stream)
+    _native.check(_native.load().vmscan_cached_conv1d_silu(
+        rows, c, k, x.dtype is torch.bfloat16, x.data_ptr(), x.stride(0), weight.data_ptr(), bias.data_ptr(),
+        out.data_ptr(), c, state.data_ptr(), state.shape[0], table.tensor.data_ptr(), table.info[0], stream),
+        "vmscan_cached_conv1d_silu")
     return out
 
 
@@ -456,49 +492,59 @@ def lora_add_cuda(base: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, b
     once.
     """
     where = "lora_add_cuda"
-    _check_batch(where, batch, x)
+    if not _batch_ok(batch, x):
+        _refuse_batch(where, batch, x)
     if not isinstance(adapters, LoraAdapters):
         raise TypeError(f"{where}: `adapters` must be LoraAdapters, got {type(adapters).__name__}")
-    rows = x.shape[0]
-    for name, t, cols in (("base", base, adapters.d_out), ("x", x, adapters.d_in), ("out", out, adapters.d_out)):
-        if t is None:
+    rows, index, dtype = x.shape[0], batch.index, adapters.a.dtype
+    wide = (rows, adapters.d_out)
+    for name, t, shape in (("x", x, (rows, adapters.d_in)), ("base", base, wide), ("out", out, wide)):
+        if t is None and name == "out":
             continue
-        if not isinstance(t, torch.Tensor) or t.device != x.device:
+        if not isinstance(t, torch.Tensor) or t.get_device() != index:
             raise RuntimeError(f"{where}: `{name}` must be a CUDA tensor on x's device (there is no CPU path)")
-        if tuple(t.shape) != (rows, cols):
-            raise ValueError(f"{where}: {name} must be {(rows, cols)}, got {tuple(t.shape)}")
-        if t.dtype != adapters.a.dtype:
-            raise TypeError(f"{where}: {name} is {t.dtype}, the adapters are {adapters.a.dtype}")
-    if adapters.a.device != x.device:
+        if t.shape != shape:
+            raise ValueError(f"{where}: {name} must be {shape}, got {tuple(t.shape)}")
+        if t.dtype is not dtype:
+            raise TypeError(f"{where}: {name} is {t.dtype}, the adapters are {dtype}")
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse_grad(where)
+    if adapters.a.get_device() != index:
         raise ValueError(f"{where}: the adapters are on {adapters.a.device}, x is on {x.device}")
     if batch.adapters is None:
         raise ValueError(f"{where}: the batch was made without adapters")
     if batch.max_adapter >= adapters.count:
         raise ValueError(f"{where}: the batch uses adapter {batch.max_adapter}, there are {adapters.count}")
-    _refuse_grad(where, base, x, out)
-    lib = _native.load()
-    with _device_guard(x.device):
-        in_place = out is not None and (out is base or (out.data_ptr() == base.data_ptr() and
-                                                        out.stride() == base.stride()))
-        if out is not None:
-            if rows and ((out.stride(1) != 1 and out.shape[1] > 1) or (rows > 1 and out.stride(0) < out.shape[1])):
-                raise ValueError(f"{where}: out must have unit column stride and rows that do not overlap")
-            if rows and (_collide(out, _rows(x, x.dtype)) or (not in_place and _collide(out, _rows(base, base.dtype)))):
-                raise ValueError(f"{where}: out overlaps x or base (it may only be base itself)")
-        x = _rows(x, x.dtype)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _lora_add(where, base, x, adapters, batch, out)
+    return _lora_add(where, base, x, adapters, batch, out)
+
+
+def _lora_add(where, base, x, adapters, batch, out):
+    rows = x.shape[0]
+    x = _rows(x, x.dtype)
+    if out is None:
+        base = _rows(base, base.dtype)
+        out = base.new_empty((rows, adapters.d_out))
+        in_place = False
+    else:
+        in_place = out is base or (out.data_ptr() == base.data_ptr() and out.stride() == base.stride())
+        if rows and ((out.stride(1) != 1 and out.shape[1] > 1) or (rows > 1 and out.stride(0) < out.shape[1])):
+            raise ValueError(f"{where}: out must have unit column stride and rows that do not overlap")
         base = base if in_place else _rows(base, base.dtype)
-        if out is None:
-            out = torch.empty((rows, adapters.d_out), dtype=base.dtype, device=base.device)
-        if rows > batch.tokens and not in_place:
-            out[batch.tokens:].copy_(base[batch.tokens:])
-        if batch.tokens == 0:
-            return out
-        table = batch._table("lora")
-        tiles = table.info[0]
-        p = _p(table.tensor)
-        _native.check(lib.vmscan_lora_add(
-            rows, adapters.d_in, adapters.d_out, adapters.rank, adapters.count, int(x.dtype == torch.bfloat16), _p(x),
-            x.stride(0), _p(adapters.a), _p(adapters.b), _p(adapters.scale), _p(base), base.stride(0), _p(out),
-            out.stride(0), p + 16 * tiles, batch.tokens, p, tiles, torch.cuda.current_stream().cuda_stream),
-            "vmscan_lora_add")
+        if rows and (_collide(out, x) or (not in_place and _collide(out, base))):
+            raise ValueError(f"{where}: out overlaps x or base (it may only be base itself)")
+    if rows > batch.tokens and not in_place:
+        out[batch.tokens:].copy_(base[batch.tokens:])
+    if batch.tokens == 0:
+        return out
+    stream = _stream_of(batch.index)
+    table = batch._table("lora", stream)
+    tiles = table.info[0]
+    p = table.tensor.data_ptr()
+    _native.check(_native.load().vmscan_lora_add(
+        rows, adapters.d_in, adapters.d_out, adapters.rank, adapters.count, x.dtype is torch.bfloat16, x.data_ptr(), x.stride(0),
+        adapters.a.data_ptr(), adapters.b.data_ptr(), adapters.scale.data_ptr(), base.data_ptr(), base.stride(0),
+        out.data_ptr(), out.stride(0), p + 16 * tiles, batch.tokens, p, tiles, stream), "vmscan_lora_add")
     return out

@@ -16,8 +16,10 @@ most 18 roundings of partial sums), and the gate's relative error of at most
 (10 + 3 |z|) EPS (ex2, the quotient's 2 steps, the products).
 
 Conv: K + 1 roundings of partial sums, SiLU's slope of at most 1.1 and its own
-error as the gate's.  Adapters: d_in + 8 and rank + 8 roundings of partial sums
-(8 covers the products' and the operand splits').  A bf16 output is off by
+error as the gate's.  Adapters: d_in + 14 and rank + 14 roundings of partial
+sums: 12 cover the products of TF32 parts (a part is rounded to 11 bits, so hi +
+lo leaves 2^-22 = 4 EPS of each factor, and the product of the two lo parts
+that is not formed is another 2^-22), 2 the scale and the sum over the warps.  A bf16 output is off by
 another half step, 2^-8 relative.
 
 All bounds carry a factor 1.05 for their second-order terms.
@@ -108,7 +110,7 @@ def lora(base, x, adapters, batch):
         r = slice(at[i], at[i + 1])
         low, mag = x[r] @ a[k].t(), x[r].abs() @ a[k].abs().t()
         part = (mag @ b[k].abs().t()) * scale[k].abs()
-        tol[r] = ((adapters.d_in + 8) + (adapters.rank + 8)) * EPS * part + 2 * EPS * y[r].abs()
+        tol[r] = ((adapters.d_in + 14) + (adapters.rank + 14)) * EPS * part + 2 * EPS * y[r].abs()
         y[r] = y[r] + scale[k] * (low @ b[k].t())
         tol[r] = tol[r] + y[r].abs() * (EPS + HALF_STEP[base.dtype])
     return y, 1.05 * tol
