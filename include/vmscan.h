@@ -426,21 +426,23 @@ int vmscan_gemm_tf32x3(int64_t M, int64_t N, int64_t K,
  *
  * vmscan_request_pieces (host only) cuts requests into pieces of at most
  * max_rows rows (0: one piece per request): it writes n records of 8 int32
- * {t0, t1, begin, end, source, slot, carry row, 0 / 1} followed by n_chains
- * records of 4 int32 {first carry row, pieces, source, 0} into `pieces`
- * (capacity in int32) and {n_carry, n_chains, carry_rows} into info[3], and
- * returns n; with pieces == NULL it only counts.  by_length != 0 orders the
- * pieces for vmscan_cached_scan (pieces with a carry first, then long ones
- * first); 0 keeps row order (vmscan_cached_conv1d_silu).  Negative on a bad
- * argument.
+ * {t0, t1, begin, end, source, slot, carry row, ordinal} into `pieces`
+ * (capacity in int32) and returns n; with pieces == NULL it only counts.
+ * scan == 0: in row order, for vmscan_cached_conv1d_silu.  scan != 0: for
+ * vmscan_cached_scan, which runs two phases: the first info[0] records
+ * (requests of one piece, and all but the last piece of the others) and then
+ * the rest (all but the first pieces of split requests), long ones first in
+ * each, followed by info[1] records of 4 int32 {first carry row, pieces, 0, 0},
+ * one for each split request; info[2] is the number of carry rows, info[3] the
+ * most pieces of a request.  Negative on a bad argument.
  *
  * vmscan_cached_scan_rows (host only) gives max_rows for vmscan_cached_scan on
  * the current device: 0 when one warp per request and 32 channels keeps the
  * GPU busy, else the rows a piece should have.
  */
 int64_t vmscan_request_pieces(int64_t count, const int32_t* lengths, const int32_t* slots, const int32_t* sources,
-                              int64_t max_rows, int by_length, int32_t* pieces, int64_t capacity, int64_t* info);
-int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d_inner);
+                              int64_t max_rows, int scan, int32_t* pieces, int64_t capacity, int64_t* info);
+int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d_inner, int bf16);
 int64_t vmscan_cached_scan_workspace_bytes(int64_t d_inner, int64_t carry_rows);
 
 /*
@@ -452,9 +454,9 @@ int64_t vmscan_cached_scan_workspace_bytes(int64_t d_inner, int64_t carry_rows);
 int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
                        const void* delta, int64_t lddelta, const float* A, const void* B, int64_t ldB, const void* C,
                        int64_t ldC, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
-                       int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
-                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* workspace,
-                       size_t workspace_bytes, vmscan_stream_t stream);
+                       int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_first,
+                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, int64_t longest_chain,
+                       void* workspace, size_t workspace_bytes, vmscan_stream_t stream);
 
 /*
  * The same for single tokens: row i is request i, with slots[i] and

@@ -125,12 +125,12 @@ SIGNATURES = {
          _p],
     ),
     "vmscan_request_pieces": (_i64, [_i64, _p, _p, _p, _i64, ctypes.c_int, _p, _i64, _p]),
-    "vmscan_cached_scan_rows": (_i64, [_i64, _p, _i64]),
+    "vmscan_cached_scan_rows": (_i64, [_i64, _p, _i64, ctypes.c_int]),
     "vmscan_cached_scan_workspace_bytes": (_i64, [_i64, _i64]),
     "vmscan_cached_scan": (
         ctypes.c_int,
         [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64,
-         _p, _i64, _i64, _p, _i64, _i64, _p, _sz, _p],
+         _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _sz, _p],
     ),
     "vmscan_cached_step": (
         ctypes.c_int,

@@ -1,9 +1,11 @@
-"""Builds libvmscan.so (the sm_100a selective-scan library) in-tree.
+"""Builds libvmscan.so (the sm_100a selective-scan library) and _serving_ext.so
+(the Python entry points of the serving operators) in-tree.
 
 Usage: ``python -m mlx_vision_mamba_b200.build`` or ``build()`` from Python.
 The library is a single nvcc translation unit (csrc/vmscan.cu) with the CUDA
 runtime linked statically, so it loads without a GPU and travels with the
-source tree.
+source tree.  The extension (csrc/serving_ext.cpp, g++) links against it and
+against the installed PyTorch.
 """
 
 from __future__ import annotations
@@ -19,6 +21,8 @@ LIB_PATH = os.path.join(PKG_DIR, "libvmscan.so")
 SOURCES = ["vmscan.cu"]
 DEPS = ["vmscan.cu", "vmscan_common.cuh", "vmscan_fwd.cuh", "vmscan_bwd.cuh", "vmscan_conv.cuh", "vmscan_dt.cuh",
         "vmscan_gemm.cuh", "vmscan_norm.cuh", "vmscan_cached.cuh", "vmscan_lora.cuh"]
+EXT_PATH = os.path.join(PKG_DIR, "_serving_ext.so")
+EXT_SOURCE = os.path.join(CSRC, "serving_ext.cpp")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -39,9 +43,16 @@ def _stale() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
-    """Compile libvmscan.so for sm_100a if missing or out of date; return its path."""
-    if not force and not _stale():
-        return LIB_PATH
+    """Compile libvmscan.so for sm_100a and _serving_ext.so if missing or out
+    of date; return the library's path."""
+    if force or _stale():
+        _build_library(verbose, extra_flags)
+    if force or _ext_stale():
+        _build_ext()
+    return LIB_PATH
+
+
+def _build_library(verbose: bool, extra_flags) -> None:
     cmd = [
         nvcc_path(),
         *ARCH_FLAGS,
@@ -66,7 +77,34 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     if verbose:
         sys.stdout.write(proc.stdout + proc.stderr)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
-    return LIB_PATH
+
+
+def _ext_stale() -> bool:
+    if not os.path.exists(EXT_PATH):
+        return True
+    header = os.path.join(os.path.dirname(PKG_DIR), "include", "vmscan.h")
+    return any(os.path.getmtime(p) > os.path.getmtime(EXT_PATH) for p in (EXT_SOURCE, header))
+
+
+def _build_ext() -> None:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda_home = os.path.dirname(os.path.dirname(nvcc_path()))
+    lib_dirs = [*cpp_extension.library_paths(), PKG_DIR]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for inc in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda_home, "include")):
+        cmd += ["-isystem", inc]
+    cmd += ["-o", EXT_PATH + ".tmp", EXT_SOURCE]
+    for d in lib_dirs:
+        cmd += ["-L" + d]
+    cmd += ["-l:libvmscan.so", "-Wl,-rpath,$ORIGIN", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-ldl"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + " ".join(cmd) + "\n" + proc.stdout + proc.stderr)
+    os.replace(EXT_PATH + ".tmp", EXT_PATH)
 
 
 if __name__ == "__main__":

@@ -7,6 +7,7 @@
 // driver entry point and the sticky device status word.
 #include <cudaTypedefs.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -1285,6 +1286,20 @@ struct PieceSplit {
   int64_t count, rows;
 };
 
+// Measured on B200 (gated): cycles that a row of 32 channels takes on a
+// scheduler with four warps, there only for its carry, and on a scheduler with
+// one warp (with odd bf16 rows, whose loads go through registers); a piece's
+// start (parameters, state, first rows); a launch in the middle of a call; a
+// piece in the chain.
+constexpr double kScanMainCycles = 185, kScanCarryCycles = 145, kScanAloneCycles = 255, kScanOddAloneCycles = 490,
+                 kScanStartCycles = 1200, kScanLaunchCycles = 8000, kScanChainCycles = 80;
+// how much longer a row takes with one, two, three warps on a scheduler than with four
+constexpr double kScanFew[4] = {1.38, 1.15, 1.06, 1.0};
+constexpr int64_t kScanMinRows = 16;
+// Pieces of a request up to which a piece chains the maps before it itself
+// (each costs 16 exponentials a lane); above, a kernel does it for all.
+constexpr int64_t kChainInPiece = 8;
+
 PieceSplit split_request(int64_t len, int64_t max_rows, bool even) {
   if (max_rows <= 0 || len <= max_rows) return {1, len};
   int64_t rows = max_rows;
@@ -1325,15 +1340,17 @@ bool four_wide(const void* p, int64_t ld) {
 
 struct CachedScanPlan {
   int groups;       // CTAs per piece
+  int rows;         // carry rows
   size_t carry, sums, total;
 };
 
 CachedScanPlan cached_scan_plan(int64_t d_inner, int64_t carry_rows) {
   CachedScanPlan p;
   p.groups = int((d_inner + CSC_WARPS * 32 - 1) / (CSC_WARPS * 32));
+  p.rows = int(carry_rows);
   p.carry = align256(size_t(carry_rows) * d_inner * NS * 4);
   p.sums = align256(size_t(carry_rows) * d_inner * 4);
-  p.total = carry_rows > 0 ? 2 * p.carry + p.sums : 0;
+  p.total = carry_rows > 0 ? 2 * p.carry + p.sums : 0;  // end states, sums, start states
   return p;
 }
 
@@ -1353,46 +1370,57 @@ int cached_scan_grain(const CachedScanArgs& a) {
   return a.z != nullptr ? std::min(g, row_grain<T>(a.z, a.ldz, a.dn)) : g;
 }
 
-template <typename T, int G, bool HAS_Z, bool CARRY>
-int launch_scan_pass(const CachedScanArgs& a, const int32_t* pieces, int64_t n, int groups, const float* h_start,
-                     float* carry_h, float* carry_s, cudaStream_t s) {
+template <typename T, int G, bool HAS_Z>
+int launch_scan_phase(const CachedScanArgs& a, const int32_t* pieces, int64_t n, int groups, bool first,
+                      const ScanCarries& k, cudaStream_t s) {
   constexpr size_t smem = cached_scan_smem<T>();
-  auto kern = cached_scan_kernel<T, G, HAS_Z, CARRY>;
+  auto kern = cached_scan_kernel<T, G, HAS_Z>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
     return fail(VMSCAN_ERR_LAUNCH, "cudaFuncSetAttribute(cached_scan_kernel) failed");
   const int bc = std::min(row_grain<T>(a.B, a.ldb, NS), row_grain<T>(a.C, a.ldc, NS));
-  kern<<<unsigned(n * groups), CSC_WARPS * 32, smem, s>>>(a, pieces, groups, bc, h_start, carry_h, carry_s);
+  kern<<<unsigned(n * groups), CSC_WARPS * 32, smem, s>>>(a, pieces, groups, bc, first ? 1 : 0, k);
   return check_launch();
 }
 
-template <typename T, int G>
-int launch_cached_scan(const CachedScanArgs& a, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
-                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* ws, cudaStream_t s) {
-  const CachedScanPlan p = cached_scan_plan(a.dn, carry_rows);
+struct ScanPieces {
+  const int32_t* pieces;
+  int64_t n, n_first;
+  const int32_t* chains;
+  int64_t n_chains, longest;
+};
+
+template <typename T, int G, bool HAS_Z>
+int launch_cached_scan(const CachedScanArgs& a, const ScanPieces& q, const CachedScanPlan& p, void* ws,
+                       cudaStream_t s) {
   char* w = static_cast<char*>(ws);
-  float* carry_h = reinterpret_cast<float*>(w);
-  float* h_start = reinterpret_cast<float*>(w + p.carry);
-  float* carry_s = reinterpret_cast<float*>(w + 2 * p.carry);
-  if (n_chains > 0) {
-    VM_TRY((launch_scan_pass<T, G, false, true>(a, pieces, n_carry, p.groups, nullptr, carry_h, carry_s, s)));
-    cached_chain_kernel<<<dim3(unsigned((int64_t(a.dn) * NS + 127) / 128), unsigned(n_chains)), 128, 0, s>>>(
-        chains, a.A, a.state, a.n_slots, carry_h, carry_s, h_start, a.dn);
+  ScanCarries k{nullptr, nullptr, nullptr, 0};
+  if (q.n_chains > 0) k = {reinterpret_cast<float*>(w), reinterpret_cast<float*>(w + p.carry), nullptr, p.rows};
+  VM_TRY((launch_scan_phase<T, G, HAS_Z>(a, q.pieces, q.n_first, p.groups, true, k, s)));
+  if (q.n == q.n_first) return VMSCAN_OK;
+  if (q.longest > kChainInPiece) {
+    float* start = reinterpret_cast<float*>(w + p.carry + p.sums);
+    cached_chain_kernel<<<dim3(unsigned((int64_t(a.dn) * NS + 127) / 128), unsigned(q.n_chains)), 128, 0, s>>>(
+        q.chains, a.A, k.h, k.sum, start, a.dn, p.rows);
     VM_TRY(check_launch());
+    k.start = start;
   }
-  if (a.z != nullptr)
-    return launch_scan_pass<T, G, true, false>(a, pieces, n_pieces, p.groups, h_start, nullptr, nullptr, s);
-  return launch_scan_pass<T, G, false, false>(a, pieces, n_pieces, p.groups, h_start, nullptr, nullptr, s);
+  return launch_scan_phase<T, G, HAS_Z>(a, q.pieces + q.n_first * PF_COUNT, q.n - q.n_first, p.groups, false, k, s);
+}
+
+template <typename T, int G>
+int launch_cached_scan_z(const CachedScanArgs& a, const ScanPieces& q, const CachedScanPlan& p, void* ws,
+                         cudaStream_t s) {
+  return a.z != nullptr ? launch_cached_scan<T, G, true>(a, q, p, ws, s) : launch_cached_scan<T, G, false>(a, q, p, ws, s);
 }
 
 template <typename T>
-int run_cached_scan(const CachedScanArgs& a, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
-                    const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* ws, cudaStream_t s) {
+int run_cached_scan(const CachedScanArgs& a, const ScanPieces& q, const CachedScanPlan& p, void* ws, cudaStream_t s) {
   const int g = cached_scan_grain<T>(a);
-  if (g == 16) return launch_cached_scan<T, 16>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, ws, s);
+  if (g == 16) return launch_cached_scan_z<T, 16>(a, q, p, ws, s);
   if constexpr (sizeof(T) == 2) {
-    if (g == 2) return launch_cached_scan<T, 2>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, ws, s);
+    if (g == 2) return launch_cached_scan_z<T, 2>(a, q, p, ws, s);
   }
-  return launch_cached_scan<T, 4>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, ws, s);
+  return launch_cached_scan_z<T, 4>(a, q, p, ws, s);
 }
 
 template <typename T>
@@ -1447,79 +1475,118 @@ int launch_lora(LoraArgs& l, int n_tiles, cudaStream_t s) {
 
 extern "C" {
 
-int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d_inner) {
+int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d_inner, int bf16) {
   if (count <= 0 || lengths == nullptr || d_inner <= 0) return -VMSCAN_ERR_SHAPE;
-  int64_t total = 0, longest = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    total += lengths[i];
-    longest = std::max<int64_t>(longest, lengths[i]);
+  int64_t longest = 0;
+  for (int64_t i = 0; i < count; ++i) longest = std::max<int64_t>(longest, lengths[i]);
+  // Estimated time, in cycles, for every way of cutting the longest request
+  // into 1, 3, 4, 6, 8, 12, ... pieces (and the others into pieces of that
+  // length).  Two pieces would only run one after the other.
+  const double alone = bf16 && d_inner % 2 != 0 ? kScanOddAloneCycles : kScanAloneCycles;
+  const double groups = double((d_inner + CSC_WARPS * 32 - 1) / (CSC_WARPS * 32)), sms = sm_count();
+  // A launch of pieces x groups CTAs (a warp on each scheduler): its work at
+  // the rate of full schedulers, as far as whole CTAs spread evenly over the
+  // SMs, or its longest piece at the rate of a lone warp, whichever is longer.
+  const auto phase = [&](double pieces, double work, double longest_rows) {
+    const double per_sm = pieces * groups / sms;
+    if (per_sm <= 0) return 0.0;
+    const double spread = std::ceil(per_sm) / per_sm * kScanFew[std::min(int(std::ceil(per_sm)), 4) - 1];
+    return std::max((work + pieces * kScanStartCycles) * groups / sms * std::min(spread, 2.0),
+                    longest_rows * alone + kScanStartCycles);
+  };
+  double best = 0;
+  int64_t best_rows = 0;
+  for (int64_t k = 1; k == 1 || longest / k >= kScanMinRows; k = k < 3 ? 3 : (k % 3 == 0 ? k / 3 * 4 : k / 2 * 3)) {
+    const int64_t rows = k == 1 ? 0 : (longest + k - 1) / k;
+    double n1 = 0, n2 = 0, work1 = 0, work2 = 0, long1 = 0, long2 = 0;
+    int64_t pieces = 1;
+    for (int64_t i = 0; i < count; ++i) {
+      const PieceSplit p = split_request(lengths[i], rows, true);
+      const double each = double(p.count > 1 ? p.rows : lengths[i]), middle = double(std::max<int64_t>(p.count - 2, 0));
+      n1 += 1 + middle;
+      work1 += each * (kScanMainCycles + middle * kScanCarryCycles);
+      long1 = std::max(long1, each);
+      if (p.count > 1) {
+        n2 += double(p.count - 1);
+        work2 += double(p.count - 1) * each * kScanMainCycles;
+        long2 = std::max(long2, each);
+      }
+      pieces = std::max(pieces, p.count);
+    }
+    double t = phase(n1, work1, long1);
+    if (pieces > 1) t += phase(n2, work2, long2) + kScanLaunchCycles;
+    if (pieces > kChainInPiece) t += kScanLaunchCycles + double(pieces) * kScanChainCycles;
+    if (k == 1 || t < best) {
+      best = t;
+      best_rows = rows;
+    }
   }
-  // rows a warp would scan if the work were spread evenly over 16 warps an SM
-  const int64_t warps = (d_inner + 31) / 32;
-  const int64_t even = total * warps / (int64_t(sm_count()) * 16) + 1;
-  if (longest <= 2 * even + 64) return 0;
-  return std::max<int64_t>(even, 64);
+  return best_rows;
 }
 
 int64_t vmscan_request_pieces(int64_t count, const int32_t* lengths, const int32_t* slots, const int32_t* sources,
-                              int64_t max_rows, int by_length, int32_t* pieces, int64_t capacity, int64_t* info) {
+                              int64_t max_rows, int scan, int32_t* pieces, int64_t capacity, int64_t* info) {
   const int rc = check_requests(count, lengths, slots, sources);
   if (rc != VMSCAN_OK) return -rc;
   if (max_rows < 0 || info == nullptr) return -VMSCAN_ERR_SHAPE;
-  int64_t n = 0, n_carry = 0, n_chains = 0, carry_rows = 0;
+  int64_t n = 0, n_first = 0, n_chains = 0, carry_rows = 0, longest = 1;
   for (int64_t i = 0; i < count; ++i) {
-    const int64_t k = split_request(lengths[i], max_rows, by_length != 0).count;
-    n += k;
-    if (k > 1) {
-      n_carry += k - 1;
+    const int64_t k = split_request(lengths[i], max_rows, scan != 0).count;
+    n += scan && k > 1 ? 2 * k - 2 : k;  // the pieces between first and last are in both phases
+    n_first += scan && k > 1 ? k - 1 : k;
+    if (scan && k > 1) {
       n_chains += 1;
       carry_rows += k;
+      longest = std::max(longest, k);
     }
   }
   if (n > INT32_MAX) return -VMSCAN_ERR_SHAPE;
-  info[0] = n_carry;
+  info[0] = n_first;
   info[1] = n_chains;
   info[2] = carry_rows;
+  info[3] = longest;
   if (pieces == nullptr) return n;
   if (capacity < n * PF_COUNT + n_chains * 4) return -VMSCAN_ERR_WORKSPACE;
   PieceRecord* out = reinterpret_cast<PieceRecord*>(pieces);
   int32_t* chain = pieces + n * PF_COUNT;
-  int64_t at = 0, begin = 0, carry = 0;
+  int64_t first = 0, later = n_first, begin = 0, carry = 0;
   for (int64_t i = 0; i < count; ++i) {
     const int64_t len = lengths[i];
-    const PieceSplit sp = split_request(len, max_rows, by_length != 0);
+    const PieceSplit sp = split_request(len, max_rows, scan != 0);
     const int64_t k = sp.count;
-    const int64_t source = slots[i] < 0 ? -1 : sources[i];
     for (int64_t j = 0; j < k; ++j) {
       PieceRecord r;
       r.f[PF_T0] = int32_t(begin + j * sp.rows);
       r.f[PF_T1] = int32_t(begin + (j + 1 < k ? (j + 1) * sp.rows : len));
       r.f[PF_BEGIN] = int32_t(begin);
       r.f[PF_END] = int32_t(begin + len);
-      r.f[PF_SOURCE] = int32_t(source);
+      r.f[PF_SOURCE] = slots[i] < 0 ? -1 : sources[i];
       r.f[PF_SLOT] = slots[i];
-      r.f[PF_CARRY] = k > 1 ? int32_t(carry + j) : -1;
-      r.f[PF_PAD] = k > 1 && j + 1 < k ? 1 : 0;
-      out[at++] = r;
+      r.f[PF_CARRY] = scan && k > 1 ? int32_t(carry + j) : -1;
+      r.f[PF_ORDINAL] = int32_t(j);
+      if (!scan || j + 1 < k || k == 1) out[first++] = r;
+      if (scan && j > 0) out[later++] = r;
     }
-    if (k > 1) {
+    if (scan && k > 1) {
       chain[0] = int32_t(carry);
       chain[1] = int32_t(k);
-      chain[2] = int32_t(source);
-      chain[3] = 0;
+      chain[2] = chain[3] = 0;
       chain += 4;
       carry += k;
     }
     begin += len;
   }
-  if (by_length)
-    std::sort(out, out + n, [](const PieceRecord& x, const PieceRecord& y) {
-      if (x.f[PF_PAD] != y.f[PF_PAD]) return x.f[PF_PAD] > y.f[PF_PAD];
+  if (scan) {
+    // long pieces first: the short ones fill the gaps at the end
+    const auto longer = [](const PieceRecord& x, const PieceRecord& y) {
       const int32_t lx = x.f[PF_T1] - x.f[PF_T0], ly = y.f[PF_T1] - y.f[PF_T0];
       if (lx != ly) return lx > ly;
       if (x.f[PF_T0] != y.f[PF_T0]) return x.f[PF_T0] < y.f[PF_T0];
       return x.f[PF_SLOT] < y.f[PF_SLOT];
-    });
+    };
+    std::sort(out, out + n_first, longer);
+    std::sort(out + n_first, out + n, longer);
+  }
   return n;
 }
 
@@ -1532,26 +1599,25 @@ int64_t vmscan_cached_scan_workspace_bytes(int64_t d_inner, int64_t carry_rows) 
 int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,
                        const void* delta, int64_t ldd, const float* A, const void* B, int64_t ldb, const void* C,
                        int64_t ldc, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
-                       int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_carry,
-                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, void* workspace,
-                       size_t workspace_bytes, vmscan_stream_t stream) {
+                       int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_first,
+                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, int64_t longest_chain,
+                       void* workspace, size_t workspace_bytes, vmscan_stream_t stream) {
   CachedScanArgs a;
   VM_TRY(cached_scan_args(a, rows, d_inner, d_state, u, ldu, delta, ldd, A, B, ldb, C, ldc, D, z, ldz, y, ldy, state,
                           n_slots));
   if (pieces == nullptr || (n_chains > 0 && chains == nullptr)) return VMSCAN_ERR_NULL;
   if (!aligned16(pieces) || !aligned16(chains)) return fail(VMSCAN_ERR_ALIGN, "pieces and chains must be 16-byte aligned");
-  const CachedScanPlan p = cached_scan_plan(d_inner, carry_rows);
-  if (n_pieces <= 0 || n_carry < 0 || n_carry > n_pieces || n_chains < 0 || n_chains > 65535 || carry_rows < 0 ||
-      (n_chains > 0) != (carry_rows > 0) || (n_chains > 0) != (n_carry > 0) || n_pieces * p.groups > INT32_MAX)
-    return fail(VMSCAN_ERR_SHAPE, "cached scan: %lld pieces (%lld with carries), %lld chains, %lld carry rows",
-                (long long)n_pieces, (long long)n_carry, (long long)n_chains, (long long)carry_rows);
+  const CachedScanPlan p = cached_scan_plan(d_inner, std::max<int64_t>(carry_rows, 0));
+  if (n_pieces <= 0 || n_first <= 0 || n_first > n_pieces || n_chains < 0 || n_chains > 65535 || carry_rows < 0 || carry_rows > INT32_MAX ||
+      (n_chains > 0) != (carry_rows > 0) || (n_chains > 0) != (n_first < n_pieces) || n_pieces * p.groups > INT32_MAX)
+    return fail(VMSCAN_ERR_SHAPE, "cached scan: %lld pieces (%lld first), %lld chains, %lld carry rows",
+                (long long)n_pieces, (long long)n_first, (long long)n_chains, (long long)carry_rows);
   if (p.total > 0 && (workspace == nullptr || workspace_bytes < p.total || !aligned16(workspace)))
     return fail(VMSCAN_ERR_WORKSPACE, "cached scan: needs %zu bytes of 16-byte aligned workspace", p.total);
   VM_TRY(ensure_context(state));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (bf16)
-    return run_cached_scan<__nv_bfloat16>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
-  return run_cached_scan<float>(a, pieces, n_pieces, n_carry, chains, n_chains, carry_rows, workspace, s);
+  const ScanPieces q{pieces, n_pieces, n_first, chains, n_chains, longest_chain};
+  return bf16 ? run_cached_scan<__nv_bfloat16>(a, q, p, workspace, s) : run_cached_scan<float>(a, q, p, workspace, s);
 }
 
 int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16, const void* u, int64_t ldu,

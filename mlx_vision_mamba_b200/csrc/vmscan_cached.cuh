@@ -23,11 +23,12 @@ namespace vmscan {
 // One piece: rows [T0, T1) of the request that owns rows [BEGIN, END).
 // SOURCE: slot its state is read from (-1: zeros), SLOT: slot written (-1: a
 // padding request, whose rows are set to zero).  CARRY: row of the carry
-// arrays when the request is scanned in several pieces, else -1.
-enum PieceField { PF_T0, PF_T1, PF_BEGIN, PF_END, PF_SOURCE, PF_SLOT, PF_CARRY, PF_PAD, PF_COUNT };
+// arrays when the request is scanned in several pieces, else -1; ORDINAL: the
+// piece's place among them (their carry rows are consecutive).
+enum PieceField { PF_T0, PF_T1, PF_BEGIN, PF_END, PF_SOURCE, PF_SLOT, PF_CARRY, PF_ORDINAL, PF_COUNT };
 
 struct Piece {
-  int t0, t1, begin, end, source, slot, carry;
+  int t0, t1, begin, end, source, slot, carry, ordinal;
 };
 
 // Reads a piece and keeps it inside the arrays whatever the table holds: rows
@@ -43,6 +44,7 @@ __device__ __forceinline__ Piece load_piece(const int32_t* __restrict__ pieces, 
   p.source = b.x < n_slots ? b.x : -1;
   p.slot = b.y < n_slots ? b.y : -1;
   p.carry = b.z;
+  p.ordinal = b.w;
   return p;
 }
 
@@ -83,8 +85,9 @@ struct CachedScanArgs {
 // (cached_scan_grain): 16, 4 (two bf16 or one fp32) or 2 (odd bf16 rows: plain
 // loads, kept in registers while the block before is computed).  bc_grain: the
 // same for B and C.
-// CARRY: only the state at the piece's end from a zero state and the sum of
-// delta (the piece maps h to exp(A sum delta) h + carry_h).
+// A request that would keep a few warps busy long after the others is split
+// into pieces.  CARRY: a piece whose start is not known yet only yields its
+// map h -> exp(A sum delta) h + (its end state from zero).
 // ---------------------------------------------------------------------------
 constexpr int CSC_WARPS = 4;
 constexpr int CSC_ROWS = 8;
@@ -136,16 +139,21 @@ constexpr size_t cached_scan_smem() {
   return sizeof(ScanRing<T>) * CSC_WARPS;
 }
 
+// Where the pieces of split requests leave and find their states.
+struct ScanCarries {
+  float* h;             // (carry rows, dn, 16): state at a piece's end (a first piece: the true one; later: from zero)
+  float* sum;           // (carry rows, dn): sum of delta over a later piece
+  const float* start;   // (carry rows, dn, 16): state entering a later piece, or NULL: chained here
+  int rows;             // carry rows
+};
+
 template <typename T, int G, bool HAS_Z, bool CARRY>
-__global__ void __launch_bounds__(CSC_WARPS * 32)
-    cached_scan_kernel(const CachedScanArgs a, const int32_t* __restrict__ pieces, int groups, int bc_grain,
-                       const float* __restrict__ h_start, float* __restrict__ carry_h, float* __restrict__ carry_s) {
+__device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const Piece& p, int group, int bc_grain,
+                                                  const ScanCarries& k, unsigned char* smem_raw) {
   constexpr bool LOAD_Z = HAS_Z && !CARRY;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ScanRing<T>& ring = reinterpret_cast<ScanRing<T>*>(smem_raw)[warp];
-  const Piece p = load_piece(pieces, blockIdx.x / groups, a.rows, a.n_slots);
-  const int d0 = ((blockIdx.x % groups) * CSC_WARPS + warp) * 32;
+  const int d0 = (group * CSC_WARPS + warp) * 32;
   if (d0 >= a.dn) return;  // whole warps: the rest shuffles and syncs by warp only
   const int hb = lane & 1, pc = lane & ~1;
   const int own = d0 + lane, dp = d0 + pc;
@@ -224,10 +232,10 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
   float2 A2[2][4], h[2][4];
   const float* src = nullptr;
   if (!CARRY) {
-    if (p.carry >= 0)  // also for a first piece: another piece may write the source's slot meanwhile
-      src = h_start + int64_t(p.carry) * a.dn * NS;
-    else if (p.source >= 0)
-      src = a.state + int64_t(p.source) * a.dn * NS;
+    if (p.carry < 0 || p.ordinal == 0)
+      src = p.source >= 0 ? a.state + int64_t(p.source) * a.dn * NS : nullptr;
+    else
+      src = k.start != nullptr ? k.start + int64_t(p.carry) * a.dn * NS : k.h + int64_t(p.carry - p.ordinal) * a.dn * NS;
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -240,6 +248,22 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
       const float4 g = src != nullptr ? *reinterpret_cast<const float4*>(src + off + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
       h[c][2 * j] = make_float2(g.x, g.y);
       h[c][2 * j + 1] = make_float2(g.z, g.w);
+    }
+  }
+  if (!CARRY && p.carry >= 0 && k.start == nullptr) {
+    // the maps of the later pieces before this one, onto the first piece's end
+    for (int i = 1; i < p.ordinal; ++i) {
+      const int64_t at = int64_t(p.carry - p.ordinal + i) * a.dn;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int64_t ch = at + min(dp + c, a.dn - 1);
+        const float sum = k.sum[ch];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 g = *reinterpret_cast<const float2*>(k.h + ch * NS + 8 * hb + 2 * j);
+          h[c][j] = fma2(make_float2(expf(A2[c][j].x * sum), expf(A2[c][j].y * sum)), h[c][j], g);
+        }
+      }
     }
   }
   const float Dd = a.D[min(own, a.dn - 1)];
@@ -274,23 +298,23 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
       float2 e[2][4];
       float2 u, d;
     };
-    auto decay = [&](int r, Decay& k) {
-      k.u = ld_pair(&st.u[r][pc]);
-      k.d = ld_pair(&st.dl[r][pc]);
-      const float2 dlog = mul2(k.d, bcast2(kLog2e)), off = bcast2(kEx2ArgBias);
+    auto decay = [&](int r, Decay& w) {
+      w.u = ld_pair(&st.u[r][pc]);
+      w.d = ld_pair(&st.dl[r][pc]);
+      const float2 dlog = mul2(w.d, bcast2(kLog2e)), off = bcast2(kEx2ArgBias);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float2 dg = bcast2(c ? dlog.y : dlog.x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 arg = fma2(dg, A2[c][j], off);
-          k.e[c][j] = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+          w.e[c][j] = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
         }
       }
     };
-    auto row = [&](int r, const Decay& k) {
-      const float2 du = mul2(k.d, k.u);
-      if (CARRY) dsum = add2(dsum, k.d);
+    auto row = [&](int r, const Decay& w) {
+      const float2 du = mul2(w.d, w.u);
+      if (CARRY) dsum = add2(dsum, w.d);
       const float* s = bc + r * 32 + 8 * hb;
       const float4 b0 = lds4(s), b1 = lds4(s + 4);
       const float2 B2[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y),
@@ -299,7 +323,7 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
       for (int c = 0; c < 2; ++c) {
         const float2 db = bcast2(c ? du.y : du.x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[c][j] = fma2(k.e[c][j], h[c][j], mul2(db, B2[j]));
+        for (int j = 0; j < 4; ++j) h[c][j] = fma2(w.e[c][j], h[c][j], mul2(db, B2[j]));
       }
       if (!CARRY) {
         const float4 e0 = lds4(s + NS), e1 = lds4(s + NS + 4);
@@ -312,7 +336,7 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
               add2(fma2(C2[1], h[c][1], mul2(C2[0], h[c][0])), fma2(C2[3], h[c][3], mul2(C2[2], h[c][2])));
           part[c] = acc.x + acc.y;
         }
-        float yy = fmaf(hb ? k.u.y : k.u.x, Dd, pair_scatter(part[0], part[1], hb));
+        float yy = fmaf(hb ? w.u.y : w.u.x, Dd, pair_scatter(part[0], part[1], hb));
         if (HAS_Z) yy *= silu_f(ld_one(&st.z[r][lane]));
         // an explicit global store: a generic one could alias the ring, and would keep the next row's
         // shared loads behind it
@@ -340,10 +364,12 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
   }
   float* dst = nullptr;
   if (CARRY) {
-    dst = carry_h + int64_t(p.carry) * a.dn * NS;
-    if (ok) carry_s[int64_t(p.carry) * a.dn + own] = hb ? dsum.y : dsum.x;
+    dst = k.h + int64_t(p.carry) * a.dn * NS;
+    if (ok) k.sum[int64_t(p.carry) * a.dn + own] = hb ? dsum.y : dsum.x;
   } else if (p.t1 == p.end) {
     dst = a.state + int64_t(p.slot) * a.dn * NS;
+  } else if (p.carry >= 0 && p.ordinal == 0) {
+    dst = k.h + int64_t(p.carry) * a.dn * NS;
   }
   if (dst == nullptr) return;
 #pragma unroll
@@ -356,23 +382,57 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
     }
 }
 
-// State entering every piece of the split requests: chain i =
-// {first carry row, pieces, source slot, 0}; one thread per (chain, channel,
-// state) walks the pieces' maps.
+// A launch runs pieces of one phase (the request's pieces in two launches, so
+// that a later piece finds its start and no slot is written before it is read):
+// first: whole requests and first pieces from their source's state, and the
+//        carries of the pieces between the first and the last one;
+// later: pieces after the first, from the chained carries.
+template <typename T, int G, bool HAS_Z>
+__global__ void __launch_bounds__(CSC_WARPS * 32)
+    cached_scan_kernel(const CachedScanArgs a, const int32_t* __restrict__ pieces, int groups, int bc_grain,
+                       int first_phase, const ScanCarries k) {
+  extern __shared__ __align__(16) unsigned char scan_raw[];
+  Piece p = load_piece(pieces, blockIdx.x / groups, a.rows, a.n_slots);
+  p.carry = p.carry < k.rows ? p.carry : -1;
+  p.ordinal = min(max(p.ordinal, 0), max(p.carry, 0));
+  if (first_phase && p.carry >= 0 && p.ordinal > 0)
+    cached_scan_piece<T, G, HAS_Z, true>(a, p, blockIdx.x % groups, bc_grain, k, scan_raw);
+  else
+    cached_scan_piece<T, G, HAS_Z, false>(a, p, blockIdx.x % groups, bc_grain, k, scan_raw);
+}
+
+// State entering every later piece of the split requests: chain i = {first
+// carry row, pieces, 0, 0}; one thread per (chain, channel, state) walks the
+// pieces' maps, the loads of CCH_AHEAD pieces at a time.  Only for requests of
+// many pieces: a few are chained by the pieces themselves.
+constexpr int CCH_AHEAD = 8;
 __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const float* __restrict__ A,
-                                    const float* __restrict__ state, int64_t n_slots,
                                     const float* __restrict__ carry_h, const float* __restrict__ carry_s,
-                                    float* __restrict__ h_start, int dn) {
+                                    float* __restrict__ h_start, int64_t dn, int rows) {
   const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= int64_t(dn) * NS) return;
-  const int4 c = reinterpret_cast<const int4*>(chains)[blockIdx.y];
+  if (i >= dn * NS) return;
+  int4 c = reinterpret_cast<const int4*>(chains)[blockIdx.y];
+  if (c.x < 0 || c.x >= rows) return;
+  c.y = min(c.y, rows - c.x);
   const float An = A[i];
-  float h = c.z >= 0 && c.z < n_slots ? state[int64_t(c.z) * dn * NS + i] : 0.f;
-  h_start[int64_t(c.x) * dn * NS + i] = h;
-  for (int k = 0; k + 1 < c.y; ++k) {
-    const int64_t row = c.x + k;
-    h = fmaf(expf(An * carry_s[row * dn + i / NS]), h, carry_h[row * dn * NS + i]);
-    h_start[(row + 1) * dn * NS + i] = h;
+  const int64_t ch = i / NS;
+  float h = carry_h[int64_t(c.x) * dn * NS + i];
+  for (int k0 = 1; k0 < c.y; k0 += CCH_AHEAD) {
+    float s[CCH_AHEAD], g[CCH_AHEAD];
+#pragma unroll
+    for (int q = 0; q < CCH_AHEAD; ++q) {
+      const bool in = k0 + q + 1 < c.y;  // the last piece has no map
+      const int64_t row = c.x + (in ? k0 + q : 0);
+      s[q] = in ? __ldg(carry_s + row * dn + ch) : 0.f;
+      g[q] = in ? __ldg(carry_h + row * dn * NS + i) : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < CCH_AHEAD; ++q) {
+      if (k0 + q < c.y) {
+        h_start[int64_t(c.x + k0 + q) * dn * NS + i] = h;
+        h = fmaf(expf(An * s[q]), h, g[q]);
+      }
+    }
   }
 }
 

@@ -51,59 +51,64 @@ def test_allowed_batches():
     assert RequestBatch([1], sources=[-1]).sources.tolist() == [-1]
 
 
-def _pieces(batch, rows, by_length):
+def _pieces(batch, rows, scan):
     lib = _native.load()
-    info = np.zeros(3, dtype=np.int64)
+    info = np.zeros(4, dtype=np.int64)
     p = lambda a: a.ctypes.data  # noqa: E731
-    args = (batch.count, p(batch.lengths), p(batch.slots), p(batch.sources), rows, by_length)
+    args = (batch.count, p(batch.lengths), p(batch.slots), p(batch.sources), rows, scan)
     n = lib.vmscan_request_pieces(*args, None, 0, p(info))
-    table = np.full(8 * n + 4 * int(info[1]) + 8, 77, dtype=np.int32)
-    assert lib.vmscan_request_pieces(*args, p(table), 8 * n + 4 * int(info[1]), p(info)) == n
-    assert (table[8 * n + 4 * int(info[1]):] == 77).all()  # writes what it counted
-    assert lib.vmscan_request_pieces(*args, p(table), 8 * n + 4 * int(info[1]) - 1, p(info)) == -6
-    return table[:8 * n].reshape(n, 8), table[8 * n:8 * n + 4 * int(info[1])].reshape(-1, 4), info
+    size = 8 * n + 4 * int(info[1])
+    table = np.full(size + 8, 77, dtype=np.int32)
+    assert lib.vmscan_request_pieces(*args, p(table), size, p(info)) == n
+    assert (table[size:] == 77).all()  # writes what it counted
+    assert lib.vmscan_request_pieces(*args, p(table), size - 1, p(info)) == -6
+    return table[:8 * n].reshape(n, 8), table[8 * n:size].reshape(-1, 4), info
 
 
-@pytest.mark.parametrize("by_length", [0, 1])
+@pytest.mark.parametrize("scan", [0, 1])
 @pytest.mark.parametrize("rows", [0, 1, 7, 8, 32, 64, 1000])
 @pytest.mark.parametrize("lengths", [[1], [0], [0, 0, 3], [65, 0, 1, 64, 63, 200], [1000], [8, 9, 7, 16, 17]])
-def test_pieces_cover_every_row_once(lengths, rows, by_length):
+def test_pieces_cover_every_row_once(lengths, rows, scan):
     n = len(lengths)
     slots = [i if i != 2 else -1 for i in range(n)]
     batch = RequestBatch(lengths, slots=slots, sources=[(n + i) if i % 2 else -1 for i in range(n)])
-    pieces, chains, info = _pieces(batch, rows, by_length)
+    pieces, chains, info = _pieces(batch, rows, scan)
+    first, later = pieces[:int(info[0])], pieces[int(info[0]):]
     begins = np.concatenate([[0], np.cumsum(lengths)])
-    seen = np.zeros(int(begins[-1]), dtype=int)
+    written = np.zeros(int(begins[-1]), dtype=int)
     owners = {}
-    for t0, t1, begin, end, source, slot, carry, later in pieces:
-        assert begin <= t0 <= t1 <= end
-        assert rows == 0 or t1 - t0 <= max(rows, (rows + 7) // 8 * 8 if by_length else rows)
-        seen[t0:t1] += 1
-        assert t1 > t0 or begin == end  # only an empty request has an empty piece
-        owners.setdefault((begin, end, slot), []).append((t0, t1, source, carry, later))
-    assert (seen == 1).all()
-    assert len(pieces) >= n
+    for phase, group in enumerate((first, later)):
+        for t0, t1, begin, end, source, slot, carry, ordinal in group:
+            assert begin <= t0 <= t1 <= end and (t1 > t0 or begin == end)  # only an empty request has an empty piece
+            assert rows == 0 or t1 - t0 <= ((rows + 7) // 8 * 8 if scan else rows)
+            if not (phase == 0 and carry >= 0 and ordinal > 0):  # a carry writes no rows
+                written[t0:t1] += 1
+                owners.setdefault((begin, end, slot), []).append((ordinal, t0, t1, source, carry, phase))
+            else:
+                assert [t0, t1, begin, end, source, slot, carry, ordinal] in later.tolist() and t1 < end
+    assert (written == 1).all()
     used = []
     for i in range(n):
         mine = sorted(owners[(begins[i], begins[i + 1], slots[i])])
-        assert mine[0][0] == begins[i] and mine[-1][1] == begins[i + 1]
-        assert all(m[2] == batch.sources[i] for m in mine)
-        if len(mine) == 1:
-            assert mine[0][3] == -1 and mine[0][4] == 0
+        assert [m[0] for m in mine] == list(range(len(mine)))
+        assert mine[0][1] == begins[i] and mine[-1][2] == begins[i + 1]
+        assert all(m[3] == batch.sources[i] for m in mine)
+        if scan:
+            assert [m[5] for m in mine] == [0] + [1] * (len(mine) - 1)
+        if not scan or len(mine) == 1:
+            assert all(m[4] == -1 for m in mine)
         else:
-            carries = [m[3] for m in mine]
+            carries = [m[4] for m in mine]
             assert carries == list(range(carries[0], carries[0] + len(mine)))
-            assert [m[4] for m in mine] == [1] * (len(mine) - 1) + [0]
-            assert [carries[0], len(mine), batch.sources[i], 0] in chains.tolist()
+            assert [carries[0], len(mine), 0, 0] in chains.tolist() and len(mine) <= info[3]
+            # the pieces between the first and the last one leave a carry in the first phase
+            assert sorted(r[7] for r in first.tolist() if r[6] in carries) == list(range(len(mine) - 1))
             used += carries
     assert sorted(used) == list(range(int(info[2]))) and len(chains) == info[1]
-    assert (pieces[:, 7] == 1).sum() == info[0]
-    if by_length:  # pieces with a carry first, then by length
-        assert (pieces[:int(info[0]), 7] == 1).all()
-        rest = (pieces[:, 1] - pieces[:, 0])[int(info[0]):]
-        assert (np.diff(rest) <= 0).all()
+    if scan:  # long pieces first
+        assert (np.diff(first[:, 1] - first[:, 0]) <= 0).all() and (np.diff(later[:, 1] - later[:, 0]) <= 0).all()
     else:
-        assert (np.diff(pieces[:, 0]) >= 0).all()
+        assert len(later) == 0 and (np.diff(pieces[:, 0]) >= 0).all()
 
 
 def test_scan_rows_rule():
@@ -112,12 +117,12 @@ def test_scan_rows_rule():
 
     def rows(lengths, dn):
         a = np.asarray(lengths, np.int32)
-        return lib.vmscan_cached_scan_rows(a.size, a.ctypes.data, dn)
+        return lib.vmscan_cached_scan_rows(a.size, a.ctypes.data, dn, 0)
 
     assert 0 < rows([32768], 768) < 8192
     assert rows([512] * 256, 1536) == 0
     assert rows([1] * 10, 64) == 0
-    assert lib.vmscan_cached_scan_rows(0, None, 64) == -2
+    assert lib.vmscan_cached_scan_rows(0, None, 64, 0) == -2
 
 
 @pytest.mark.parametrize("lengths", [[1] * 40, [100, 0, 3, 17, 16, 1], [0, 0]])
@@ -166,18 +171,18 @@ def test_c_entry_points_validate():
     P = 4096
     scan = lambda **o: lib.vmscan_cached_scan(*[{**dict(  # noqa: E731
         rows=4, dn=8, ds=16, bf16=0, u=P, ldu=8, dl=P, ldd=8, A=P, B=P, ldb=16, C=P, ldc=16, D=P, z=None, ldz=0, y=P,
-        ldy=8, state=P, slots=2, pieces=P, n=1, nc=0, chains=None, nch=0, cr=0, ws=None, wn=0, stream=None), **o}[k]
-        for k in ("rows dn ds bf16 u ldu dl ldd A B ldb C ldc D z ldz y ldy state slots pieces n nc chains nch cr ws wn "
+        ldy=8, state=P, slots=2, pieces=P, n=1, nf=1, chains=None, nch=0, cr=0, lc=1, ws=None, wn=0, stream=None), **o}[k]
+        for k in ("rows dn ds bf16 u ldu dl ldd A B ldb C ldc D z ldz y ldy state slots pieces n nf chains nch cr lc ws wn "
                   "stream").split()])
     assert scan(ds=8) == 3
     assert scan(A=None) == 1 and scan(u=None) == 1 and scan(state=None) == 1 and scan(pieces=None) == 1
     assert scan(dn=0) == 2 and scan(rows=-1) == 2 and scan(slots=0) == 2 and scan(ldy=7) == 2 and scan(ldu=-8) == 2
-    assert scan(n=0) == 2 and scan(n=1, nc=2) == 2 and scan(cr=3) == 2
+    assert scan(n=0) == 2 and scan(n=1, nf=2) == 2 and scan(nf=0) == 2 and scan(cr=3) == 2 and scan(n=2) == 2
     assert scan(A=P + 4) == 4 and scan(state=P + 8) == 4 and scan(pieces=P + 4) == 4
-    assert scan(n=4, nc=2, chains=P, nch=1, cr=3) == 6  # no workspace
+    assert scan(n=4, nf=2, chains=P, nch=1, cr=3) == 6  # no workspace
     need = lib.vmscan_cached_scan_workspace_bytes(8, 3)
     assert need >= 3 * 8 * 33 * 4
-    assert scan(n=4, nc=2, chains=P, nch=1, cr=3, ws=P, wn=need - 1) == 6
+    assert scan(n=4, nf=2, chains=P, nch=1, cr=3, ws=P, wn=need - 1) == 6
     assert lib.vmscan_cached_scan_workspace_bytes(0, 3) == -2
     step = lambda **o: lib.vmscan_cached_step(*[{**dict(  # noqa: E731
         rows=4, dn=8, ds=16, bf16=0, u=P, ldu=8, dl=P, ldd=8, A=P, B=P, ldb=16, C=P, ldc=16, D=P, z=None, ldz=0, y=P,
