@@ -342,7 +342,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (b.tokens > 0) {
     vmscan_stream_t stream = stream_of(b);
     Range range(where);
-    const Table t = table_of(b, g_names.lora, stream, 0);
+    const Table t = table_of(b, g_names.lora, stream, count);
     const int64_t tiles = t.info[0];
     check(vmscan_lora_add(rows, d_in, d_out, rank, count, dt == at::kBFloat16, x_.data_ptr(), x_.stride(0), a.data_ptr(),
                           bb.data_ptr(), static_cast<const float*>(scale.data_ptr()), base_.data_ptr(), base_.stride(0),

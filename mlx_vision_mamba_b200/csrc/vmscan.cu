@@ -1452,23 +1452,36 @@ int launch_cached_conv(const CachedConvArgs& a, const int32_t* pieces, int64_t n
   return check_launch();
 }
 
-template <typename T>
-int launch_lora(LoraArgs& l, int n_tiles, cudaStream_t s) {
-  l.wide_in = row_grain<T>(l.x, l.ldx, l.d_in) == 16 && row_grain<T>(l.a, l.d_in, l.d_in) == 16;
-  l.wide_rank = l.rank % 4 == 0 && four_wide<T>(l.b, l.rank);
-  l.wide_out = l.d_out % 4 == 0 && four_wide<T>(l.base, l.ldbase) && four_wide<T>(l.out, l.ldout);
-  // column shares (of whole 64-column rounds of the CTA's warps): enough that
-  // a few tiles still occupy the SMs; each share forms the rank-wide products
-  // of its tile again
-  const int rounds = (l.d_out + 16 * LORA_WARPS - 1) / (16 * LORA_WARPS);
-  const int shares = std::max(1, std::min(rounds, 2 * sm_count() / n_tiles));
+template <typename T, bool WIDE, int STEPS>
+int launch_lora(const LoraArgs& l, int n_tiles, cudaStream_t s) {
+  // column shares (of whole 64-column rounds of the CTA's warps): a few tiles
+  // are spread over four CTAs an SM; each share forms the rank-wide products of
+  // its tile again, which from two tiles an SM on costs more than it brings
+  // (520 tiles 384 -> 1536, rank 16: 62 us in one share, 69 in two; 35 tiles:
+  // 10.2 us in four shares, 8.5 in all 24)
+  const int rounds = (l.d_out + 16 * LORA_WARPS - 1) / (16 * LORA_WARPS), sms = sm_count();
+  const int shares = n_tiles >= 2 * sms ? 1 : std::min(rounds, (4 * sms + n_tiles - 1) / n_tiles);
   const int cols = (rounds + shares - 1) / shares * 16 * LORA_WARPS;
   const size_t smem = lora_smem<T>(l.rank);
-  if (cudaFuncSetAttribute(lora_add_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           int(lora_smem<T>(LORA_RMAX))) != cudaSuccess)
+  auto kern = lora_add_kernel<T, WIDE, STEPS>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(lora_smem<T>(LORA_RMAX))) != cudaSuccess)
     return fail(VMSCAN_ERR_LAUNCH, "cudaFuncSetAttribute(lora_add_kernel) failed");
-  lora_add_kernel<T><<<dim3(unsigned(n_tiles), unsigned((l.d_out + cols - 1) / cols)), LORA_WARPS * 32, smem, s>>>(l, cols);
+  kern<<<dim3(unsigned(n_tiles), unsigned((l.d_out + cols - 1) / cols)), LORA_WARPS * 32, smem, s>>>(l, cols);
   return check_launch();
+}
+
+// Rows that do not start on whole accesses take one kernel of scalar accesses;
+// ranks of up to 16, 32 and 64 keep a group's share of B in registers.
+template <typename T>
+int run_lora(const LoraArgs& l, int n_tiles, cudaStream_t s) {
+  const bool wide = row_grain<T>(l.x, l.ldx, l.d_in) == 16 && row_grain<T>(l.a, l.d_in, l.d_in) == 16 &&
+                    l.rank % 4 == 0 && four_wide<T>(l.b, l.rank) && l.d_out % 4 == 0 &&
+                    four_wide<T>(l.base, l.ldbase) && four_wide<T>(l.out, l.ldout);
+  if (!wide) return launch_lora<T, false, 0>(l, n_tiles, s);
+  if (l.rank <= 16) return launch_lora<T, true, 1>(l, n_tiles, s);
+  if (l.rank <= 32) return launch_lora<T, true, 2>(l, n_tiles, s);
+  if (l.rank > 48 && l.rank <= 64) return launch_lora<T, true, 4>(l, n_tiles, s);
+  return launch_lora<T, true, 0>(l, n_tiles, s);
 }
 
 }  // namespace
@@ -1663,14 +1676,17 @@ int64_t vmscan_lora_tiles(int64_t count, const int32_t* lengths, const int32_t* 
   const int rc = check_requests(count, lengths, adapters, adapters);
   if (rc != VMSCAN_OK) return -rc;
   if (n_adapters < 0 || n_adapters > INT32_MAX) return -VMSCAN_ERR_SHAPE;
-  int64_t most = 0;  // tiles when no two requests share an adapter
+  int64_t most = 0, rows = 0;  // tiles when no two requests share an adapter
   for (int64_t i = 0; i < count; ++i) {
     if (adapters[i] < -1 || adapters[i] >= n_adapters) {
       fail(VMSCAN_ERR_SHAPE, "request %lld has adapter %d of %lld", (long long)i, adapters[i], (long long)n_adapters);
       return -VMSCAN_ERR_SHAPE;
     }
     most += (lengths[i] + LORA_ROWS - 1) / LORA_ROWS;
+    rows += lengths[i];
   }
+  // each adapter, and none, adds at most one tile that is not full
+  most = std::min(most, rows / LORA_ROWS + n_adapters + 1);
   if (tiles == nullptr || row_index == nullptr) return most;
   if (tile_capacity < most) return -VMSCAN_ERR_WORKSPACE;
   // requests by adapter, then by position: {adapter, first row, rows}
@@ -1727,9 +1743,9 @@ int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int
   VM_TRY(ensure_context(out));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   LoraArgs l{x, a, b, base, out, scale, row_index, tiles, ldx, ldbase, ldout, int(rows), int(d_in), int(d_out),
-             int(rank), int(n_adapters), int(n_index), 0, 0, 0};
-  if (bf16) return launch_lora<__nv_bfloat16>(l, int(n_tiles), s);
-  return launch_lora<float>(l, int(n_tiles), s);
+             int(rank), int(n_adapters), int(n_index)};
+  if (bf16) return run_lora<__nv_bfloat16>(l, int(n_tiles), s);
+  return run_lora<float>(l, int(n_tiles), s);
 }
 
 }  // extern "C"

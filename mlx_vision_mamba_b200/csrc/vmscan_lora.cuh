@@ -42,7 +42,6 @@ struct LoraArgs {
   const int32_t* tiles;
   int64_t ldx, ldbase, ldout;
   int rows, d_in, d_out, rank, adapters, n_index;
-  int wide_in, wide_rank, wide_out;  // 16-byte (x, A), 4-element (B), 4-element (base, out) accesses fit
 };
 
 __device__ __forceinline__ void mma_tf32(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -62,10 +61,10 @@ struct Chunk {
   static constexpr int N = 16 / int(sizeof(T));
   uint32_t w[4];
 };
-template <typename T>
-__device__ __forceinline__ Chunk<T> ld_chunk(const T* row, int c, int limit, bool wide) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ Chunk<T> ld_chunk(const T* row, int c, int limit) {
   Chunk<T> k;
-  if (wide) {  // limit is a multiple of N: a chunk is inside or outside
+  if constexpr (WIDE) {  // limit is a multiple of N: a chunk is inside or outside
     const uint4 q = c < limit ? __ldg(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
     k.w[0] = q.x, k.w[1] = q.y, k.w[2] = q.z, k.w[3] = q.w;
   } else if constexpr (sizeof(T) == 4) {
@@ -90,11 +89,11 @@ struct Four {
 };
 // Ordinary loads (base may be the output: no read-only path), which the
 // compiler may still move across the stores of other columns.
-template <typename T>
-__device__ __forceinline__ Four<T> ld_quad(const T* row, int c, int limit, bool wide) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ Four<T> ld_quad(const T* row, int c, int limit) {
   Four<T> k;
   if constexpr (sizeof(T) == 4) {
-    if (wide) {
+    if constexpr (WIDE) {
       k.w[0] = k.w[1] = k.w[2] = k.w[3] = 0;
       if (c < limit)
         asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -105,7 +104,7 @@ __device__ __forceinline__ Four<T> ld_quad(const T* row, int c, int limit, bool 
       for (int i = 0; i < 4; ++i) k.w[i] = c + i < limit ? __float_as_uint(row[c + i]) : 0u;
     }
   } else {
-    if (wide) {
+    if constexpr (WIDE) {
       k.w[0] = k.w[1] = 0;
       if (c < limit) asm("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(k.w[0]), "=r"(k.w[1]) : "l"(row + c));
     } else {
@@ -132,10 +131,10 @@ __device__ __forceinline__ float4 four_f(const Four<T>& k) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void st_quad(T* row, int c, int limit, bool wide, const float4& v) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ void st_quad(T* row, int c, int limit, const float4& v) {
   if constexpr (sizeof(T) == 4) {
-    if (wide) {
+    if constexpr (WIDE) {
       if (c < limit) *reinterpret_cast<float4*>(row + c) = v;
       return;
     }
@@ -145,7 +144,7 @@ __device__ __forceinline__ void st_quad(T* row, int c, int limit, bool wide, con
     if (c + 3 < limit) row[c + 3] = v.w;
   } else {
     const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    if (wide) {
+    if constexpr (WIDE) {
       uint2 q;
       q.x = *reinterpret_cast<const uint32_t*>(&a);
       q.y = *reinterpret_cast<const uint32_t*>(&b);
@@ -176,28 +175,38 @@ constexpr size_t lora_smem(int rank) {
           size_t(2) * ((rank + 15) / 16) * 32 * 4 * LoraFrag<T>::GROUPS) * 4;
 }
 
-// MT: 16-row blocks of the tile in use.
-template <typename T, int MT>
+// MT: 16-row blocks of the tile in use.  WIDE: every row of x, A, B, base and
+// out starts on a whole access (16 bytes; B, base and out four elements).
+// STEPS: 16-column steps of the rank, 0: any number.
+template <typename T, bool WIDE, int MT, int STEPS>
 __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int n, int ad, int c_begin, int c_end,
                                           float* part, uint32_t* frag) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   constexpr int CN = Chunk<T>::N;
+  constexpr int NT = STEPS == 1 ? 2 : LORA_RCHUNK / 8;  // 8-column blocks of S a warp holds
   int r[2 * MT];  // rows g, g + 8, ... of the tile; those past the last repeat it
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i) r[i] = row[min(g + 8 * i, n - 1)];
-  const int steps = (a.rank + 15) / 16;
+  const int steps = STEPS > 0 ? STEPS : (a.rank + 15) / 16;
   if (ad >= 0) {
     const T* A = static_cast<const T*>(a.a) + int64_t(ad) * a.rank * a.d_in;
+    const T* xr[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) xr[i] = static_cast<const T*>(a.x) + r[i] * a.ldx;
     const float scale = a.scale[ad];
     for (int rc = 0; rc < a.rank; rc += LORA_RCHUNK) {
-      float acc[MT][4][4] = {};
-      const int nt = min(4, (a.rank - rc + 7) / 8);  // 8-column blocks of this chunk
+      float acc[MT][NT][4] = {};
+      const int nt = min(NT, (a.rank - rc + 7) / 8);
+      const T* ar[NT];  // row of A whose products this lane's B fragments hold
+#pragma unroll
+      for (int j = 0; j < NT; ++j) ar[j] = A + int64_t(min(rc + 8 * j + g, a.rank - 1)) * a.d_in;
 #pragma unroll 2
       for (int c = (warp * 4 + t) * CN; c - t * CN < a.d_in; c += LORA_WARPS * 4 * CN) {
-        Chunk<T> x[2 * MT];
+        Chunk<T> x[2 * MT], ab[NT];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)
-          x[i] = ld_chunk(static_cast<const T*>(a.x) + r[i] * a.ldx, c, a.d_in, a.wide_in != 0);
+        for (int i = 0; i < 2 * MT; ++i) x[i] = ld_chunk<T, WIDE>(xr[i], c, a.d_in);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ab[j] = ld_chunk<T, WIDE>(ar[j], c, a.d_in);  // rows past the rank: never summed
         uint32_t xl[2 * MT][4];
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -210,11 +219,9 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NT; ++j) {
           if (j < nt) {
-            const int k = rc + 8 * j + g;
-            Chunk<T> b{};
-            if (k < a.rank) b = ld_chunk(A + int64_t(k) * a.d_in, c, a.d_in, a.wide_in != 0);
+            const Chunk<T>& b = ab[j];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // words 2h and 2h + 1 of the chunk are one step of the product
               uint32_t bh[2] = {b.w[2 * h], b.w[2 * h + 1]}, bl[2];
@@ -250,7 +257,7 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NT; ++j)
           if (j < nt) {
             float* p = part + (warp * LORA_ROWS + 16 * m + g) * LD + 8 * j + 2 * t;
             p[0] = acc[m][j][0];
@@ -259,7 +266,7 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
             p[8 * LD + 1] = acc[m][j][3];
           }
       __syncthreads();
-      const int here = min(2, steps - rc / 16);  // 16-column steps of this chunk
+      const int here = min(NT / 2, steps - rc / 16);  // 16-column steps of this chunk
       for (int e = threadIdx.x; e < MT * here * 32; e += LORA_WARPS * 32) {
         const int fl = e & 31, s = (e >> 5) % here, m = (e >> 5) / here;
         const int fr = 16 * m + (fl >> 2), fc = 16 * s + 4 * (fl & 3);
@@ -301,69 +308,99 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
           }
         }
       }
-      __syncthreads();
+      if (rc + LORA_RCHUNK < a.rank) __syncthreads();  // part is read before the next chunk's is written
     }
   }
   // columns in groups of 16: lane t of a quad owns columns 4t .. 4t + 3 of its
   // rows, which are columns 2t, 2t + 1 of the group's two 8-column blocks
   const T* B = static_cast<const T*>(a.b) + int64_t(max(ad, 0)) * a.d_out * a.rank;
-#pragma unroll 2
-  for (int c0 = c_begin + 16 * warp; c0 < c_end; c0 += 16 * LORA_WARPS) {
-    Four<T> base[2 * MT];
+  const T* br[2 * MT];
+  T* outr[2 * MT];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i)
-      base[i] = ld_quad(static_cast<const T*>(a.base) + r[i] * a.ldbase, c0 + 4 * t, a.d_out, a.wide_out != 0);
+  for (int i = 0; i < 2 * MT; ++i) {
+    br[i] = static_cast<const T*>(a.base) + r[i] * a.ldbase;
+    outr[i] = static_cast<T*>(a.out) + r[i] * a.ldout;
+  }
+  constexpr int HELD = STEPS == 0 ? 1 : STEPS;  // steps of B loaded together
+  struct Group {
+    Four<T> base[2 * MT], b[HELD][2];
+  };
+  auto load_b = [&](int c0, int s, Four<T> b[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = c0 + 4 * (g >> 1) + (g & 1) + 2 * j;
+      b[j] = ld_quad<T, WIDE>(B + int64_t(min(col, a.d_out - 1)) * a.rank, 16 * s + 4 * t, a.rank);
+    }
+  };
+  auto load = [&](int c0, Group& k) {
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) k.base[i] = ld_quad<T, WIDE>(br[i], c0 + 4 * t, a.d_out);
+    if (STEPS > 0 && ad >= 0) {
+#pragma unroll
+      for (int s = 0; s < HELD; ++s) load_b(c0, s, k.b[s]);
+    }
+  };
+  auto multiply = [&](const Four<T> b[2], int s, float acc[MT][2][4]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const uint4* f = reinterpret_cast<const uint4*>(frag) + size_t(m * steps + s) * LoraFrag<T>::GROUPS * 32 + lane;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 fh = f[32 * h], fl = f[32 * (2 + h)];
+          const uint32_t sh[4] = {fh.x, fh.y, fh.z, fh.w}, sl[4] = {fl.x, fl.y, fl.z, fl.w};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t h0 = tf32_hi(b[j].w[2 * h]), h1 = tf32_hi(b[j].w[2 * h + 1]);
+            mma_tf32(acc[m][j], sl, h0, h1);
+            mma_tf32(acc[m][j], sh, tf32_lo(b[j].w[2 * h], h0), tf32_lo(b[j].w[2 * h + 1], h1));
+            mma_tf32(acc[m][j], sh, h0, h1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int w = 2; w >= 0; --w) {
+          const uint4 fw = f[32 * w];
+          const uint32_t sw[4] = {fw.x, fw.y, fw.z, fw.w};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma_bf16(acc[m][j], sw, b[j].w[0], b[j].w[1]);
+        }
+      }
+    }
+  };
+  constexpr int STEP = 16 * LORA_WARPS;
+  Group cur, nxt;
+  if (c_begin + 16 * warp < c_end) load(c_begin + 16 * warp, cur);
+  if (ad >= 0) __syncthreads();  // S is complete
+  for (int c0 = c_begin + 16 * warp; c0 < c_end; c0 += STEP) {
+    if (c0 + STEP < c_end) load(c0 + STEP, nxt);
     float acc[MT][2][4] = {};
     if (ad >= 0) {
-      for (int s = 0; s < steps; ++s) {
-        Four<T> b[2];
+      if constexpr (STEPS > 0) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col = c0 + 4 * (g >> 1) + (g & 1) + 2 * j;
-          b[j] = Four<T>{};
-          if (col < a.d_out) b[j] = ld_quad(B + int64_t(col) * a.rank, 16 * s + 4 * t, a.rank, a.wide_rank != 0);
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint4* f = reinterpret_cast<const uint4*>(frag) + size_t(m * steps + s) * LoraFrag<T>::GROUPS * 32 + lane;
-          if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4 fh = f[32 * h], fl = f[32 * (2 + h)];
-              const uint32_t sh[4] = {fh.x, fh.y, fh.z, fh.w}, sl[4] = {fl.x, fl.y, fl.z, fl.w};
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const uint32_t h0 = tf32_hi(b[j].w[2 * h]), h1 = tf32_hi(b[j].w[2 * h + 1]);
-                mma_tf32(acc[m][j], sl, h0, h1);
-                mma_tf32(acc[m][j], sh, tf32_lo(b[j].w[2 * h], h0), tf32_lo(b[j].w[2 * h + 1], h1));
-                mma_tf32(acc[m][j], sh, h0, h1);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int w = 2; w >= 0; --w) {
-              const uint4 fw = f[32 * w];
-              const uint32_t sw[4] = {fw.x, fw.y, fw.z, fw.w};
-#pragma unroll
-              for (int j = 0; j < 2; ++j) mma_bf16(acc[m][j], sw, b[j].w[0], b[j].w[1]);
-            }
-          }
+        for (int s = 0; s < STEPS; ++s) multiply(cur.b[s], s, acc);
+      } else {
+#pragma unroll 2
+        for (int s = 0; s < steps; ++s) {
+          Four<T> b[2];
+          load_b(c0, s, b);
+          multiply(b, s, acc);
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
-      const float4 v = four_f(base[i]);
+      const float4 v = four_f(cur.base[i]);
       const float* p0 = &acc[i >> 1][0][2 * (i & 1)];
       const float* p1 = &acc[i >> 1][1][2 * (i & 1)];
       if (g + 8 * i < n)
-        st_quad(static_cast<T*>(a.out) + r[i] * a.ldout, c0 + 4 * t, a.d_out, a.wide_out != 0,
-                make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]));
+        st_quad<T, WIDE>(outr[i], c0 + 4 * t, a.d_out, make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]));
     }
+    cur = nxt;
   }
 }
 
-template <typename T>
+template <typename T, bool WIDE, int STEPS>
 __global__ void __launch_bounds__(LORA_WARPS * 32) lora_add_kernel(const LoraArgs a, int cols_per_cta) {
   extern __shared__ __align__(16) unsigned char lora_raw[];
   __shared__ int row[LORA_ROWS];
@@ -379,9 +416,9 @@ __global__ void __launch_bounds__(LORA_WARPS * 32) lora_add_kernel(const LoraArg
   __syncthreads();
   const int c0 = blockIdx.y * cols_per_cta, c1 = min(c0 + cols_per_cta, a.d_out);
   if (n > 16)
-    lora_tile<T, 2>(a, row, n, ad, c0, c1, part, frag);
+    lora_tile<T, WIDE, 2, STEPS>(a, row, n, ad, c0, c1, part, frag);
   else
-    lora_tile<T, 1>(a, row, n, ad, c0, c1, part, frag);
+    lora_tile<T, WIDE, 1, STEPS>(a, row, n, ad, c0, c1, part, frag);
 }
 
 }  // namespace vmscan

@@ -154,15 +154,13 @@ class RequestBatch:
         if kind == "step":
             return _pinned(np.concatenate([self.slots, self.sources])), (self.count,)
         if kind == "lora":
-            most = lib.vmscan_lora_tiles(self.count, ptr(self.lengths), ptr(self.adapters), self.max_adapter + 1, None,
-                                         None, 0)
+            most = lib.vmscan_lora_tiles(self.count, ptr(self.lengths), ptr(self.adapters), arg, None, None, 0)
             if most < 0:
                 _native.check(-most, "vmscan_lora_tiles")
             table = np.empty(4 * most + self.tokens, dtype=np.int32)
             if self.tokens:
-                _check_count(lib.vmscan_lora_tiles(self.count, ptr(self.lengths), ptr(self.adapters),
-                                                   self.max_adapter + 1, ptr(table) + 16 * most, ptr(table), most),
-                             "vmscan_lora_tiles")
+                _check_count(lib.vmscan_lora_tiles(self.count, ptr(self.lengths), ptr(self.adapters), arg,
+                                                   ptr(table) + 16 * most, ptr(table), most), "vmscan_lora_tiles")
             return _pinned(table), (int(most),)
         if kind == "scan":
             rows, scan = lib.vmscan_cached_scan_rows(self.count, ptr(self.lengths), arg // 2, arg % 2), 1
