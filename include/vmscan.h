@@ -472,9 +472,10 @@ int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16,
  * its first one taken from the K - 1 rows of its source slot, and its last
  * K - 1 rows into its slot of `state` (n_slots, K - 1, channels), oldest row
  * first, in the type of x (an exact copy).  weight (channels, K, 1), K in
- * 1..8.  pieces: of at most vmscan_cached_conv_rows() rows, in row order.
+ * 1..8.  pieces: in row order, of vmscan_cached_conv_rows(rows, channels) rows
+ * (host only: the faster length for that size; at least 8 is required).
  */
-int vmscan_cached_conv_rows(void);
+int64_t vmscan_cached_conv_rows(int64_t rows, int64_t channels);
 int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int bf16, const void* x, int64_t ldx,
                               const float* weight, const float* bias, void* out, int64_t ldo, void* state,
                               int64_t n_slots, const int32_t* pieces, int64_t n_pieces, vmscan_stream_t stream);

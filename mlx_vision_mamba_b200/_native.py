@@ -137,7 +137,7 @@ SIGNATURES = {
         [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64,
          _p, _p, _p],
     ),
-    "vmscan_cached_conv_rows": (ctypes.c_int, []),
+    "vmscan_cached_conv_rows": (_i64, [_i64, _i64]),
     "vmscan_cached_conv1d_silu": (
         ctypes.c_int,
         [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p],

@@ -269,7 +269,7 @@ PyObject* conv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::Tensor out = out_rows(x, b);
   vmscan_stream_t stream = stream_of(b);
   Range range(where);
-  const Table t = table_of(b, g_names.conv, stream, 0);
+  const Table t = table_of(b, g_names.conv, stream, c);
   check(vmscan_cached_conv1d_silu(rows, c, k, x.scalar_type() == at::kBFloat16, x_.data_ptr(), x_.stride(0),
                                   static_cast<const float*>(w_.data_ptr()), static_cast<const float*>(b_.data_ptr()),
                                   out.data_ptr(), c, state.data_ptr(), state.size(0), i32(t.ptr), t.info[0], stream),

@@ -506,12 +506,13 @@ __global__ void __launch_bounds__(CST_WARPS * 32)
 // ---------------------------------------------------------------------------
 // Causal conv1d + SiLU.  A thread owns VEC adjacent channels of one piece and
 // slides the K-row window along its rows.  The first piece of a request (and
-// the only one that can reach rows before it: pieces hold CCV_ROWS >= K - 1
+// the only one that can reach rows before it: pieces hold at least K - 1
 // rows) reads the stored window, and writes the new one: the request's last
 // K - 1 rows, reaching back into the old window when it has fewer.  The same
 // thread reads the old window before it writes, so a slot may be both.
 // ---------------------------------------------------------------------------
-constexpr int CCV_ROWS = 32;
+constexpr int CCV_ROWS = 32;       // rows of a piece
+constexpr int CCV_FEW_ROWS = 16;   // where those would give the SMs too few threads (both at least K - 1)
 constexpr int CCV_THREADS = 64;
 constexpr int CCV_KMAX = 8;
 constexpr int CCV_AHEAD = 8;  // rows whose loads are issued together
@@ -555,14 +556,12 @@ struct CachedConvArgs {
   int rows, channels, K;
 };
 
-// KW: window slots (4 or 8, at least K); the K taps sit at the newest end.
-template <typename T, int VEC, int KW>
+template <typename T, int VEC, int K>
 __global__ void __launch_bounds__(CCV_THREADS)
     cached_conv_kernel(const CachedConvArgs a, const int32_t* __restrict__ pieces, int groups) {
   const Piece p = load_piece(pieces, blockIdx.x / groups, a.rows, a.n_slots);
   const int c = ((blockIdx.x % groups) * CCV_THREADS + threadIdx.x) * VEC;
   if (c >= a.channels) return;
-  const int K = a.K;
   T* __restrict__ out = static_cast<T*>(a.out) + c;
   if (p.slot < 0) {
     const float zero[VEC] = {};
@@ -572,60 +571,52 @@ __global__ void __launch_bounds__(CCV_THREADS)
   const T* __restrict__ x = static_cast<const T*>(a.x) + c;
   T* state = static_cast<T*>(a.state) + c;
   const int64_t C = a.channels;
-  float w[KW][VEC], win[KW][VEC], bias[VEC];
-  if (KW == 4 && K == 4) {
+  // the thread's taps lie together: VEC channels x K
+  float w[VEC * K], bias[VEC], win[K][VEC];
+  if constexpr (VEC == 4) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float4 q = *reinterpret_cast<const float4*>(a.w + int64_t(c + v) * 4);
-      w[0][v] = q.x, w[1][v] = q.y, w[KW - 2][v] = q.z, w[KW - 1][v] = q.w;
+    for (int i = 0; i < K; ++i) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(a.w + int64_t(c) * K) + i);
+      w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
     }
   } else {
 #pragma unroll
-    for (int m = 0; m < KW; ++m) {
-      const int k = m - (KW - K);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) w[m][v] = k >= 0 ? a.w[int64_t(c + v) * K + k] : 0.f;
-    }
+    for (int i = 0; i < K; ++i) w[i] = __ldg(a.w + int64_t(c) * K + i);
   }
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) bias[v] = a.bias[c + v];
+  for (int v = 0; v < VEC; ++v) bias[v] = __ldg(a.bias + c + v);
   // rows before the piece: rows of the request, or of the stored window.  Slot
-  // m is row t0 - (KW - m) before the first shift.
+  // m is row t0 - (K - m) before the first shift.
 #pragma unroll
-  for (int m = 0; m < KW; ++m) {
+  for (int m = 1; m < K; ++m) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) win[m][v] = 0.f;
-    const int t = p.t0 - (KW - m);
-    if (m > 0 && KW - m < K) {
-      if (t >= p.begin)
-        ldv<T, VEC>(x + t * a.ldx, win[m]);
-      else if (p.source >= 0)
-        ldv<T, VEC>(state + (int64_t(p.source) * (K - 1) + (K - 1 - (p.begin - t))) * C, win[m]);
-    }
+    const int t = p.t0 - (K - m);
+    if (t >= p.begin)
+      ldv<T, VEC>(x + t * a.ldx, win[m]);
+    else if (p.source >= 0)
+      ldv<T, VEC>(state + (int64_t(p.source) * (K - 1) + (K - 1 - (p.begin - t))) * C, win[m]);
   }
   if (p.t0 == p.begin) {
-    // the new window: its row j is row end - (K - 1) + j of the request, and
+    // the new window: its row m - 1 is row end - (K - m) of the request, and
     // where that lies before the request, the old window's (read above: slot s
-    // is row begin - (KW - s))
+    // is row begin - (K - s))
     const int len = p.end - p.begin;
 #pragma unroll
-    for (int m = 1; m < KW; ++m) {
-      const int j = K - 1 - (KW - m);
-      if (j >= 0) {
-        float v[VEC] = {};
-        const int t = p.end - (KW - m);
-        if (t >= p.begin) {
-          ldv<T, VEC>(x + t * a.ldx, v);
-        } else {
+    for (int m = 1; m < K; ++m) {
+      float v[VEC] = {};
+      const int t = p.end - (K - m);
+      if (t >= p.begin) {
+        ldv<T, VEC>(x + t * a.ldx, v);
+      } else {
 #pragma unroll
-          for (int s = m; s < KW; ++s)
-            if (s == m + len) {
+        for (int s = m; s < K; ++s)
+          if (s == m + len) {
 #pragma unroll
-              for (int q = 0; q < VEC; ++q) v[q] = win[s][q];
-            }
-        }
-        stv<T, VEC>(state + (int64_t(p.slot) * (K - 1) + j) * C, v);
+            for (int q = 0; q < VEC; ++q) v[q] = win[s][q];
+          }
       }
+      stv<T, VEC>(state + (int64_t(p.slot) * (K - 1) + m - 1) * C, v);
     }
   }
   for (int t0 = p.t0; t0 < p.t1; t0 += CCV_AHEAD) {
@@ -639,13 +630,27 @@ __global__ void __launch_bounds__(CCV_THREADS)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
 #pragma unroll
-          for (int m = 0; m < KW - 1; ++m) win[m][v] = win[m + 1][v];
-          win[KW - 1][v] = xs[u][v];
-          acc[v] = bias[v];
-#pragma unroll
-          for (int m = 0; m < KW; ++m) acc[v] = fmaf(w[m][v], win[m][v], acc[v]);
-          acc[v] = silu_f(acc[v]);
+          for (int m = 0; m < K - 1; ++m) win[m][v] = win[m + 1][v];
+          win[K - 1][v] = xs[u][v];
         }
+        if constexpr (VEC == 4) {  // channels in packed pairs
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float2 s = make_float2(bias[2 * q], bias[2 * q + 1]);
+#pragma unroll
+            for (int m = 0; m < K; ++m)
+              s = fma2(make_float2(w[2 * q * K + m], w[(2 * q + 1) * K + m]),
+                       make_float2(win[m][2 * q], win[m][2 * q + 1]), s);
+            acc[2 * q] = s.x;
+            acc[2 * q + 1] = s.y;
+          }
+        } else {
+          acc[0] = bias[0];
+#pragma unroll
+          for (int m = 0; m < K; ++m) acc[0] = fmaf(w[m], win[m][0], acc[0]);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] = silu_f(acc[v]);
         stv<T, VEC>(out + (t0 + u) * a.ldo, acc);
       }
     }

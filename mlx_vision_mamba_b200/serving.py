@@ -165,7 +165,7 @@ class RequestBatch:
         if kind == "scan":
             rows, scan = lib.vmscan_cached_scan_rows(self.count, ptr(self.lengths), arg // 2, arg % 2), 1
         else:
-            rows, scan = lib.vmscan_cached_conv_rows(), 0
+            rows, scan = lib.vmscan_cached_conv_rows(self.tokens, arg), 0
         if rows < 0:
             _native.check(-rows, "vmscan_cached_scan_rows")
         info = np.zeros(4, dtype=np.int64)
