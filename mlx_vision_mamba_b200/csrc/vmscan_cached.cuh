@@ -74,6 +74,20 @@ struct CachedScanArgs {
   int rows, dn;
 };
 
+// Four adjacent elements as fp32; `wide`: the address takes one access.
+template <typename T>
+__device__ __forceinline__ float4 ld_four(const T* p, bool wide) {
+  if (!wide) return make_float4(ld_one(p), ld_one(p + 1), ld_one(p + 2), ld_one(p + 3));
+  if constexpr (sizeof(T) == 4) {
+    return __ldg(reinterpret_cast<const float4*>(p));
+  } else {
+    const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q.x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Prompts: a warp owns 32 channels of one piece.  A lane pair owns two adjacent
 // channels and each lane 8 of the 16 states of both, so a B / C value read from
@@ -117,10 +131,14 @@ template <typename T, int G>
 __device__ __forceinline__ void copy_rows(T* dst, const T* p, int64_t ld, int t0, int last, int lane) {
   constexpr int E = G / int(sizeof(T)), LPR = 32 / E;  // E rows at a time
   static_assert(CSC_ROWS % E == 0, "a copy must not reach past the block's rows");
+  dst += lane / LPR * 32 + lane % LPR * E;
+  if (t0 + CSC_ROWS - 1 <= last) {
+    const T* q = p + (t0 + lane / LPR) * ld;
 #pragma unroll
-  for (int r0 = 0; r0 < CSC_ROWS; r0 += E) {
-    const int r = r0 + lane / LPR;
-    cp_async<G>(dst + r * 32 + lane % LPR * E, p + min(t0 + r, last) * ld);
+    for (int r0 = 0; r0 < CSC_ROWS; r0 += E) cp_async<G>(dst + r0 * 32, q + r0 * ld);
+  } else {
+#pragma unroll
+    for (int r0 = 0; r0 < CSC_ROWS; r0 += E) cp_async<G>(dst + r0 * 32, p + min(t0 + r0 + lane / LPR, last) * ld);
   }
 }
 
@@ -243,8 +261,8 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float4 v = *reinterpret_cast<const float4*>(a.A + off + 4 * j);
-      A2[c][2 * j] = make_float2(v.x, v.y);
-      A2[c][2 * j + 1] = make_float2(v.z, v.w);
+      A2[c][2 * j] = make_float2(v.x * kLog2e, v.y * kLog2e);
+      A2[c][2 * j + 1] = make_float2(v.z * kLog2e, v.w * kLog2e);
       const float4 g = src != nullptr ? *reinterpret_cast<const float4*>(src + off + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
       h[c][2 * j] = make_float2(g.x, g.y);
       h[c][2 * j + 1] = make_float2(g.z, g.w);
@@ -261,7 +279,7 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 g = *reinterpret_cast<const float2*>(k.h + ch * NS + 8 * hb + 2 * j);
-          h[c][j] = fma2(make_float2(expf(A2[c][j].x * sum), expf(A2[c][j].y * sum)), h[c][j], g);
+          h[c][j] = fma2(make_float2(exp2f(A2[c][j].x * sum), exp2f(A2[c][j].y * sum)), h[c][j], g);
         }
       }
     }
@@ -301,10 +319,10 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
     auto decay = [&](int r, Decay& w) {
       w.u = ld_pair(&st.u[r][pc]);
       w.d = ld_pair(&st.dl[r][pc]);
-      const float2 dlog = mul2(w.d, bcast2(kLog2e)), off = bcast2(kEx2ArgBias);
+      const float2 off = bcast2(kEx2ArgBias);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float2 dg = bcast2(c ? dlog.y : dlog.x);
+        const float2 dg = bcast2(c ? w.d.y : w.d.x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 arg = fma2(dg, A2[c][j], off);
@@ -333,7 +351,7 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float2 acc =
-              add2(fma2(C2[1], h[c][1], mul2(C2[0], h[c][0])), fma2(C2[3], h[c][3], mul2(C2[2], h[c][2])));
+              fma2(C2[3], h[c][3], fma2(C2[2], h[c][2], fma2(C2[1], h[c][1], mul2(C2[0], h[c][0]))));
           part[c] = acc.x + acc.y;
         }
         float yy = fmaf(hb ? w.u.y : w.u.x, Dd, pair_scatter(part[0], part[1], hb));
@@ -437,70 +455,92 @@ __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const fl
 }
 
 // ---------------------------------------------------------------------------
-// Single tokens: row i is request i.  A warp owns 32 channels of one row; four
+// Single tokens: row i is request i.  A warp owns 32 channels of R rows; four
 // lanes share a channel (four states each), so the state moves as whole
-// 512-byte warp accesses.
+// 512-byte warp accesses, the R rows' of it in flight together and A read once
+// for them.  In round i the quad g works on channel 8 i + g; a transposing sum
+// over the quad leaves lane 4 g + q the output of channel 8 q + g, its own.
 // ---------------------------------------------------------------------------
 constexpr int CST_WARPS = 4;
 
-template <typename T, bool HAS_Z>
+template <typename T, bool HAS_Z, int R>
 __global__ void __launch_bounds__(CST_WARPS * 32)
     cached_step_kernel(const CachedScanArgs a, const int32_t* __restrict__ slots, const int32_t* __restrict__ sources,
-                       int groups) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x / groups;
+                       int groups, int bc_wide) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int row0 = (blockIdx.x / groups) * R;
   const int d0 = ((blockIdx.x % groups) * CST_WARPS + warp) * 32;
   if (d0 >= a.dn) return;
-  const int d = d0 + lane;
-  const bool ok = d < a.dn;
-  const int slot = slots[row], source = sources[row];
-  T* __restrict__ y = static_cast<T*>(a.y) + row * a.ldy;
-  if (slot < 0 || slot >= a.n_slots) {
-    if (ok) y[d] = from_f<T>(0.f);
-    return;
-  }
-  const int dc = ok ? d : a.dn - 1;
-  const float u = ld_one(static_cast<const T*>(a.u) + row * a.ldu + dc);
-  const float dl = ld_one(static_cast<const T*>(a.delta) + row * a.ldd + dc);
-  const float z = HAS_Z ? ld_one(static_cast<const T*>(a.z) + row * a.ldz + dc) : 0.f;
-  const float Dd = a.D[dc];
-  const int q = lane & 3;
-  float Bq[4], Cq[4];
+  const int own = d0 + 8 * q + g;
+  const bool ok = own < a.dn;
+  const int oc = min(own, a.dn - 1);
+  int slot[R], source[R];
+  float u[R], dl[R], z[R];
+  float4 B4[R], C4[R], h[R][4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    Bq[k] = ld_one(static_cast<const T*>(a.B) + row * a.ldb + 4 * q + k);
-    Cq[k] = ld_one(static_cast<const T*>(a.C) + row * a.ldc + 4 * q + k);
+  for (int r = 0; r < R; ++r) {
+    const int row = min(row0 + r, a.rows - 1);
+    slot[r] = slots[row];
+    source[r] = sources[row];
+    u[r] = ld_one(static_cast<const T*>(a.u) + row * a.ldu + oc);
+    dl[r] = ld_one(static_cast<const T*>(a.delta) + row * a.ldd + oc);
+    z[r] = HAS_Z ? ld_one(static_cast<const T*>(a.z) + row * a.ldz + oc) : 0.f;
+    B4[r] = ld_four(static_cast<const T*>(a.B) + row * a.ldb + 4 * q, bc_wide != 0);
+    C4[r] = ld_four(static_cast<const T*>(a.C) + row * a.ldc + 4 * q, bc_wide != 0);
   }
-  const bool kept = source >= 0 && source < a.n_slots;
-  float mine = 0.f;
+  // rounds past the last channel repeat it and store nothing
+  int64_t at[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = 8 * i + (lane >> 2);  // channel of this round, in the warp's 32
-    const int c = d0 + k;
-    const bool in = c < a.dn;
-    const float du = __shfl_sync(0xffffffffu, dl * u, k);
-    const float dlog = __shfl_sync(0xffffffffu, dl * kLog2e, k);
-    float part = 0.f;
-    if (in) {
-      const float4 A4 = *reinterpret_cast<const float4*>(a.A + int64_t(c) * NS + 4 * q);
-      float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (kept) h = *reinterpret_cast<const float4*>(a.state + (int64_t(source) * a.dn + c) * NS + 4 * q);
-      h.x = fmaf(ex2_approx(fmaf(dlog, A4.x, kEx2ArgBias)), h.x, du * Bq[0]);
-      h.y = fmaf(ex2_approx(fmaf(dlog, A4.y, kEx2ArgBias)), h.y, du * Bq[1]);
-      h.z = fmaf(ex2_approx(fmaf(dlog, A4.z, kEx2ArgBias)), h.z, du * Bq[2]);
-      h.w = fmaf(ex2_approx(fmaf(dlog, A4.w, kEx2ArgBias)), h.w, du * Bq[3]);
-      part = fmaf(Cq[1], h.y, Cq[0] * h.x) + fmaf(Cq[3], h.w, Cq[2] * h.z);
-      *reinterpret_cast<float4*>(a.state + (int64_t(slot) * a.dn + c) * NS + 4 * q) = h;
+  for (int i = 0; i < 4; ++i) at[i] = int64_t(min(d0 + 8 * i + g, a.dn - 1)) * NS + 4 * q;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool kept = source[r] >= 0 && source[r] < a.n_slots;
+    const float* from = a.state + int64_t(kept ? source[r] : 0) * a.dn * NS;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (kept) h[r][i] = *reinterpret_cast<const float4*>(from + at[i]);
     }
-    part += __shfl_xor_sync(0xffffffffu, part, 1);
-    part += __shfl_xor_sync(0xffffffffu, part, 2);
-    // lane l owns channel l of the warp: round l / 8, lane group l % 8
-    const float got = __shfl_sync(0xffffffffu, part, 4 * (lane & 7));
-    if ((lane >> 3) == i) mine = got;
   }
-  float yy = fmaf(u, Dd, mine);
-  if (HAS_Z) yy *= silu_f(z);
-  if (ok) y[d] = from_f<T>(yy);
+  float4 A4[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) A4[i] = *reinterpret_cast<const float4*>(a.A + at[i]);
+  const float Dd = a.D[oc];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row0 + r;
+    if (row >= a.rows) break;
+    T* y = static_cast<T*>(a.y) + row * a.ldy + oc;
+    if (slot[r] < 0 || slot[r] >= a.n_slots) {  // padding request
+      stg_if_t<T>(y, 0.f, ok);
+      continue;
+    }
+    float* to = a.state + int64_t(slot[r]) * a.dn * NS;
+    const float du = dl[r] * u[r], dlog = dl[r] * kLog2e;
+    const float2 B0 = make_float2(B4[r].x, B4[r].y), B1 = make_float2(B4[r].z, B4[r].w);
+    const float2 C0 = make_float2(C4[r].x, C4[r].y), C1 = make_float2(C4[r].z, C4[r].w);
+    float part[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 du2 = bcast2(__shfl_sync(0xffffffffu, du, (lane & ~3) + i));
+      const float2 dg = bcast2(__shfl_sync(0xffffffffu, dlog, (lane & ~3) + i)), off = bcast2(kEx2ArgBias);
+      const float2 e0 = fma2(dg, make_float2(A4[i].x, A4[i].y), off), e1 = fma2(dg, make_float2(A4[i].z, A4[i].w), off);
+      const float2 h0 = fma2(make_float2(ex2_approx(e0.x), ex2_approx(e0.y)), make_float2(h[r][i].x, h[r][i].y),
+                             mul2(du2, B0));
+      const float2 h1 = fma2(make_float2(ex2_approx(e1.x), ex2_approx(e1.y)), make_float2(h[r][i].z, h[r][i].w),
+                             mul2(du2, B1));
+      const float2 s = fma2(C1, h1, mul2(C0, h0));
+      part[i] = s.x + s.y;
+      if (d0 + 8 * i + g < a.dn) *reinterpret_cast<float4*>(to + at[i]) = make_float4(h0.x, h0.y, h1.x, h1.y);
+    }
+    // lane q of the quad keeps the sum of part[q] over the quad
+    const float p0 = (q & 1 ? part[1] : part[0]) + __shfl_xor_sync(0xffffffffu, q & 1 ? part[0] : part[1], 1);
+    const float p1 = (q & 1 ? part[3] : part[2]) + __shfl_xor_sync(0xffffffffu, q & 1 ? part[2] : part[3], 1);
+    const float sum = (q & 2 ? p1 : p0) + __shfl_xor_sync(0xffffffffu, q & 2 ? p0 : p1, 2);
+    float yy = fmaf(u[r], Dd, sum);
+    if (HAS_Z) yy *= silu_f(z[r]);
+    stg_if_t<T>(y, yy, ok);
+  }
 }
 
 // ---------------------------------------------------------------------------
