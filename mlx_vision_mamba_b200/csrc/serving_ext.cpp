@@ -9,6 +9,7 @@
 // Exceptions are the Python ones: TypeError, ValueError, RuntimeError.
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <nvtx3/nvToolsExt.h>
@@ -154,10 +155,11 @@ struct Table {
   int64_t info[5];
 };
 
-Table table_of(const Batch& b, PyObject* kind, void* stream, int64_t arg) {
-  Ref s(PyLong_FromVoidPtr(stream)), a(PyLong_FromLongLong(arg));
-  PyObject* args[4] = {b.self, kind, s.p, a.p};
-  Ref r(PyObject_VectorcallMethod(g_names.table, args, 4, nullptr));
+Table table_of(const Batch& b, PyObject* kind, void* stream, int64_t arg, int64_t slots) {
+  const bool capturing = c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+  Ref s(PyLong_FromVoidPtr(stream)), a(PyLong_FromLongLong(arg)), n(PyLong_FromLongLong(slots));
+  PyObject* args[6] = {b.self, kind, s.p, a.p, capturing ? Py_True : Py_False, n.p};
+  Ref r(PyObject_VectorcallMethod(g_names.table, args, 6, nullptr));
   TORCH_CHECK(PyTuple_Check(r.p) && PyTuple_GET_SIZE(r.p) <= 6, "RequestBatch._table returned no table");
   Table t{};
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(r.p); ++i) {
@@ -217,7 +219,7 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t ldz = z_ == nullptr ? 0 : z_->stride(0);
   Ref single(PyObject_GetAttr(b.self, g_names.single_tokens));
   if (single.p == Py_True) {
-    const Table t = table_of(b, g_names.step, stream, 0);
+    const Table t = table_of(b, g_names.step, stream, 0, state.size(0));
     check(vmscan_cached_step(b.tokens, dn, kState, bf16, x_.data_ptr(), x_.stride(0), d_.data_ptr(), d_.stride(0),
                              static_cast<const float*>(A_.data_ptr()), B_.data_ptr(), B_.stride(0), C_.data_ptr(),
                              C_.stride(0), static_cast<const float*>(D_.data_ptr()), zp, ldz, y.data_ptr(), dn,
@@ -226,7 +228,7 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
           where, "vmscan_cached_step");
     return THPVariable_Wrap(y);
   }
-  const Table t = table_of(b, g_names.scan, stream, 2 * dn + bf16);
+  const Table t = table_of(b, g_names.scan, stream, 2 * dn + bf16, state.size(0));
   const int64_t n = t.info[0], chains = t.info[2], carry_rows = t.info[3];
   at::Tensor ws;
   int64_t ws_bytes = 0;
@@ -269,7 +271,7 @@ PyObject* conv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::Tensor out = out_rows(x, b);
   vmscan_stream_t stream = stream_of(b);
   Range range(where);
-  const Table t = table_of(b, g_names.conv, stream, c);
+  const Table t = table_of(b, g_names.conv, stream, c, state.size(0));
   check(vmscan_cached_conv1d_silu(rows, c, k, x.scalar_type() == at::kBFloat16, x_.data_ptr(), x_.stride(0),
                                   static_cast<const float*>(w_.data_ptr()), static_cast<const float*>(b_.data_ptr()),
                                   out.data_ptr(), c, state.data_ptr(), state.size(0), i32(t.ptr), t.info[0], stream),
@@ -308,6 +310,11 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       rs(PyObject_GetAttr(args[2], g_names.scale));
   const at::Tensor &a = tensor(where, "adapters", ra.p), &bb = tensor(where, "adapters", rb.p),
                    &scale = tensor(where, "adapters", rs.p);
+  VALUE(a.dim() == 3 && bb.dim() == 3 && scale.dim() == 1 && bb.size(0) == a.size(0) && scale.size(0) == a.size(0) &&
+            bb.size(2) == a.size(1) && a.is_contiguous() && bb.is_contiguous() && scale.is_contiguous() &&
+            bb.scalar_type() == a.scalar_type() && scale.scalar_type() == at::kFloat && a.is_cuda() &&
+            bb.device() == a.device() && scale.device() == a.device(),
+        "the adapters' tensors are not as LoraAdapters made them");
   const int64_t rows = x.size(0), count = a.size(0), rank = a.size(1), d_in = a.size(2), d_out = bb.size(1);
   const at::Tensor& base = beside(where, "base", args[0], b.index);
   const at::Tensor* given = args[4] == Py_None ? nullptr : &beside(where, "out", args[4], b.index);
@@ -342,7 +349,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (b.tokens > 0) {
     vmscan_stream_t stream = stream_of(b);
     Range range(where);
-    const Table t = table_of(b, g_names.lora, stream, count);
+    const Table t = table_of(b, g_names.lora, stream, count, 0);
     const int64_t tiles = t.info[0];
     check(vmscan_lora_add(rows, d_in, d_out, rank, count, dt == at::kBFloat16, x_.data_ptr(), x_.stride(0), a.data_ptr(),
                           bb.data_ptr(), static_cast<const float*>(scale.data_ptr()), base_.data_ptr(), base_.stride(0),

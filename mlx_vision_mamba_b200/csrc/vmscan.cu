@@ -788,7 +788,7 @@ int launch_ln_bwd(int rows, int dim, const float* x, int64_t ldx, const float* w
 
 extern "C" {
 
-int vmscan_version(void) { return 100; }
+int vmscan_version(void) { return 101; }
 
 const char* vmscan_strerror(int status) {
   switch (status) {
@@ -1399,8 +1399,9 @@ int launch_cached_scan(const CachedScanArgs& a, const ScanPieces& q, const Cache
   if (q.n == q.n_first) return VMSCAN_OK;
   if (q.longest > kChainInPiece) {
     float* start = reinterpret_cast<float*>(w + p.carry + p.sums);
-    cached_chain_kernel<<<dim3(unsigned((int64_t(a.dn) * NS + 127) / 128), unsigned(q.n_chains)), 128, 0, s>>>(
-        q.chains, a.A, k.h, k.sum, start, a.dn, p.rows);
+    const int blocks = int((int64_t(a.dn) * NS + 127) / 128);
+    cached_chain_kernel<<<unsigned(q.n_chains * blocks), 128, 0, s>>>(q.chains, a.A, k.h, k.sum, start, a.dn, p.rows,
+                                                                     blocks);
     VM_TRY(check_launch());
     k.start = start;
   }
@@ -1451,7 +1452,8 @@ int launch_cached_conv(const CachedConvArgs& a, const int32_t* pieces, int64_t n
   const bool wide = a.channels % 4 == 0 && four_wide<T>(a.x, a.ldx) && four_wide<T>(a.out, a.ldo) &&
                     four_wide<T>(a.state, a.channels);
   const int groups = (a.channels + CCV_THREADS * (wide ? 4 : 1) - 1) / (CCV_THREADS * (wide ? 4 : 1));
-  if (n_pieces * groups > INT32_MAX) return fail(VMSCAN_ERR_SHAPE, "cached conv: %lld pieces", (long long)n_pieces);
+  if (n_pieces > INT32_MAX || n_pieces * groups > INT32_MAX)
+    return fail(VMSCAN_ERR_SHAPE, "cached conv: %lld pieces", (long long)n_pieces);
   const unsigned grid = unsigned(n_pieces * groups);
 #define VM_CONV(K)                                                                        \
   case K:                                                                                 \
@@ -1642,9 +1644,10 @@ int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16,
                           n_slots));
   if (pieces == nullptr || (n_chains > 0 && chains == nullptr)) return VMSCAN_ERR_NULL;
   if (!aligned16(pieces) || !aligned16(chains)) return fail(VMSCAN_ERR_ALIGN, "pieces and chains must be 16-byte aligned");
-  const CachedScanPlan p = cached_scan_plan(d_inner, std::max<int64_t>(carry_rows, 0));
-  if (n_pieces <= 0 || n_first <= 0 || n_first > n_pieces || n_chains < 0 || n_chains > 65535 || carry_rows < 0 || carry_rows > INT32_MAX ||
-      (n_chains > 0) != (carry_rows > 0) || (n_chains > 0) != (n_first < n_pieces) || n_pieces * p.groups > INT32_MAX)
+  const CachedScanPlan p = cached_scan_plan(d_inner, std::min<int64_t>(std::max<int64_t>(carry_rows, 0), INT32_MAX));
+  if (n_pieces <= 0 || n_pieces > INT32_MAX || n_pieces * p.groups > INT32_MAX || n_first <= 0 || n_first > n_pieces ||
+      n_chains < 0 || n_chains > n_pieces || n_chains * ((d_inner * NS + 127) / 128) > INT32_MAX || carry_rows < 0 ||
+      carry_rows > INT32_MAX || (n_chains > 0) != (carry_rows > 0) || (n_chains > 0) != (n_first < n_pieces))
     return fail(VMSCAN_ERR_SHAPE, "cached scan: %lld pieces (%lld first), %lld chains, %lld carry rows",
                 (long long)n_pieces, (long long)n_first, (long long)n_chains, (long long)carry_rows);
   if (p.total > 0 && (workspace == nullptr || workspace_bytes < p.total || !aligned16(workspace)))

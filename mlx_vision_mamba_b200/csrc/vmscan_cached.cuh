@@ -426,10 +426,10 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
 constexpr int CCH_AHEAD = 8;
 __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const float* __restrict__ A,
                                     const float* __restrict__ carry_h, const float* __restrict__ carry_s,
-                                    float* __restrict__ h_start, int64_t dn, int rows) {
-  const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+                                    float* __restrict__ h_start, int64_t dn, int rows, int blocks) {
+  const int64_t i = int64_t(blockIdx.x % blocks) * blockDim.x + threadIdx.x;
   if (i >= dn * NS) return;
-  int4 c = reinterpret_cast<const int4*>(chains)[blockIdx.y];
+  int4 c = reinterpret_cast<const int4*>(chains)[blockIdx.x / blocks];
   if (c.x < 0 || c.x >= rows) return;
   c.y = min(c.y, rows - c.x);
   const float An = A[i];

@@ -53,17 +53,20 @@ def _int_list(name: str, values, count: Optional[int] = None) -> np.ndarray:
         raise ValueError(f"RequestBatch: `{name}` has {arr.size} entries for {count} requests")
     if arr.size and (int(arr.min()) < -1 or int(arr.max()) >= 1 << 31):
         raise ValueError(f"RequestBatch: `{name}` has an entry outside [-1, 2^31)")
-    return np.ascontiguousarray(arr, dtype=np.int32)
+    return np.array(arr, dtype=np.int32, order="C")  # a copy: what was checked stays as it was
 
 
 class _Table:
-    """A device table, its pinned source, and what the operators are told of
-    it: (address, sizes...)."""
+    """A device table, its pinned source, the stream it was made on and what the
+    operators are told of it: (address, sizes...).  limit: slots of the smallest
+    cache that a captured graph uses it with."""
 
-    __slots__ = ("tensor", "host", "told", "captured")
+    __slots__ = ("tensor", "host", "stream", "told", "limit")
 
-    def __init__(self, tensor, host, info):
-        self.tensor, self.host, self.told, self.captured = tensor, host, (tensor.data_ptr(), *info), False
+    def __init__(self, host, info, device):
+        self.host, self.stream = host, torch.cuda.current_stream(device)
+        self.tensor = host.to(device, non_blocking=True)
+        self.told, self.limit = (self.tensor.data_ptr(), *info), None
 
 
 class RequestBatch:
@@ -72,7 +75,7 @@ class RequestBatch:
     lengths:  rows of each request (0 allowed: only its state is carried over).
     slots:    cache slot each request's state is written to; default 0, 1, ...;
               -1 makes a padding request: its rows come out as zeros (as `base`
-              from lora_add_cuda) and no state is touched.
+              from lora_add_cuda, whatever its adapter) and no state is touched.
     sources:  slot each request's state is read from; default its own slot (a
               running request goes on); -1 starts from zeros (a fresh prompt);
               another slot forks a kept state (a shared prompt).
@@ -86,7 +89,7 @@ class RequestBatch:
     Device tables are made on first use, one copy per stream, and live as long
     as the batch: keep it while a CUDA graph captured with it is replayed.
     `update` changes slots, sources and adapters in place, also for captured
-    graphs; the lengths are fixed.
+    graphs; the lengths are fixed.  The attributes are for reading.
     """
 
     def __init__(self, lengths: Sequence[int], slots=None, sources=None, adapters=None, device="cuda"):
@@ -105,10 +108,10 @@ class RequestBatch:
         self.index = -2 if self.device.type != "cuda" else self.device.index
         self.single_tokens = bool((self.lengths == 1).all())
         self._tables = {}
-        self._set(slots if slots is not None else np.arange(self.count), sources, adapters)
+        self._set(slots, sources, adapters)
 
     def _set(self, slots, sources, adapters):
-        slots = _int_list("slots", slots, self.count)
+        slots = _int_list("slots", np.arange(self.count) if slots is None else slots, self.count)
         sources = slots.copy() if sources is None else _int_list("sources", sources, self.count)
         sources[slots < 0] = -1
         written = slots[slots >= 0]
@@ -117,34 +120,49 @@ class RequestBatch:
         foreign = sources[(sources >= 0) & (sources != slots)]
         if np.intersect1d(foreign, written).size:
             raise ValueError("RequestBatch: a request reads a slot that another request writes")
-        adapters = None if adapters is None else _int_list("adapters", adapters, self.count)
-        self.slots, self.sources, self.adapters = slots, sources, adapters
+        given = None if adapters is None else _int_list("adapters", adapters, self.count)
+        adapters = None if given is None else np.where(slots < 0, np.int32(-1), given)
+        for a in (self.lengths, slots, sources, given, adapters):
+            if a is not None:
+                a.setflags(write=False)
+        self.slots, self.sources, self.adapters, self._adapters_given = slots, sources, adapters, given
         self.max_slot = int(max(slots.max(), sources.max()))
         self.max_adapter = -2 if adapters is None else int(adapters.max())  # -2: made without adapters
 
     def update(self, slots=None, sources=None, adapters=None) -> None:
-        """New slots, sources and adapters (each default as in the constructor;
-        adapters None keeps the present ones) for the same lengths.  The device
-        tables are rewritten in order on the current stream: call it on the
-        stream that uses the batch or replays graphs captured with it."""
+        """New slots, sources and adapters (slots and sources default as in the
+        constructor; adapters None keeps the present ones) for the same lengths.
+        The device tables are rewritten on the current stream, after what other
+        streams have run with this batch so far and before what they run later;
+        graphs captured with it must be replayed in order with the current
+        stream.  Nothing changes when the new values are refused."""
         if _capturing():
             raise RuntimeError("RequestBatch.update: not while a CUDA graph is being captured")
-        if adapters is not None and self.adapters is None and any(k[0] == "lora" for k in self._tables):
-            raise RuntimeError("RequestBatch.update: the batch was made without adapters")
-        self._set(slots if slots is not None else np.arange(self.count), sources,
-                  self.adapters if adapters is None else adapters)
-        if not self._tables:
-            return
-        here = torch.cuda.current_stream(self.device).cuda_stream
-        # tables that another stream uses are dropped (made again there), unless
-        # a graph has captured them: those are rewritten on this stream
-        self._tables = {k: t for k, t in self._tables.items() if k[-1] == here or t.captured}
-        for key, table in self._tables.items():
-            host, info = self._build(key)
-            if info != table.told[1:] or host.numel() != table.host.numel():
+        names = ("slots", "sources", "adapters", "_adapters_given", "max_slot", "max_adapter")
+        before = {n: getattr(self, n) for n in names}
+        try:
+            self._set(slots, sources, self._adapters_given if adapters is None else adapters)
+            limit = min((t.limit for t in self._tables.values() if t.limit is not None), default=None)
+            if limit is not None and self.max_slot >= limit:
+                raise ValueError(f"RequestBatch.update: slot {self.max_slot} in a graph whose cache has {limit} slots")
+            new = [(table, *self._build(key)) for key, table in self._tables.items()]
+            if any(info != table.told[1:] for table, _, info in new):
                 raise RuntimeError("RequestBatch.update: table sizes changed")
-            table.tensor.copy_(host, non_blocking=True)
+        except Exception:
+            for n, v in before.items():
+                setattr(self, n, v)
+            raise
+        if not new:
+            return
+        here = torch.cuda.current_stream(self.device)
+        for table, host, _ in new:
+            if table.stream != here:
+                here.wait_stream(table.stream)
+            with torch.cuda.stream(here):
+                table.tensor.copy_(host, non_blocking=True)
             table.host = host
+            if table.stream != here:
+                table.stream.wait_stream(here)
 
     def _build(self, key):
         """(pinned int32 host table, its sizes) of kind key[0]."""
@@ -175,24 +193,23 @@ class RequestBatch:
         _check_count(lib.vmscan_request_pieces(*args, ptr(table), table.size, ptr(info)), "vmscan_request_pieces")
         return _pinned(table), (int(n), *(int(v) for v in info))
 
-    def _table(self, kind: str, stream: int, arg: int = 0):
+    def _table(self, kind: str, stream: int, arg: int, capturing: bool, slots: int):
         """(address, sizes...) of the device table of a kind for the current
-        stream; called by the operators."""
+        stream; called by the operators (slots: of the cache they are given)."""
         key = (kind, arg, stream)
         table = self._tables.get(key)
-        if table is not None and not _capturing():
-            return table.told
-        if table is None and not _capturing():
+        if capturing:
+            # any stream's table will do: capture starts after a device-wide
+            # synchronisation, so its upload has completed
+            if table is None:
+                table = next((t for k, t in self._tables.items() if k[:2] == key[:2]), None)
+            if table is None:
+                raise RuntimeError("RequestBatch: call the operator once with this batch before capturing it")
+            if kind != "lora":
+                table.limit = slots if table.limit is None else min(slots, table.limit)
+        elif table is None:
             host, info = self._build(key)
-            self._tables[key] = table = _Table(host.to(self.device, non_blocking=True), host, info)
-            return table.told
-        # any stream's table will do under capture: it starts after a
-        # device-wide synchronisation, so the upload has completed
-        if table is None:
-            table = next((t for k, t in self._tables.items() if k[:2] == key[:2]), None)
-        if table is None:
-            raise RuntimeError("RequestBatch: call the operator once with this batch before capturing it")
-        table.captured = True
+            self._tables[key] = table = _Table(host, info, self.device)
         return table.told
 
 

@@ -51,6 +51,24 @@ def test_allowed_batches():
     assert RequestBatch([1], sources=[-1]).sources.tolist() == [-1]
 
 
+def test_a_batch_keeps_what_it_checked():
+    """The caller's arrays are copied, the batch's cannot be written, and a
+    padding request has neither source nor adapter."""
+    slots, sources = np.array([4, -1], np.int32), np.array([2, 3], np.int32)
+    b = RequestBatch(np.array([1, 1], np.int32), slots=slots, sources=sources, adapters=[0, 1])
+    assert sources.tolist() == [2, 3] and b.sources.tolist() == [2, -1] and b.adapters.tolist() == [0, -1]
+    slots[0] = 99
+    assert b.slots.tolist() == [4, -1]
+    for a in (b.lengths, b.slots, b.sources, b.adapters):
+        with pytest.raises(ValueError):
+            a[0] = 7
+    b.update(slots=[1, 2])  # the adapters that were given come back
+    assert b.sources.tolist() == [1, 2] and b.adapters.tolist() == [0, 1]
+    with pytest.raises(ValueError):
+        b.update(slots=[3, 3])
+    assert b.slots.tolist() == [1, 2] and b.max_slot == 2
+
+
 def _pieces(batch, rows, scan):
     lib = _native.load()
     info = np.zeros(4, dtype=np.int64)

@@ -287,6 +287,8 @@ def test_lora_strides_and_rows_behind():
         y = lora_add_cuda(bv, xv, ads, batch)
         ref.check("strided", y, want[0], want[1])
         assert torch.equal(y[26:], base[26:]) and torch.equal(y[5:25], base[5:25])
+    padded = RequestBatch([5, 20, 1], slots=[0, 1, -1], adapters=[1, -1, 0])
+    assert torch.equal(lora_add_cuda(base, x, ads, padded)[25], base[25])  # a padding request has no adapter
     out = torch.zeros(31, 64, device="cuda")[:, 3:33]
     assert torch.equal(lora_add_cuda(base, x, ads, batch, out=out), out)
     ref.check("out", out, want[0], want[1])
@@ -396,6 +398,70 @@ def test_other_streams_and_graphs():
     s2, w2 = inp["state"].clone(), win.clone()
     for p, q in zip(step(s2, w2) + (s2, w2), captured + (state, window)):
         assert torch.equal(p, q)
+
+
+def test_update_is_ordered_and_refused_whole():
+    """update waits for other streams' calls and holds back their next ones; a
+    slot outside a captured cache, or an adapter outside the captured ones, is
+    refused and changes nothing."""
+    count, dn = 5, 64
+    batch = RequestBatch([1] * count, adapters=[0, 1, 0, 1, 0])
+    inp = _scan_inputs(count, dn, 2 * count, seed=12)
+    base, xl, ads = _lora_inputs(batch, 2, 24, 40, 4, F32, seed=3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for k in range(3):
+        slots = [(i + k) % count + (count if k == 2 else 0) for i in range(count)]
+        batch.update(slots=slots, sources=[-1 if i == k else s for i, s in enumerate(slots)])
+        with torch.cuda.stream(side):
+            state = inp["state"].clone()
+            y = selective_scan_cached_cuda(batch=batch, **dict(inp, state=state))
+        torch.cuda.current_stream().wait_stream(side)
+        want = ref.scan(batch=batch, **inp)
+        ref.check("y", y, want[0], want[1])
+        ref.check("state", state, want[2], want[3])
+    lora_add_cuda(base, xl, ads, batch)
+    graph = torch.cuda.CUDAGraph()
+    state = inp["state"].clone()
+    with torch.cuda.graph(graph):
+        selective_scan_cached_cuda(batch=batch, **dict(inp, state=state))
+        lora_add_cuda(base, xl, ads, batch)
+    before = batch.slots.tolist()
+    with pytest.raises(ValueError, match="cache"):
+        batch.update(slots=[0, 1, 2, 3, 2 * count])
+    with pytest.raises(RuntimeError):
+        batch.update(adapters=[0, 1, 2, 0, 0])
+    assert batch.slots.tolist() == before and batch.adapters.tolist() == [0, 1, 0, 1, 0]
+    state.copy_(inp["state"])
+    graph.replay()
+    want = ref.scan(batch=batch, **inp)
+    ref.check("state", state, want[2], want[3])
+
+
+def test_requests_without_rows():
+    """A call that only forks, clears and keeps states."""
+    inp = _scan_inputs(0, 40, 6, seed=1)
+    batch = RequestBatch([0, 0, 0, 0], slots=[3, 4, -1, 2], sources=[0, -1, 1, 2])
+    state = inp["state"].clone()
+    y = selective_scan_cached_cuda(batch=batch, **dict(inp, state=state))
+    assert y.shape == (0, 40)
+    want = inp["state"].clone()
+    want[3], want[4] = inp["state"][0], 0
+    assert torch.equal(state, want)
+    window = torch.randn(6, 3, 40, device="cuda")
+    new = window.clone()
+    conv1d_silu_cached_cuda(inp["x"], torch.randn(40, 4, 1, device="cuda"), torch.randn(40, device="cuda"), new, batch)
+    window[3], window[4] = window[0].clone(), 0
+    assert torch.equal(new, window)
+    lb = RequestBatch([0, 0], adapters=[0, 1])
+    base, x, ads = _lora_inputs(lb, 2, 8, 12, 4, F32, rows=3)
+    assert torch.equal(lora_add_cuda(base, x, ads, lb), base)
+    block = MambaBlock(d_model=32).cuda()
+    cache = block.new_cache(2)
+    cache.ssm.normal_()
+    kept = cache.ssm[0].clone()
+    assert block.serve(torch.empty(0, 32, device="cuda"), cache, RequestBatch([0], slots=[1], sources=[0])).shape == (0, 32)
+    assert torch.equal(cache.ssm[1], kept)
 
 
 def test_capture_needs_an_eager_call():
