@@ -434,7 +434,8 @@ int vmscan_gemm_tf32x3(int64_t M, int64_t N, int64_t K,
  * the rest (all but the first pieces of split requests), long ones first in
  * each, followed by info[1] records of 4 int32 {first carry row, pieces, 0, 0},
  * one for each split request; info[2] is the number of carry rows, info[3] the
- * most pieces of a request.  Negative on a bad argument.
+ * most pieces of a request, info[4] whether the pieces are uneven (info holds
+ * 5 values).  Negative on a bad argument.
  *
  * vmscan_cached_scan_rows (host only) gives max_rows for vmscan_cached_scan on
  * the current device: 0 when one warp per request and 32 channels keeps the
@@ -455,7 +456,7 @@ int vmscan_cached_scan(int64_t rows, int64_t d_inner, int64_t d_state, int bf16,
                        const void* delta, int64_t lddelta, const float* A, const void* B, int64_t ldB, const void* C,
                        int64_t ldC, const float* D, const void* z, int64_t ldz, void* y, int64_t ldy, float* state,
                        int64_t n_slots, const int32_t* pieces, int64_t n_pieces, int64_t n_first,
-                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, int64_t longest_chain,
+                       const int32_t* chains, int64_t n_chains, int64_t carry_rows, int64_t longest_chain, int uneven,
                        void* workspace, size_t workspace_bytes, vmscan_stream_t stream);
 
 /*

@@ -130,7 +130,7 @@ SIGNATURES = {
     "vmscan_cached_scan": (
         ctypes.c_int,
         [_i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64,
-         _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _sz, _p],
+         _p, _i64, _i64, _p, _i64, _i64, _i64, ctypes.c_int, _p, _sz, _p],
     ),
     "vmscan_cached_step": (
         ctypes.c_int,

@@ -148,11 +148,11 @@ at::Tensor out_rows(const at::Tensor& x, const Batch& b) {
   return y;
 }
 
-// The batch's device table of a kind for a stream: its address and up to five
-// sizes (RequestBatch._table makes and keeps it).
+// The batch's device table of a kind for a stream: its address and up to six
+// numbers (RequestBatch._table makes and keeps it).
 struct Table {
   int64_t ptr;
-  int64_t info[5];
+  int64_t info[6];
 };
 
 Table table_of(const Batch& b, PyObject* kind, void* stream, int64_t arg, int64_t slots) {
@@ -160,7 +160,7 @@ Table table_of(const Batch& b, PyObject* kind, void* stream, int64_t arg, int64_
   Ref s(PyLong_FromVoidPtr(stream)), a(PyLong_FromLongLong(arg)), n(PyLong_FromLongLong(slots));
   PyObject* args[6] = {b.self, kind, s.p, a.p, capturing ? Py_True : Py_False, n.p};
   Ref r(PyObject_VectorcallMethod(g_names.table, args, 6, nullptr));
-  TORCH_CHECK(PyTuple_Check(r.p) && PyTuple_GET_SIZE(r.p) <= 6, "RequestBatch._table returned no table");
+  TORCH_CHECK(PyTuple_Check(r.p) && PyTuple_GET_SIZE(r.p) <= 7, "RequestBatch._table returned no table");
   Table t{};
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(r.p); ++i) {
     const int64_t v = PyLong_AsLongLong(PyTuple_GET_ITEM(r.p, i));
@@ -241,7 +241,7 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                            static_cast<const float*>(A_.data_ptr()), B_.data_ptr(), B_.stride(0), C_.data_ptr(),
                            C_.stride(0), static_cast<const float*>(D_.data_ptr()), zp, ldz, y.data_ptr(), dn,
                            static_cast<float*>(state.data_ptr()), state.size(0), i32(t.ptr), n, t.info[1],
-                           chains > 0 ? i32(t.ptr) + 8 * n : nullptr, chains, carry_rows, t.info[4],
+                           chains > 0 ? i32(t.ptr) + 8 * n : nullptr, chains, carry_rows, t.info[4], int(t.info[5]),
                            ws.defined() ? ws.data_ptr() : nullptr, size_t(ws_bytes), stream),
         where, "vmscan_cached_scan");
   return THPVariable_Wrap(y);

@@ -186,7 +186,7 @@ class RequestBatch:
             rows, scan = lib.vmscan_cached_conv_rows(self.tokens, arg), 0
         if rows < 0:
             _native.check(-rows, "vmscan_cached_scan_rows")
-        info = np.zeros(4, dtype=np.int64)
+        info = np.zeros(5, dtype=np.int64)
         args = (self.count, ptr(self.lengths), ptr(self.slots), ptr(self.sources), rows, scan)
         n = _check_count(lib.vmscan_request_pieces(*args, None, 0, ptr(info)), "vmscan_request_pieces")
         table = np.empty(8 * n + 4 * int(info[1]), dtype=np.int32)

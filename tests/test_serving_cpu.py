@@ -71,7 +71,7 @@ def test_a_batch_keeps_what_it_checked():
 
 def _pieces(batch, rows, scan):
     lib = _native.load()
-    info = np.zeros(4, dtype=np.int64)
+    info = np.zeros(5, dtype=np.int64)
     p = lambda a: a.ctypes.data  # noqa: E731
     args = (batch.count, p(batch.lengths), p(batch.slots), p(batch.sources), rows, scan)
     n = lib.vmscan_request_pieces(*args, None, 0, p(info))
@@ -189,8 +189,8 @@ def test_c_entry_points_validate():
     P = 4096
     scan = lambda **o: lib.vmscan_cached_scan(*[{**dict(  # noqa: E731
         rows=4, dn=8, ds=16, bf16=0, u=P, ldu=8, dl=P, ldd=8, A=P, B=P, ldb=16, C=P, ldc=16, D=P, z=None, ldz=0, y=P,
-        ldy=8, state=P, slots=2, pieces=P, n=1, nf=1, chains=None, nch=0, cr=0, lc=1, ws=None, wn=0, stream=None), **o}[k]
-        for k in ("rows dn ds bf16 u ldu dl ldd A B ldb C ldc D z ldz y ldy state slots pieces n nf chains nch cr lc ws wn "
+        ldy=8, state=P, slots=2, pieces=P, n=1, nf=1, chains=None, nch=0, cr=0, lc=1, un=0, ws=None, wn=0, stream=None), **o}[k]
+        for k in ("rows dn ds bf16 u ldu dl ldd A B ldb C ldc D z ldz y ldy state slots pieces n nf chains nch cr lc un ws wn "
                   "stream").split()])
     assert scan(ds=8) == 3
     assert scan(A=None) == 1 and scan(u=None) == 1 and scan(state=None) == 1 and scan(pieces=None) == 1

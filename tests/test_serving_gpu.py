@@ -66,7 +66,7 @@ def test_scan_split_prompts(lengths, dn, dtype):
     """Prompts long enough to be scanned in several pieces, from and to the same slot and forked."""
     n = len(lengths)
     for batch in (RequestBatch(lengths), RequestBatch(lengths, slots=list(range(n, 2 * n)), sources=[0] * n)):
-        n_pieces, n_first, chains, _, most = batch._build(("scan", 2 * dn))[1]
+        n_pieces, n_first, chains, _, most, _ = batch._build(("scan", 2 * dn))[1]
         assert chains > 0 and n_pieces > n_first and most > 2
         _scan_check(f"scan {lengths} {dn}", _scan_inputs(batch.tokens, dn, 2 * n, dtype, seed=7), batch)
 
