@@ -483,9 +483,11 @@ int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int
 
 /*
  * out_t = base_t + scale[a] (x_t A_a^T) B_a^T with a the adapter of row t's
- * request (-1: out_t = base_t); A (adapters, rank, d_in) and B (adapters,
- * d_out, rank) in the type of x, rank in 1..128, products and the rank-wide
- * values in fp32.  out may be base.  vmscan_lora_tiles (host only) sorts the
+ * request (-1: out_t = base_t); A (adapters, rank, lda) and B (adapters,
+ * d_out, rank) in the type of x, rank a multiple of 4 of at most 128 (smaller
+ * ones padded with zeros), lda at least d_in and a multiple of 16 bytes, A's
+ * columns from d_in on zero; products and the rank-wide values in fp32.  out
+ * may be base.  vmscan_lora_tiles (host only) sorts the
  * rows by adapter into row_index (one int32 per row) and cuts them into tiles
  * of 4 int32; it returns the number of tiles that any assignment of adapters
  * to these lengths can need, and fills them all (with row_index or tiles NULL
@@ -494,9 +496,9 @@ int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int
 int64_t vmscan_lora_tiles(int64_t count, const int32_t* lengths, const int32_t* adapters, int64_t n_adapters,
                           int32_t* row_index, int32_t* tiles, int64_t tile_capacity);
 int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int64_t n_adapters, int bf16,
-                    const void* x, int64_t ldx, const void* a, const void* b, const float* scale, const void* base,
-                    int64_t ldbase, void* out, int64_t ldout, const int32_t* row_index, int64_t n_index,
-                    const int32_t* tiles, int64_t n_tiles, vmscan_stream_t stream);
+                    const void* x, int64_t ldx, const void* a, int64_t lda, const void* b, const float* scale,
+                    const void* base, int64_t ldbase, void* out, int64_t ldout, const int32_t* row_index,
+                    int64_t n_index, const int32_t* tiles, int64_t n_tiles, vmscan_stream_t stream);
 
 /*
  * Host-only introspection (no CUDA call): writes the token index visited at

@@ -145,7 +145,8 @@ SIGNATURES = {
     "vmscan_lora_tiles": (_i64, [_i64, _p, _p, _i64, _p, _p, _i64]),
     "vmscan_lora_add": (
         ctypes.c_int,
-        [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
+        [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64,
+         _p],
     ),
     "vmscan_scan_order": (ctypes.c_int, [_i64, _D, ctypes.c_int, _p, _p]),
     "vmscan_device_status": (ctypes.c_int, [_p, ctypes.c_int]),

@@ -310,12 +310,17 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       rs(PyObject_GetAttr(args[2], g_names.scale));
   const at::Tensor &a = tensor(where, "adapters", ra.p), &bb = tensor(where, "adapters", rb.p),
                    &scale = tensor(where, "adapters", rs.p);
+  // padded storage: a (count, padded rank, lda), b (count, d_out, padded rank)
   VALUE(a.dim() == 3 && bb.dim() == 3 && scale.dim() == 1 && bb.size(0) == a.size(0) && scale.size(0) == a.size(0) &&
-            bb.size(2) == a.size(1) && a.is_contiguous() && bb.is_contiguous() && scale.is_contiguous() &&
-            bb.scalar_type() == a.scalar_type() && scale.scalar_type() == at::kFloat && a.is_cuda() &&
-            bb.device() == a.device() && scale.device() == a.device(),
+            bb.size(2) == a.size(1) && a.size(1) <= bb.stride(1) && a.size(2) <= a.stride(1) && a.stride(2) == 1 &&
+            bb.stride(2) == 1 && a.stride(0) == bb.stride(1) * a.stride(1) && bb.stride(0) == bb.size(1) * bb.stride(1) &&
+            a.storage_offset() == 0 && bb.storage_offset() == 0 &&
+            int64_t(a.storage().nbytes()) >= a.size(0) * a.stride(0) * int64_t(a.element_size()) &&
+            int64_t(bb.storage().nbytes()) >= bb.size(0) * bb.stride(0) * int64_t(bb.element_size()) &&
+            scale.is_contiguous() && bb.scalar_type() == a.scalar_type() && scale.scalar_type() == at::kFloat &&
+            a.is_cuda() && bb.device() == a.device() && scale.device() == a.device(),
         "the adapters' tensors are not as LoraAdapters made them");
-  const int64_t rows = x.size(0), count = a.size(0), rank = a.size(1), d_in = a.size(2), d_out = bb.size(1);
+  const int64_t rows = x.size(0), count = a.size(0), rank = bb.stride(1), d_in = a.size(2), d_out = bb.size(1);
   const at::Tensor& base = beside(where, "base", args[0], b.index);
   const at::Tensor* given = args[4] == Py_None ? nullptr : &beside(where, "out", args[4], b.index);
   shaped(where, "x", x, rows, d_in);
@@ -352,7 +357,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const Table t = table_of(b, g_names.lora, stream, count, 0);
     const int64_t tiles = t.info[0];
     check(vmscan_lora_add(rows, d_in, d_out, rank, count, dt == at::kBFloat16, x_.data_ptr(), x_.stride(0), a.data_ptr(),
-                          bb.data_ptr(), static_cast<const float*>(scale.data_ptr()), base_.data_ptr(), base_.stride(0),
+                          a.stride(1), bb.data_ptr(), static_cast<const float*>(scale.data_ptr()), base_.data_ptr(), base_.stride(0),
                           out.data_ptr(), out.stride(0), i32(t.ptr) + 4 * tiles, b.tokens, i32(t.ptr), tiles, stream),
           where, "vmscan_lora_add");
   }

@@ -1506,18 +1506,20 @@ int launch_lora(const LoraArgs& l, int n_tiles, cudaStream_t s) {
   return check_launch();
 }
 
-// Rows that do not start on whole accesses take one kernel of scalar accesses;
-// ranks of up to 16, 32 and 64 keep a group's share of B in registers.
+// Ranks of up to 16, 32 and 64 keep a group's share of B in registers.
+template <typename T, bool WIDE>
+int launch_lora_rank(const LoraArgs& l, int n_tiles, cudaStream_t s) {
+  if (l.rank <= 16) return launch_lora<T, WIDE, 1>(l, n_tiles, s);
+  if (l.rank <= 32) return launch_lora<T, WIDE, 2>(l, n_tiles, s);
+  if (l.rank > 48 && l.rank <= 64) return launch_lora<T, WIDE, 4>(l, n_tiles, s);
+  return launch_lora<T, WIDE, 0>(l, n_tiles, s);
+}
+
 template <typename T>
 int run_lora(const LoraArgs& l, int n_tiles, cudaStream_t s) {
-  const bool wide = row_grain<T>(l.x, l.ldx, l.d_in) == 16 && row_grain<T>(l.a, l.d_in, l.d_in) == 16 &&
-                    l.rank % 4 == 0 && four_wide<T>(l.b, l.rank) && l.d_out % 4 == 0 &&
-                    four_wide<T>(l.base, l.ldbase) && four_wide<T>(l.out, l.ldout);
-  if (!wide) return launch_lora<T, false, 0>(l, n_tiles, s);
-  if (l.rank <= 16) return launch_lora<T, true, 1>(l, n_tiles, s);
-  if (l.rank <= 32) return launch_lora<T, true, 2>(l, n_tiles, s);
-  if (l.rank > 48 && l.rank <= 64) return launch_lora<T, true, 4>(l, n_tiles, s);
-  return launch_lora<T, true, 0>(l, n_tiles, s);
+  const bool wide = row_grain<T>(l.x, l.ldx, l.d_in) == 16 && l.d_out % 4 == 0 && four_wide<T>(l.base, l.ldbase) &&
+                    four_wide<T>(l.out, l.ldout);
+  return wide ? launch_lora_rank<T, true>(l, n_tiles, s) : launch_lora_rank<T, false>(l, n_tiles, s);
 }
 
 }  // namespace
@@ -1773,9 +1775,9 @@ int64_t vmscan_lora_tiles(int64_t count, const int32_t* lengths, const int32_t* 
 }
 
 int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int64_t n_adapters, int bf16,
-                    const void* x, int64_t ldx, const void* a, const void* b, const float* scale, const void* base,
-                    int64_t ldbase, void* out, int64_t ldout, const int32_t* row_index, int64_t n_index,
-                    const int32_t* tiles, int64_t n_tiles, vmscan_stream_t stream) {
+                    const void* x, int64_t ldx, const void* a, int64_t lda, const void* b, const float* scale,
+                    const void* base, int64_t ldbase, void* out, int64_t ldout, const int32_t* row_index,
+                    int64_t n_index, const int32_t* tiles, int64_t n_tiles, vmscan_stream_t stream) {
   if (rows <= 0 || rows > (int64_t(1) << 30) || d_in <= 0 || d_in > (int64_t(1) << 24) || d_out <= 0 ||
       d_out > (int64_t(1) << 24) || rank < 1 || rank > LORA_RMAX || n_adapters <= 0 || n_adapters > INT32_MAX ||
       n_index < 0 || n_index > rows || n_tiles <= 0 || n_tiles > INT32_MAX)
@@ -1786,12 +1788,15 @@ int vmscan_lora_add(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int
       row_index == nullptr || tiles == nullptr)
     return VMSCAN_ERR_NULL;
   if (!aligned16(tiles)) return fail(VMSCAN_ERR_ALIGN, "lora: tiles must be 16-byte aligned");
+  if (!aligned16(a) || !aligned16(b) || rank % 4 != 0 || lda < d_in || lda > INT32_MAX || lda % (bf16 ? 8 : 4) != 0)
+    return fail(VMSCAN_ERR_ALIGN, "lora: a and b must be 16-byte aligned, the rank %lld a multiple of 4 and the rows of "
+                "a (%lld elements) whole multiples of 16 bytes", (long long)rank, (long long)lda);
   VM_TRY(check_row_stride("x", ldx, rows));
   VM_TRY(check_row_stride("base", ldbase, rows));
   VM_TRY(check_out_stride("out", ldout, d_out, rows));
   VM_TRY(ensure_context(out));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  LoraArgs l{x, a, b, base, out, scale, row_index, tiles, ldx, ldbase, ldout, int(rows), int(d_in), int(d_out),
+  LoraArgs l{x, a, b, base, out, scale, row_index, tiles, lda, ldx, ldbase, ldout, int(rows), int(d_in), int(d_out),
              int(rank), int(n_adapters), int(n_index)};
   if (bf16) return run_lora<__nv_bfloat16>(l, int(n_tiles), s);
   return run_lora<float>(l, int(n_tiles), s);

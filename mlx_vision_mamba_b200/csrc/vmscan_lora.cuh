@@ -33,14 +33,14 @@ constexpr int LORA_RCHUNK = 32;  // rank columns whose partial products a warp h
 
 struct LoraArgs {
   const void* x;
-  const void* a;      // (adapters, rank, d_in)
+  const void* a;      // (adapters, rank, lda), columns from d_in on zero
   const void* b;      // (adapters, d_out, rank)
   const void* base;
   void* out;
   const float* scale; // (adapters)
   const int32_t* row_index;
   const int32_t* tiles;
-  int64_t ldx, ldbase, ldout;
+  int64_t lda, ldx, ldbase, ldout;
   int rows, d_in, d_out, rank, adapters, n_index;
 };
 
@@ -82,45 +82,70 @@ __device__ __forceinline__ Chunk<T> ld_chunk(const T* row, int c, int limit) {
 }
 
 // Four elements of a row from column c on as they lie in memory (fp32: 4
-// words, bf16: 2), zero past `limit`.
+// words, bf16: 2), zero from `limit` (a multiple of 4) on.  Ordinary loads
+// (base may be the output: no read-only path), which the compiler may still
+// move across the stores of other columns.
 template <typename T>
 struct Four {
   uint32_t w[sizeof(T)];
 };
-// Ordinary loads (base may be the output: no read-only path), which the
-// compiler may still move across the stores of other columns.
-template <typename T, bool WIDE>
+template <typename T>
 __device__ __forceinline__ Four<T> ld_quad(const T* row, int c, int limit) {
-  Four<T> k;
+  Four<T> k{};
   if constexpr (sizeof(T) == 4) {
-    if constexpr (WIDE) {
-      k.w[0] = k.w[1] = k.w[2] = k.w[3] = 0;
-      if (c < limit)
-        asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
-            : "=r"(k.w[0]), "=r"(k.w[1]), "=r"(k.w[2]), "=r"(k.w[3])
-            : "l"(row + c));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) k.w[i] = c + i < limit ? __float_as_uint(row[c + i]) : 0u;
-    }
+    if (c < limit)
+      asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+          : "=r"(k.w[0]), "=r"(k.w[1]), "=r"(k.w[2]), "=r"(k.w[3])
+          : "l"(row + c));
   } else {
-    if constexpr (WIDE) {
-      k.w[0] = k.w[1] = 0;
-      if (c < limit) asm("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(k.w[0]), "=r"(k.w[1]) : "l"(row + c));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t lo = c + 2 * i < limit ? __bfloat16_as_ushort(row[c + 2 * i]) : 0;
-        const uint32_t hi = c + 2 * i + 1 < limit ? __bfloat16_as_ushort(row[c + 2 * i + 1]) : 0;
-        k.w[i] = lo | hi << 16;
-      }
-    }
+    if (c < limit) asm("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(k.w[0]), "=r"(k.w[1]) : "l"(row + c));
   }
   return k;
 }
 
+__device__ __forceinline__ float ld_scalar(const float* p) {
+  float v;
+  asm("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float ld_scalar(const __nv_bfloat16* p) {
+  unsigned short v;
+  asm("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return __uint_as_float(uint32_t(v) << 16);
+}
+
+// Elements 0, 4, 8, 12 from p on, zero from `left` on.
 template <typename T>
-__device__ __forceinline__ float4 four_f(const Four<T>& k) {
+__device__ __forceinline__ float4 ld_apart(const T* p, int left) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (left > 0) v.x = ld_scalar(p);
+  if (left > 4) v.y = ld_scalar(p + 4);
+  if (left > 8) v.z = ld_scalar(p + 8);
+  if (left > 12) v.w = ld_scalar(p + 12);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void st_apart(T* p, int left, const float4& v) {
+  stg_if_t<T>(p, v.x, left > 0);
+  stg_if_t<T>(p + 4, v.y, left > 4);
+  stg_if_t<T>(p + 8, v.z, left > 8);
+  stg_if_t<T>(p + 12, v.w, left > 12);
+}
+
+template <typename T, bool WIDE>
+struct BaseOf {
+  using type = Four<T>;
+};
+template <typename T>
+struct BaseOf<T, false> {
+  using type = float4;
+};
+template <typename T>
+__device__ __forceinline__ float4 base_f(const float4& v) {
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ float4 base_f(const Four<T>& k) {
   if constexpr (sizeof(T) == 4) {
     return make_float4(__uint_as_float(k.w[0]), __uint_as_float(k.w[1]), __uint_as_float(k.w[2]),
                        __uint_as_float(k.w[3]));
@@ -131,30 +156,18 @@ __device__ __forceinline__ float4 four_f(const Four<T>& k) {
   }
 }
 
-template <typename T, bool WIDE>
+// Columns c .. c + 3 of a row, c and limit multiples of 4.
+template <typename T>
 __device__ __forceinline__ void st_quad(T* row, int c, int limit, const float4& v) {
+  if (c >= limit) return;
   if constexpr (sizeof(T) == 4) {
-    if constexpr (WIDE) {
-      if (c < limit) *reinterpret_cast<float4*>(row + c) = v;
-      return;
-    }
-    if (c < limit) row[c] = v.x;
-    if (c + 1 < limit) row[c + 1] = v.y;
-    if (c + 2 < limit) row[c + 2] = v.z;
-    if (c + 3 < limit) row[c + 3] = v.w;
+    *reinterpret_cast<float4*>(row + c) = v;
   } else {
     const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    if constexpr (WIDE) {
-      uint2 q;
-      q.x = *reinterpret_cast<const uint32_t*>(&a);
-      q.y = *reinterpret_cast<const uint32_t*>(&b);
-      if (c < limit) *reinterpret_cast<uint2*>(row + c) = q;
-      return;
-    }
-    if (c < limit) row[c] = a.x;
-    if (c + 1 < limit) row[c + 1] = a.y;
-    if (c + 2 < limit) row[c + 2] = b.x;
-    if (c + 3 < limit) row[c + 3] = b.y;
+    uint2 q;
+    q.x = *reinterpret_cast<const uint32_t*>(&a);
+    q.y = *reinterpret_cast<const uint32_t*>(&b);
+    *reinterpret_cast<uint2*>(row + c) = q;
   }
 }
 
@@ -175,9 +188,23 @@ constexpr size_t lora_smem(int rank) {
           size_t(2) * ((rank + 15) / 16) * 32 * 4 * LoraFrag<T>::GROUPS) * 4;
 }
 
-// MT: 16-row blocks of the tile in use.  WIDE: every row of x, A, B, base and
-// out starts on a whole access (16 bytes; B, base and out four elements).
-// STEPS: 16-column steps of the rank, 0: any number.
+// The columns of a group that a lane adds to base, element i of four: adjacent
+// where rows take whole accesses, else four apart, so that a quad's scalar
+// accesses are adjacent.  lora_col: the column that stands for column g of the
+// group's 8-column block j in the product, so that lane t's accumulators are
+// those columns.
+template <bool WIDE>
+__device__ __forceinline__ int lora_own(int t, int i) {
+  return WIDE ? 4 * t + i : t + 4 * i;
+}
+template <bool WIDE>
+__device__ __forceinline__ int lora_col(int g, int j) {
+  return lora_own<WIDE>(g >> 1, 2 * j + (g & 1));
+}
+
+// MT: 16-row blocks of the tile in use.  WIDE: every row of x, base and out
+// takes whole accesses (x 16 bytes, base and out four elements); A and B
+// always do.  STEPS: 16-column steps of the rank, 0: any number.
 template <typename T, bool WIDE, int MT, int STEPS>
 __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int n, int ad, int c_begin, int c_end,
                                           float* part, uint32_t* frag) {
@@ -189,7 +216,7 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
   for (int i = 0; i < 2 * MT; ++i) r[i] = row[min(g + 8 * i, n - 1)];
   const int steps = STEPS > 0 ? STEPS : (a.rank + 15) / 16;
   if (ad >= 0) {
-    const T* A = static_cast<const T*>(a.a) + int64_t(ad) * a.rank * a.d_in;
+    const T* A = static_cast<const T*>(a.a) + int64_t(ad) * a.rank * a.lda;
     const T* xr[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) xr[i] = static_cast<const T*>(a.x) + r[i] * a.ldx;
@@ -199,14 +226,14 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
       const int nt = min(NT, (a.rank - rc + 7) / 8);
       const T* ar[NT];  // row of A whose products this lane's B fragments hold
 #pragma unroll
-      for (int j = 0; j < NT; ++j) ar[j] = A + int64_t(min(rc + 8 * j + g, a.rank - 1)) * a.d_in;
+      for (int j = 0; j < NT; ++j) ar[j] = A + int64_t(min(rc + 8 * j + g, a.rank - 1)) * a.lda;
 #pragma unroll 2
       for (int c = (warp * 4 + t) * CN; c - t * CN < a.d_in; c += LORA_WARPS * 4 * CN) {
         Chunk<T> x[2 * MT], ab[NT];
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) x[i] = ld_chunk<T, WIDE>(xr[i], c, a.d_in);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) ab[j] = ld_chunk<T, WIDE>(ar[j], c, a.d_in);  // rows past the rank: never summed
+        for (int j = 0; j < NT; ++j) ab[j] = ld_chunk<T, true>(ar[j], c, int(a.lda));  // rows past the rank: never summed
         uint32_t xl[2 * MT][4];
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -311,8 +338,7 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
       if (rc + LORA_RCHUNK < a.rank) __syncthreads();  // part is read before the next chunk's is written
     }
   }
-  // columns in groups of 16: lane t of a quad owns columns 4t .. 4t + 3 of its
-  // rows, which are columns 2t, 2t + 1 of the group's two 8-column blocks
+  // columns in groups of 16, two 8-column blocks of the product
   const T* B = static_cast<const T*>(a.b) + int64_t(max(ad, 0)) * a.d_out * a.rank;
   const T* br[2 * MT];
   T* outr[2 * MT];
@@ -322,19 +348,26 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
     outr[i] = static_cast<T*>(a.out) + r[i] * a.ldout;
   }
   constexpr int HELD = STEPS == 0 ? 1 : STEPS;  // steps of B loaded together
+  using Base = typename BaseOf<T, WIDE>::type;  // packed as loaded, or four values
   struct Group {
-    Four<T> base[2 * MT], b[HELD][2];
+    Base base[2 * MT];
+    Four<T> b[HELD][2];
   };
   auto load_b = [&](int c0, int s, Four<T> b[2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int col = c0 + 4 * (g >> 1) + (g & 1) + 2 * j;
-      b[j] = ld_quad<T, WIDE>(B + int64_t(min(col, a.d_out - 1)) * a.rank, 16 * s + 4 * t, a.rank);
+      const int col = c0 + lora_col<WIDE>(g, j);
+      b[j] = ld_quad<T>(B + int64_t(min(col, a.d_out - 1)) * a.rank, 16 * s + 4 * t, a.rank);
     }
   };
   auto load = [&](int c0, Group& k) {
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) k.base[i] = ld_quad<T, WIDE>(br[i], c0 + 4 * t, a.d_out);
+    for (int i = 0; i < 2 * MT; ++i) {
+      if constexpr (WIDE)
+        k.base[i] = ld_quad<T>(br[i], c0 + 4 * t, a.d_out);
+      else
+        k.base[i] = ld_apart(br[i] + c0 + t, a.d_out - c0 - t);
+    }
     if (STEPS > 0 && ad >= 0) {
 #pragma unroll
       for (int s = 0; s < HELD; ++s) load_b(c0, s, k.b[s]);
@@ -390,18 +423,32 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
     }
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
-      const float4 v = four_f(cur.base[i]);
+      const float4 v = base_f<T>(cur.base[i]);
       const float* p0 = &acc[i >> 1][0][2 * (i & 1)];
       const float* p1 = &acc[i >> 1][1][2 * (i & 1)];
-      if (g + 8 * i < n)
-        st_quad<T, WIDE>(outr[i], c0 + 4 * t, a.d_out, make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]));
+      if (g + 8 * i < n) {
+        const float4 o = make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]);
+        if constexpr (WIDE)
+          st_quad(outr[i], c0 + 4 * t, a.d_out, o);
+        else
+          st_apart(outr[i] + c0 + t, a.d_out - c0 - t, o);
+      }
     }
     cur = nxt;
   }
 }
 
+// CTAs an SM is to hold (registers): 16384 rows 384 -> 1536, rank 16, fp32
+// take 50 us with four, 54 with five, 72 with three; rank 64 fp32 141 with
+// four, 129 with three; 5000 rows 457 -> 763, rank 10, bf16 29 with four, 23
+// with five.
 template <typename T, bool WIDE, int STEPS>
-__global__ void __launch_bounds__(LORA_WARPS * 32) lora_add_kernel(const LoraArgs a, int cols_per_cta) {
+constexpr int lora_ctas() {
+  return STEPS == 1 ? (WIDE ? 4 : 5) : STEPS == 4 && sizeof(T) == 4 ? 3 : 4;
+}
+
+template <typename T, bool WIDE, int STEPS>
+__global__ void __launch_bounds__(LORA_WARPS * 32, (lora_ctas<T, WIDE, STEPS>())) lora_add_kernel(const LoraArgs a, int cols_per_cta) {
   extern __shared__ __align__(16) unsigned char lora_raw[];
   __shared__ int row[LORA_ROWS];
   float* part = reinterpret_cast<float*>(lora_raw);

@@ -237,7 +237,11 @@ class LoraAdapters:
     a: (adapters, rank, d_in) and b: (adapters, d_out, rank), CUDA, fp32 or
     bf16 (the type of the activations they are used with); scale: one number
     per adapter (a list, or a tensor), default 1.  Adapters of a smaller rank
-    are padded with zero rows / columns; rank is at most 128."""
+    than the others' are given with zero rows / columns; rank is at most 128.
+
+    The factors are copied: `a` and `b` are views of the copies, whose rows are
+    padded with zeros to whole accesses (ranks to a multiple of 4, rows of a to
+    16 bytes), and later changes to the tensors that were passed are not seen."""
 
     MAX_RANK = 128
 
@@ -254,13 +258,18 @@ class LoraAdapters:
             raise ValueError(f"LoraAdapters: rank {a.shape[1]} (at most {self.MAX_RANK})")
         self.count, self.rank, self.d_in = a.shape
         self.d_out = b.shape[1]
-        self.a, self.b = a.detach().contiguous(), b.detach().contiguous()
+        unit = 16 // a.element_size()
+        rank, wide = -(-self.rank // 4) * 4, -(-self.d_in // unit) * unit
+        self.a = a.new_zeros((self.count, rank, wide))[:, :self.rank, :self.d_in]
+        self.b = b.new_zeros((self.count, self.d_out, rank))[:, :, :self.rank]
+        self.a.copy_(a.detach())
+        self.b.copy_(b.detach())
         if scale is None:
             scale = torch.ones(self.count)
         scale = torch.as_tensor(scale, dtype=torch.float32)
         if tuple(scale.shape) != (self.count,):
             raise ValueError(f"LoraAdapters: scale must have {self.count} entries, got {tuple(scale.shape)}")
-        self.scale = scale.detach().to(a.device).contiguous()
+        self.scale = scale.detach().to(a.device, copy=True).contiguous()
 
 
 _ext_module = None

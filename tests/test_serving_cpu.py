@@ -213,8 +213,9 @@ def test_c_entry_points_validate():
     assert conv(k=0) == 10 and conv(k=9) == 10 and conv(state=None) == 1 and conv(x=None) == 1 and conv(n=0) == 2
     assert conv(ldo=4) == 2 and conv(c=0) == 2 and conv(pieces=P + 8) == 4
     lora = lambda **o: lib.vmscan_lora_add(*[{**dict(  # noqa: E731
-        rows=4, di=8, do=8, r=4, ad=2, bf16=0, x=P, ldx=8, a=P, b=P, s=P, base=P, ldb=8, out=P, ldo=8, idx=P, ni=4,
+        rows=4, di=8, do=8, r=4, ad=2, bf16=0, x=P, ldx=8, a=P, lda=8, b=P, s=P, base=P, ldb=8, out=P, ldo=8, idx=P, ni=4,
         tiles=P, nt=1, stream=None), **o}[k]
-        for k in "rows di do r ad bf16 x ldx a b s base ldb out ldo idx ni tiles nt stream".split()])
+        for k in "rows di do r ad bf16 x ldx a lda b s base ldb out ldo idx ni tiles nt stream".split()])
     assert lora(r=0) == 2 and lora(r=129) == 2 and lora(rows=0) == 2 and lora(ni=5) == 2 and lora(nt=0) == 2
+    assert lora(r=3) == 4 and lora(lda=6) == 4 and lora(lda=4) == 4 and lora(bf16=1, lda=12) == 4 and lora(a=P + 4) == 4
     assert lora(x=None) == 1 and lora(s=None) == 1 and lora(tiles=P + 4) == 4 and lora(ldo=7) == 2
