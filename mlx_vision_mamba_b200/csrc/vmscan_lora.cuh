@@ -29,6 +29,7 @@ namespace vmscan {
 constexpr int LORA_ROWS = 32;
 constexpr int LORA_WARPS = 4;
 constexpr int LORA_RMAX = 128;
+constexpr int LORA_LD = 18;       // row of 16 products in shared memory (two more keep the rows off each other's banks)
 constexpr int LORA_RCHUNK = 32;  // rank columns whose partial products a warp holds at a time
 
 struct LoraArgs {
@@ -114,38 +115,8 @@ __device__ __forceinline__ float ld_scalar(const __nv_bfloat16* p) {
   return __uint_as_float(uint32_t(v) << 16);
 }
 
-// Elements 0, 4, 8, 12 from p on, zero from `left` on.
 template <typename T>
-__device__ __forceinline__ float4 ld_apart(const T* p, int left) {
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (left > 0) v.x = ld_scalar(p);
-  if (left > 4) v.y = ld_scalar(p + 4);
-  if (left > 8) v.z = ld_scalar(p + 8);
-  if (left > 12) v.w = ld_scalar(p + 12);
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ void st_apart(T* p, int left, const float4& v) {
-  stg_if_t<T>(p, v.x, left > 0);
-  stg_if_t<T>(p + 4, v.y, left > 4);
-  stg_if_t<T>(p + 8, v.z, left > 8);
-  stg_if_t<T>(p + 12, v.w, left > 12);
-}
-
-template <typename T, bool WIDE>
-struct BaseOf {
-  using type = Four<T>;
-};
-template <typename T>
-struct BaseOf<T, false> {
-  using type = float4;
-};
-template <typename T>
-__device__ __forceinline__ float4 base_f(const float4& v) {
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ float4 base_f(const Four<T>& k) {
+__device__ __forceinline__ float4 four_f(const Four<T>& k) {
   if constexpr (sizeof(T) == 4) {
     return make_float4(__uint_as_float(k.w[0]), __uint_as_float(k.w[1]), __uint_as_float(k.w[2]),
                        __uint_as_float(k.w[3]));
@@ -188,23 +159,13 @@ constexpr size_t lora_smem(int rank) {
           size_t(2) * ((rank + 15) / 16) * 32 * 4 * LoraFrag<T>::GROUPS) * 4;
 }
 
-// The columns of a group that a lane adds to base, element i of four: adjacent
-// where rows take whole accesses, else four apart, so that a quad's scalar
-// accesses are adjacent.  lora_col: the column that stands for column g of the
-// group's 8-column block j in the product, so that lane t's accumulators are
-// those columns.
-template <bool WIDE>
-__device__ __forceinline__ int lora_own(int t, int i) {
-  return WIDE ? 4 * t + i : t + 4 * i;
-}
-template <bool WIDE>
-__device__ __forceinline__ int lora_col(int g, int j) {
-  return lora_own<WIDE>(g >> 1, 2 * j + (g & 1));
-}
-
 // MT: 16-row blocks of the tile in use.  WIDE: every row of x, base and out
 // takes whole accesses (x 16 bytes, base and out four elements); A and B
-// always do.  STEPS: 16-column steps of the rank, 0: any number.
+// always do.  Without, base and out move as rows of 16 adjacent elements, two
+// rows an access, and the products cross to that layout in shared memory (as
+// scalars in the products' own layout, 4 columns of 8 rows an access, 16384
+// rows 700 -> 1411, rank 10, bf16 took 119 us).  STEPS: 16-column steps of the
+// rank, 0: any number.
 template <typename T, bool WIDE, int MT, int STEPS>
 __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int n, int ad, int c_begin, int c_end,
                                           float* part, uint32_t* frag) {
@@ -338,7 +299,10 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
       if (rc + LORA_RCHUNK < a.rank) __syncthreads();  // part is read before the next chunk's is written
     }
   }
-  // columns in groups of 16, two 8-column blocks of the product
+  // columns in groups of 16, two 8-column blocks of the product.  WIDE: lane t
+  // of a quad owns columns 4t .. 4t + 3 of its rows, which stand for columns
+  // 2t, 2t + 1 of the two blocks; else lane l owns column l % 16 of rows
+  // l / 16, l / 16 + 2, ...
   const T* B = static_cast<const T*>(a.b) + int64_t(max(ad, 0)) * a.d_out * a.rank;
   const T* br[2 * MT];
   T* outr[2 * MT];
@@ -348,25 +312,31 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
     outr[i] = static_cast<T*>(a.out) + r[i] * a.ldout;
   }
   constexpr int HELD = STEPS == 0 ? 1 : STEPS;  // steps of B loaded together
-  using Base = typename BaseOf<T, WIDE>::type;  // packed as loaded, or four values
+  const int half = lane >> 4, lcol = lane & 15;
+  float* stage = part + warp * LORA_ROWS * (LORA_RCHUNK + 1);  // !WIDE: the warp's products, free since S is complete
   struct Group {
-    Base base[2 * MT];
+    Four<T> base[WIDE ? 2 * MT : 1];
+    float one[WIDE ? 1 : 8 * MT];
     Four<T> b[HELD][2];
   };
   auto load_b = [&](int c0, int s, Four<T> b[2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int col = c0 + lora_col<WIDE>(g, j);
+      const int col = c0 + (WIDE ? 4 * (g >> 1) + (g & 1) + 2 * j : 8 * j + g);
       b[j] = ld_quad<T>(B + int64_t(min(col, a.d_out - 1)) * a.rank, 16 * s + 4 * t, a.rank);
     }
   };
   auto load = [&](int c0, Group& k) {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      if constexpr (WIDE)
-        k.base[i] = ld_quad<T>(br[i], c0 + 4 * t, a.d_out);
-      else
-        k.base[i] = ld_apart(br[i] + c0 + t, a.d_out - c0 - t);
+      for (int i = 0; i < 2 * MT; ++i) k.base[i] = ld_quad<T>(br[i], c0 + 4 * t, a.d_out);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8 * MT; ++i) {
+        k.one[i] = 0.f;
+        if (c0 + lcol < a.d_out)
+          k.one[i] = ld_scalar(static_cast<const T*>(a.base) + row[min(2 * i + half, n - 1)] * a.ldbase + c0 + lcol);
+      }
     }
     if (STEPS > 0 && ad >= 0) {
 #pragma unroll
@@ -421,17 +391,29 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
         }
       }
     }
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const float4 v = base_f<T>(cur.base[i]);
-      const float* p0 = &acc[i >> 1][0][2 * (i & 1)];
-      const float* p1 = &acc[i >> 1][1][2 * (i & 1)];
-      if (g + 8 * i < n) {
-        const float4 o = make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]);
-        if constexpr (WIDE)
-          st_quad(outr[i], c0 + 4 * t, a.d_out, o);
-        else
-          st_apart(outr[i] + c0 + t, a.d_out - c0 - t, o);
+      for (int i = 0; i < 2 * MT; ++i) {
+        const float4 v = four_f(cur.base[i]);
+        const float* p0 = &acc[i >> 1][0][2 * (i & 1)];
+        const float* p1 = &acc[i >> 1][1][2 * (i & 1)];
+        if (g + 8 * i < n)
+          st_quad(outr[i], c0 + 4 * t, a.d_out, make_float4(v.x + p0[0], v.y + p0[1], v.z + p1[0], v.w + p1[1]));
+      }
+    } else {
+      __syncwarp();  // every lane has read the group before
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<float2*>(stage + (g + 8 * i) * LORA_LD + 8 * j + 2 * t) =
+              make_float2(acc[i >> 1][j][2 * (i & 1)], acc[i >> 1][j][2 * (i & 1) + 1]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8 * MT; ++i) {
+        const int rr = 2 * i + half;
+        stg_if_t<T>(static_cast<T*>(a.out) + row[min(rr, n - 1)] * a.ldout + c0 + lcol,
+                    cur.one[i] + stage[rr * LORA_LD + lcol], rr < n && c0 + lcol < a.d_out);
       }
     }
     cur = nxt;
