@@ -473,7 +473,7 @@ int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16,
  * its first one taken from the K - 1 rows of its source slot, and its last
  * K - 1 rows into its slot of `state` (n_slots, K - 1, channels), oldest row
  * first, in the type of x (an exact copy).  weight (channels, K, 1), K in
- * 1..8.  pieces: in row order, of vmscan_cached_conv_rows(rows, channels) rows
+ * 1..8, 16-byte aligned.  pieces: in row order, of vmscan_cached_conv_rows(rows, channels) rows
  * (host only: the faster length for that size; at least 8 is required).
  */
 int64_t vmscan_cached_conv_rows(int64_t rows, int64_t channels);

@@ -1490,14 +1490,14 @@ int launch_cached_conv(const CachedConvArgs& a, const int32_t* pieces, int64_t n
 
 template <typename T, bool WIDE, int STEPS>
 int launch_lora(const LoraArgs& l, int n_tiles, cudaStream_t s) {
-  // column shares (of whole 64-column rounds of the CTA's warps): a few tiles
+  // column shares (of whole 64-column turns of the CTA's warps): a few tiles
   // are spread over four CTAs an SM; each share forms the rank-wide products of
   // its tile again, which from two tiles an SM on costs more than it brings
   // (520 tiles 384 -> 1536, rank 16: 62 us in one share, 69 in two; 35 tiles:
   // 10.2 us in four shares, 8.5 in all 24)
-  const int rounds = (l.d_out + 16 * LORA_WARPS - 1) / (16 * LORA_WARPS), sms = sm_count();
-  const int shares = n_tiles >= 2 * sms ? 1 : std::min(rounds, (4 * sms + n_tiles - 1) / n_tiles);
-  const int cols = (rounds + shares - 1) / shares * 16 * LORA_WARPS;
+  const int turns = (l.d_out + 16 * LORA_WARPS - 1) / (16 * LORA_WARPS), sms = sm_count();
+  const int shares = n_tiles >= 2 * sms ? 1 : std::min(turns, (4 * sms + n_tiles - 1) / n_tiles);
+  const int cols = (turns + shares - 1) / shares * 16 * LORA_WARPS;
   const size_t smem = lora_smem<T>(l.rank);
   auto kern = lora_add_kernel<T, WIDE, STEPS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(lora_smem<T>(LORA_RMAX))) != cudaSuccess)

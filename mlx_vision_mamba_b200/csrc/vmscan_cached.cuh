@@ -102,6 +102,24 @@ __device__ __forceinline__ float4 ld_four(const T* p, bool wide) {
 // A request that would keep a few warps busy long after the others is split
 // into pieces.  CARRY: a piece whose start is not known yet only yields its
 // map h -> exp(A sum delta) h + (its end state from zero).
+//
+// Bound: the exponential unit.  A row of 32 channels is 512 decays, the gate's
+// exponential and reciprocal: 18 warp instructions of 8 cycles on that unit,
+// 144 cycles a scheduler, against 88 cycles of HBM traffic for fp32 at full
+// rate over all SMs and about 92 instructions to issue.  Measured on B200: 180
+// cycles with four warps a scheduler (64 requests of 512 rows x 1536, fp32,
+// gated: 277 us, 2.9e12 decays/s), 250 with one; the unit is busy 79 % of the
+// time in the first phase of 32 uneven prompts, 71 % in the second.  Of what
+// that took: rows through the ring instead of one register block ahead, an
+// explicit global store (338 -> 316 us on those 64 requests, with the decays
+// computed one row ahead), A in exponent units (-5 %).  Tried and slower:
+// part of the decays by a polynomial on the FMA pipe (one of eight pairs:
+// within 3 %, two: +9 %), one channel and 16 states a lane (fp32 +3 to 5 %),
+// five CTAs an SM, dependent launches that overlap (their waiting CTAs take
+// SMs unevenly: +27 % on uneven prompts).
+// Whole calls: 32 prompts of 32768 rows x 1536, bf16: 357 us; one prompt of
+// 32768 x 768 fp32: 253 us (in 96 pieces; 4.3 ms in one); 24 requests, 9001
+// rows x 768, fp32: 74 us; 196 rows x 768: 14.5 us.
 // ---------------------------------------------------------------------------
 constexpr int CSC_WARPS = 4;
 constexpr int CSC_ROWS = 8;
@@ -458,8 +476,12 @@ __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const fl
 // Single tokens: row i is request i.  A warp owns 32 channels of R rows; four
 // lanes share a channel (four states each), so the state moves as whole
 // 512-byte warp accesses, the R rows' of it in flight together and A read once
-// for them.  In round i the quad g works on channel 8 i + g; a transposing sum
+// for them.  In turn i the quad g works on channel 8 i + g; a transposing sum
 // over the quad leaves lane 4 g + q the output of channel 8 q + g, its own.
+// Bound: HBM, 128 bytes of state a channel and token.  256 x 1536 fp32, gated,
+// states from HBM: 13.3 us, 4.3 TB/s (16.2 with one state after the other in
+// scalar arithmetic, 390 instructions a warp instead of about 130); 1024 x
+// 1536: 45 us, 5.0 TB/s; 1 x 768: 2.1 us.
 // ---------------------------------------------------------------------------
 constexpr int CST_WARPS = 4;
 
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(CST_WARPS * 32)
     B4[r] = ld_four(static_cast<const T*>(a.B) + row * a.ldb + 4 * q, bc_wide != 0);
     C4[r] = ld_four(static_cast<const T*>(a.C) + row * a.ldc + 4 * q, bc_wide != 0);
   }
-  // rounds past the last channel repeat it and store nothing
+  // turns past the last channel repeat it and store nothing
   int64_t at[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) at[i] = int64_t(min(d0 + 8 * i + g, a.dn - 1)) * NS + 4 * q;
@@ -550,6 +572,11 @@ __global__ void __launch_bounds__(CST_WARPS * 32)
 // rows) reads the stored window, and writes the new one: the request's last
 // K - 1 rows, reaching back into the old window when it has fewer.  The same
 // thread reads the old window before it writes, so a slot may be both.
+// Bound: HBM, a read and a write of each element; with bf16 rows the
+// exponential unit is next (two of its operations an element, 22 us of the 46
+// below).  32768 x 1536, K = 4: fp32 70 us, 5.7 TB/s (148 with one row's loads
+// at a time), bf16 46 us; K = 8 fp32 111 us (the window of 7 rows before each
+// piece and 140 registers); 64 tokens x 768: 2.9 us.
 // ---------------------------------------------------------------------------
 constexpr int CCV_ROWS = 32;       // rows of a piece
 constexpr int CCV_FEW_ROWS = 16;   // where those would give the SMs too few threads (both at least K - 1)

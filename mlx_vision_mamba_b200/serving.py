@@ -181,7 +181,8 @@ class RequestBatch:
                                                    ptr(table) + 16 * most, ptr(table), most), "vmscan_lora_tiles")
             return _pinned(table), (int(most),)
         if kind == "scan":
-            rows, scan = lib.vmscan_cached_scan_rows(self.count, ptr(self.lengths), arg // 2, arg % 2), 1
+            with torch.cuda.device(self.index if self.index >= 0 and torch.cuda.is_initialized() else -1):
+                rows, scan = lib.vmscan_cached_scan_rows(self.count, ptr(self.lengths), arg // 2, arg % 2), 1
         else:
             rows, scan = lib.vmscan_cached_conv_rows(self.tokens, arg), 0
         if rows < 0:
