@@ -1370,13 +1370,32 @@ int cached_scan_grain(const CachedScanArgs& a) {
   return a.z != nullptr ? std::min(g, row_grain<T>(a.z, a.ldz, a.dn)) : g;
 }
 
+// A launch that may start before the kernel in front of it has ended (which
+// calls launch_next, and this one wait_previous), or an ordinary one.
+template <typename... P, typename... A>
+int launch_after(bool overlap, void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, P(args)...);
+  if (e == cudaSuccess) return VMSCAN_OK;
+  return fail(VMSCAN_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(e));
+}
+
 // Shared memory with which three CTAs fit an SM (228 KB, 1 KB of it reserved
 // for each CTA).
 constexpr size_t kScanThreePerSm = 62 * 1024;
 
 template <typename T, int G, bool HAS_Z>
-int launch_scan_phase(const CachedScanArgs& a, const int32_t* pieces, int64_t n, int groups, bool uneven, bool first,
-                      const ScanCarries& k, cudaStream_t s) {
+int launch_scan_phase(const CachedScanArgs& a, const int32_t* pieces, int64_t n, int groups, bool uneven, ScanPhase phase,
+                      bool overlap, const ScanCarries& k, cudaStream_t s) {
   auto kern = cached_scan_kernel<T, G, HAS_Z>;
   // Uneven pieces that nearly fill the four CTAs an SM holds are given three
   // (by claiming more shared memory): the short ones then fill in where the
@@ -1388,8 +1407,8 @@ int launch_scan_phase(const CachedScanArgs& a, const int32_t* pieces, int64_t n,
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kScanThreePerSm)) != cudaSuccess)
     return fail(VMSCAN_ERR_LAUNCH, "cudaFuncSetAttribute(cached_scan_kernel) failed");
   const int bc = std::min(row_grain<T>(a.B, a.ldb, NS), row_grain<T>(a.C, a.ldc, NS));
-  kern<<<unsigned(n * groups), CSC_WARPS * 32, smem, s>>>(a, pieces, groups, bc, first ? 1 : 0, k);
-  return check_launch();
+  return launch_after(overlap, kern, dim3(unsigned(n * groups)), dim3(CSC_WARPS * 32), smem, s, a, pieces, groups, bc,
+                      int(phase), k);
 }
 
 struct ScanPieces {
@@ -1406,18 +1425,22 @@ int launch_cached_scan(const CachedScanArgs& a, const ScanPieces& q, const Cache
   char* w = static_cast<char*>(ws);
   ScanCarries k{nullptr, nullptr, nullptr, 0};
   if (q.n_chains > 0) k = {reinterpret_cast<float*>(w), reinterpret_cast<float*>(w + p.carry), nullptr, p.rows};
-  VM_TRY((launch_scan_phase<T, G, HAS_Z>(a, q.pieces, q.n_first, p.groups, q.uneven, true, k, s)));
+  VM_TRY((launch_scan_phase<T, G, HAS_Z>(a, q.pieces, q.n_first, p.groups, q.uneven,
+                                          q.n > q.n_first ? SCAN_FIRST : SCAN_WHOLE, false, k, s)));
   if (q.n == q.n_first) return VMSCAN_OK;
+  // Overlapped where the CTAs of both phases find room at once (196 rows x 768:
+  // 14.5 -> 13.5 us); else those that wait take the SMs' places unevenly (32
+  // uneven prompts: 377 -> 477 us).
+  const bool overlap = q.n * p.groups <= 3 * int64_t(sm_count());
   if (q.longest > kChainInPiece) {
     float* start = reinterpret_cast<float*>(w + p.carry + p.sums);
     const int blocks = int((int64_t(a.dn) * NS + 127) / 128);
-    cached_chain_kernel<<<unsigned(q.n_chains * blocks), 128, 0, s>>>(q.chains, a.A, k.h, k.sum, start, a.dn, p.rows,
-                                                                     blocks);
-    VM_TRY(check_launch());
+    VM_TRY(launch_after(overlap, cached_chain_kernel, dim3(unsigned(q.n_chains * blocks)), dim3(128), 0, s, q.chains, a.A,
+                        k.h, k.sum, start, a.dn, p.rows, blocks));
     k.start = start;
   }
-  return launch_scan_phase<T, G, HAS_Z>(a, q.pieces + q.n_first * PF_COUNT, q.n - q.n_first, p.groups, q.uneven, false, k,
-                                        s);
+  return launch_scan_phase<T, G, HAS_Z>(a, q.pieces + q.n_first * PF_COUNT, q.n - q.n_first, p.groups, q.uneven,
+                                        SCAN_LATER, overlap, k, s);
 }
 
 template <typename T, int G>
@@ -1436,27 +1459,16 @@ int run_cached_scan(const CachedScanArgs& a, const ScanPieces& q, const CachedSc
   return launch_cached_scan_z<T, 4>(a, q, p, ws, s);
 }
 
-template <typename T, int R>
+template <typename T>
 int launch_cached_step(const CachedScanArgs& a, const int32_t* slots, const int32_t* sources, cudaStream_t s) {
   const int groups = (a.dn + CST_WARPS * 32 - 1) / (CST_WARPS * 32);
-  const unsigned grid = unsigned(int64_t((a.rows + R - 1) / R) * groups);
+  const unsigned grid = unsigned(int64_t(a.rows) * groups);
   const int wide = four_wide<T>(a.B, a.ldb) && four_wide<T>(a.C, a.ldc);
   if (a.z != nullptr)
-    cached_step_kernel<T, true, R><<<grid, CST_WARPS * 32, 0, s>>>(a, slots, sources, groups, wide);
+    cached_step_kernel<T, true><<<grid, CST_WARPS * 32, 0, s>>>(a, slots, sources, groups, wide);
   else
-    cached_step_kernel<T, false, R><<<grid, CST_WARPS * 32, 0, s>>>(a, slots, sources, groups, wide);
+    cached_step_kernel<T, false><<<grid, CST_WARPS * 32, 0, s>>>(a, slots, sources, groups, wide);
   return check_launch();
-}
-
-// Rows of a warp: one while that gives the SMs fewer warps than they hold, then
-// more, which read A once for all of them.
-// 256 x 1536 fp32 with states from HBM: 13.2 us with one row, 13.5 with two;
-// 1024 x 1536: 46.2 and 45.2; 333 x 771 bf16: 8.5 and 8.2.
-template <typename T>
-int run_cached_step(const CachedScanArgs& a, const int32_t* slots, const int32_t* sources, cudaStream_t s) {
-  const int64_t warps = int64_t(a.rows) * ((a.dn + 31) / 32);
-  if (warps <= int64_t(sm_count()) * 32) return launch_cached_step<T, 1>(a, slots, sources, s);
-  return launch_cached_step<T, 2>(a, slots, sources, s);
 }
 
 template <typename T>
@@ -1689,7 +1701,7 @@ int vmscan_cached_step(int64_t rows, int64_t d_inner, int64_t d_state, int bf16,
     return fail(VMSCAN_ERR_SHAPE, "cached step: rows %lld, d_inner %lld", (long long)rows, (long long)d_inner);
   VM_TRY(ensure_context(state));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return bf16 ? run_cached_step<__nv_bfloat16>(a, slots, sources, s) : run_cached_step<float>(a, slots, sources, s);
+  return bf16 ? launch_cached_step<__nv_bfloat16>(a, slots, sources, s) : launch_cached_step<float>(a, slots, sources, s);
 }
 
 int vmscan_cached_conv1d_silu(int64_t rows, int64_t channels, int64_t ksize, int bf16, const void* x, int64_t ldx,

@@ -59,6 +59,14 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);  // the output's one rounding (half a bf16 step)
 }
 
+// The launches of a small split scan overlap: a kernel lets the next one's CTAs
+// start while it runs (`launch_next`), and that one waits for all of it to be
+// done and visible (`wait_previous`) before it touches what they share.  Every
+// CTA of such a kernel waits, so that the end of the last one is the end of
+// all.  In a launch that does not overlap both do nothing.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct CachedScanArgs {
   const void* u;
   const void* delta;
@@ -115,11 +123,10 @@ __device__ __forceinline__ float4 ld_four(const T* p, bool wide) {
 // computed one row ahead), A in exponent units (-5 %).  Tried and slower:
 // part of the decays by a polynomial on the FMA pipe (one of eight pairs:
 // within 3 %, two: +9 %), one channel and 16 states a lane (fp32 +3 to 5 %),
-// five CTAs an SM, dependent launches that overlap (their waiting CTAs take
-// SMs unevenly: +27 % on uneven prompts).
+// five CTAs an SM.
 // Whole calls: 32 prompts of 32768 rows x 1536, bf16: 357 us; one prompt of
 // 32768 x 768 fp32: 253 us (in 96 pieces; 4.3 ms in one); 24 requests, 9001
-// rows x 768, fp32: 74 us; 196 rows x 768: 14.5 us.
+// rows x 768, fp32: 75 us; 196 rows x 768: 13.6 us.
 // ---------------------------------------------------------------------------
 constexpr int CSC_WARPS = 4;
 constexpr int CSC_ROWS = 8;
@@ -185,11 +192,12 @@ struct ScanCarries {
 
 template <typename T, int G, bool HAS_Z, bool CARRY>
 __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const Piece& p, int group, int bc_grain,
-                                                  const ScanCarries& k, unsigned char* smem_raw) {
+                                                  bool later, const ScanCarries& k, unsigned char* smem_raw) {
   constexpr bool LOAD_Z = HAS_Z && !CARRY;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ScanRing<T>& ring = reinterpret_cast<ScanRing<T>*>(smem_raw)[warp];
   const int d0 = (group * CSC_WARPS + warp) * 32;
+  if (later && (d0 >= a.dn || p.slot < 0)) wait_previous();
   if (d0 >= a.dn) return;  // whole warps: the rest shuffles and syncs by warp only
   const int hb = lane & 1, pc = lane & ~1;
   const int own = d0 + lane, dp = d0 + pc;
@@ -265,6 +273,7 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
     settle(p.t0 + k * CSC_ROWS, ring.st[k]);
   }
 
+  if (later) wait_previous();  // the rows are on their way; states and carries from here on
   float2 A2[2][4], h[2][4];
   const float* src = nullptr;
   if (!CARRY) {
@@ -422,19 +431,22 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
 // that a later piece finds its start and no slot is written before it is read):
 // first: whole requests and first pieces from their source's state, and the
 //        carries of the pieces between the first and the last one;
-// later: pieces after the first, from the chained carries.
+// later: pieces after the first, from the chained carries;
+// whole: no request is split, there is one launch.
+enum ScanPhase { SCAN_WHOLE, SCAN_FIRST, SCAN_LATER };
 template <typename T, int G, bool HAS_Z>
 __global__ void __launch_bounds__(CSC_WARPS * 32)
     cached_scan_kernel(const CachedScanArgs a, const int32_t* __restrict__ pieces, int groups, int bc_grain,
-                       int first_phase, const ScanCarries k) {
+                       int phase, const ScanCarries k) {
   extern __shared__ __align__(16) unsigned char scan_raw[];
   Piece p = load_piece(pieces, blockIdx.x / groups, a.rows, a.n_slots);
   p.carry = p.carry < k.rows ? p.carry : -1;
   p.ordinal = min(max(p.ordinal, 0), max(p.carry, 0));
-  if (first_phase && p.carry >= 0 && p.ordinal > 0)
-    cached_scan_piece<T, G, HAS_Z, true>(a, p, blockIdx.x % groups, bc_grain, k, scan_raw);
+  if (phase == SCAN_FIRST) launch_next();
+  if (phase == SCAN_FIRST && p.carry >= 0 && p.ordinal > 0)
+    cached_scan_piece<T, G, HAS_Z, true>(a, p, blockIdx.x % groups, bc_grain, false, k, scan_raw);
   else
-    cached_scan_piece<T, G, HAS_Z, false>(a, p, blockIdx.x % groups, bc_grain, k, scan_raw);
+    cached_scan_piece<T, G, HAS_Z, false>(a, p, blockIdx.x % groups, bc_grain, phase == SCAN_LATER, k, scan_raw);
 }
 
 // State entering every later piece of the split requests: chain i = {first
@@ -445,6 +457,8 @@ constexpr int CCH_AHEAD = 8;
 __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const float* __restrict__ A,
                                     const float* __restrict__ carry_h, const float* __restrict__ carry_s,
                                     float* __restrict__ h_start, int64_t dn, int rows, int blocks) {
+  launch_next();
+  wait_previous();
   const int64_t i = int64_t(blockIdx.x % blocks) * blockDim.x + threadIdx.x;
   if (i >= dn * NS) return;
   int4 c = reinterpret_cast<const int4*>(chains)[blockIdx.x / blocks];
@@ -459,8 +473,8 @@ __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const fl
     for (int q = 0; q < CCH_AHEAD; ++q) {
       const bool in = k0 + q + 1 < c.y;  // the last piece has no map
       const int64_t row = c.x + (in ? k0 + q : 0);
-      s[q] = in ? __ldg(carry_s + row * dn + ch) : 0.f;
-      g[q] = in ? __ldg(carry_h + row * dn * NS + i) : 0.f;
+      s[q] = in ? carry_s[row * dn + ch] : 0.f;
+      g[q] = in ? carry_h[row * dn * NS + i] : 0.f;
     }
 #pragma unroll
     for (int q = 0; q < CCH_AHEAD; ++q) {
@@ -473,96 +487,80 @@ __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const fl
 }
 
 // ---------------------------------------------------------------------------
-// Single tokens: row i is request i.  A warp owns 32 channels of R rows; four
+// Single tokens: row i is request i.  A warp owns 32 channels of one row; four
 // lanes share a channel (four states each), so the state moves as whole
-// 512-byte warp accesses, the R rows' of it in flight together and A read once
-// for them.  In turn i the quad g works on channel 8 i + g; a transposing sum
-// over the quad leaves lane 4 g + q the output of channel 8 q + g, its own.
+// 512-byte warp accesses, 2 KB of it in flight a warp.  In turn i the quad g
+// works on channel 8 i + g; a transposing sum over the quad leaves lane 4 g + q
+// the output of channel 8 q + g, its own.
 // Bound: HBM, 128 bytes of state a channel and token.  256 x 1536 fp32, gated,
-// states from HBM: 13.3 us, 4.3 TB/s (16.2 with one state after the other in
-// scalar arithmetic, 390 instructions a warp instead of about 130); 1024 x
-// 1536: 45 us, 5.0 TB/s; 1 x 768: 2.1 us.
+// states from HBM: 12.1 us, 4.7 TB/s (16.2 in scalar arithmetic, 390
+// instructions a warp instead of about 130; 13.4 with two rows a warp, whose
+// registers halve the warps an SM holds; 14.0 with ten CTAs an SM, which
+// spill); 1024 x 1536: 40 to 43 us, 5.3 to 5.7 TB/s; 1 x 768: 2.0 us.
 // ---------------------------------------------------------------------------
 constexpr int CST_WARPS = 4;
+constexpr int CST_CTAS = 8;  // an SM is to hold
 
-template <typename T, bool HAS_Z, int R>
-__global__ void __launch_bounds__(CST_WARPS * 32)
+template <typename T, bool HAS_Z>
+__global__ void __launch_bounds__(CST_WARPS * 32, CST_CTAS)
     cached_step_kernel(const CachedScanArgs a, const int32_t* __restrict__ slots, const int32_t* __restrict__ sources,
                        int groups, int bc_wide) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int row0 = (blockIdx.x / groups) * R;
+  const int row = blockIdx.x / groups;
   const int d0 = ((blockIdx.x % groups) * CST_WARPS + warp) * 32;
   if (d0 >= a.dn) return;
   const int own = d0 + 8 * q + g;
   const bool ok = own < a.dn;
   const int oc = min(own, a.dn - 1);
-  int slot[R], source[R];
-  float u[R], dl[R], z[R];
-  float4 B4[R], C4[R], h[R][4];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = min(row0 + r, a.rows - 1);
-    slot[r] = slots[row];
-    source[r] = sources[row];
-    u[r] = ld_one(static_cast<const T*>(a.u) + row * a.ldu + oc);
-    dl[r] = ld_one(static_cast<const T*>(a.delta) + row * a.ldd + oc);
-    z[r] = HAS_Z ? ld_one(static_cast<const T*>(a.z) + row * a.ldz + oc) : 0.f;
-    B4[r] = ld_four(static_cast<const T*>(a.B) + row * a.ldb + 4 * q, bc_wide != 0);
-    C4[r] = ld_four(static_cast<const T*>(a.C) + row * a.ldc + 4 * q, bc_wide != 0);
+  const int slot = slots[row], source = sources[row];
+  const float u = ld_one(static_cast<const T*>(a.u) + row * a.ldu + oc);
+  const float dl = ld_one(static_cast<const T*>(a.delta) + row * a.ldd + oc);
+  const float z = HAS_Z ? ld_one(static_cast<const T*>(a.z) + row * a.ldz + oc) : 0.f;
+  const float4 B4 = ld_four(static_cast<const T*>(a.B) + row * a.ldb + 4 * q, bc_wide != 0);
+  const float4 C4 = ld_four(static_cast<const T*>(a.C) + row * a.ldc + 4 * q, bc_wide != 0);
+  T* y = static_cast<T*>(a.y) + row * a.ldy + oc;
+  if (slot < 0 || slot >= a.n_slots) {  // padding request
+    stg_if_t<T>(y, 0.f, ok);
+    return;
   }
   // turns past the last channel repeat it and store nothing
   int64_t at[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) at[i] = int64_t(min(d0 + 8 * i + g, a.dn - 1)) * NS + 4 * q;
+  const bool kept = source >= 0 && source < a.n_slots;
+  const float* from = a.state + int64_t(kept ? source : 0) * a.dn * NS;
+  float* to = a.state + int64_t(slot) * a.dn * NS;
+  float4 h[4], A4[4];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const bool kept = source[r] >= 0 && source[r] < a.n_slots;
-    const float* from = a.state + int64_t(kept ? source[r] : 0) * a.dn * NS;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (kept) h[r][i] = *reinterpret_cast<const float4*>(from + at[i]);
-    }
+  for (int i = 0; i < 4; ++i) {
+    h[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kept) h[i] = *reinterpret_cast<const float4*>(from + at[i]);
   }
-  float4 A4[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) A4[i] = *reinterpret_cast<const float4*>(a.A + at[i]);
   const float Dd = a.D[oc];
+  const float du = dl * u, dlog = dl * kLog2e;
+  const float2 B0 = make_float2(B4.x, B4.y), B1 = make_float2(B4.z, B4.w);
+  const float2 C0 = make_float2(C4.x, C4.y), C1 = make_float2(C4.z, C4.w);
+  float part[4];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = row0 + r;
-    if (row >= a.rows) break;
-    T* y = static_cast<T*>(a.y) + row * a.ldy + oc;
-    if (slot[r] < 0 || slot[r] >= a.n_slots) {  // padding request
-      stg_if_t<T>(y, 0.f, ok);
-      continue;
-    }
-    float* to = a.state + int64_t(slot[r]) * a.dn * NS;
-    const float du = dl[r] * u[r], dlog = dl[r] * kLog2e;
-    const float2 B0 = make_float2(B4[r].x, B4[r].y), B1 = make_float2(B4[r].z, B4[r].w);
-    const float2 C0 = make_float2(C4[r].x, C4[r].y), C1 = make_float2(C4[r].z, C4[r].w);
-    float part[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 du2 = bcast2(__shfl_sync(0xffffffffu, du, (lane & ~3) + i));
-      const float2 dg = bcast2(__shfl_sync(0xffffffffu, dlog, (lane & ~3) + i)), off = bcast2(kEx2ArgBias);
-      const float2 e0 = fma2(dg, make_float2(A4[i].x, A4[i].y), off), e1 = fma2(dg, make_float2(A4[i].z, A4[i].w), off);
-      const float2 h0 = fma2(make_float2(ex2_approx(e0.x), ex2_approx(e0.y)), make_float2(h[r][i].x, h[r][i].y),
-                             mul2(du2, B0));
-      const float2 h1 = fma2(make_float2(ex2_approx(e1.x), ex2_approx(e1.y)), make_float2(h[r][i].z, h[r][i].w),
-                             mul2(du2, B1));
-      const float2 s = fma2(C1, h1, mul2(C0, h0));
-      part[i] = s.x + s.y;
-      if (d0 + 8 * i + g < a.dn) *reinterpret_cast<float4*>(to + at[i]) = make_float4(h0.x, h0.y, h1.x, h1.y);
-    }
-    // lane q of the quad keeps the sum of part[q] over the quad
-    const float p0 = (q & 1 ? part[1] : part[0]) + __shfl_xor_sync(0xffffffffu, q & 1 ? part[0] : part[1], 1);
-    const float p1 = (q & 1 ? part[3] : part[2]) + __shfl_xor_sync(0xffffffffu, q & 1 ? part[2] : part[3], 1);
-    const float sum = (q & 2 ? p1 : p0) + __shfl_xor_sync(0xffffffffu, q & 2 ? p0 : p1, 2);
-    float yy = fmaf(u[r], Dd, sum);
-    if (HAS_Z) yy *= silu_f(z[r]);
-    stg_if_t<T>(y, yy, ok);
+  for (int i = 0; i < 4; ++i) {
+    const float2 du2 = bcast2(__shfl_sync(0xffffffffu, du, (lane & ~3) + i));
+    const float2 dg = bcast2(__shfl_sync(0xffffffffu, dlog, (lane & ~3) + i)), off = bcast2(kEx2ArgBias);
+    const float2 e0 = fma2(dg, make_float2(A4[i].x, A4[i].y), off), e1 = fma2(dg, make_float2(A4[i].z, A4[i].w), off);
+    const float2 h0 = fma2(make_float2(ex2_approx(e0.x), ex2_approx(e0.y)), make_float2(h[i].x, h[i].y), mul2(du2, B0));
+    const float2 h1 = fma2(make_float2(ex2_approx(e1.x), ex2_approx(e1.y)), make_float2(h[i].z, h[i].w), mul2(du2, B1));
+    const float2 s = fma2(C1, h1, mul2(C0, h0));
+    part[i] = s.x + s.y;
+    if (d0 + 8 * i + g < a.dn) *reinterpret_cast<float4*>(to + at[i]) = make_float4(h0.x, h0.y, h1.x, h1.y);
   }
+  // lane q of the quad keeps the sum of part[q] over the quad
+  const float p0 = (q & 1 ? part[1] : part[0]) + __shfl_xor_sync(0xffffffffu, q & 1 ? part[0] : part[1], 1);
+  const float p1 = (q & 1 ? part[3] : part[2]) + __shfl_xor_sync(0xffffffffu, q & 1 ? part[2] : part[3], 1);
+  const float sum = (q & 2 ? p1 : p0) + __shfl_xor_sync(0xffffffffu, q & 2 ? p0 : p1, 2);
+  float yy = fmaf(u, Dd, sum);
+  if (HAS_Z) yy *= silu_f(z);
+  stg_if_t<T>(y, yy, ok);
 }
 
 // ---------------------------------------------------------------------------
