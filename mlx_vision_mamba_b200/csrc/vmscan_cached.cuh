@@ -102,7 +102,7 @@ __device__ __forceinline__ float4 ld_four(const T* p, bool wide) {
 // shared memory serves two channels.  The rows travel through a ring of
 // CSC_STAGES blocks of CSC_ROWS rows in the warp's own shared memory, filled by
 // asynchronous copies: a warp needs no other warp and no barrier, and one warp
-// alone on its scheduler still has 3 blocks in flight.
+// alone on its scheduler still has two blocks in flight.
 // G: bytes of one copy, the widest that the rows' alignment allows
 // (cached_scan_grain): 16, 4 (two bf16 or one fp32) or 2 (odd bf16 rows: plain
 // loads, kept in registers while the block before is computed).  bc_grain: the

@@ -515,6 +515,35 @@ def test_block_serves_what_it_computes(d_model):
     assert (cache.ssm[1] == 0).all() and (cache.conv[1] == 0).all()
 
 
+def test_block_serves_in_a_graph():
+    """Single tokens through a captured serve, replayed token after token with
+    new rows and then with other slots, equal the eager calls bit for bit."""
+    torch.manual_seed(3)
+    d, n = 64, 5
+    block = MambaBlock(d_model=d).cuda()
+    ain = LoraAdapters(torch.randn(2, 4, d, device="cuda") * 0.1, torch.randn(2, 4 * d, 4, device="cuda") * 0.1)
+    eager, cache = block.new_cache(8), block.new_cache(8)
+    prompts = RequestBatch([9, 4, 0, 30, 1], sources=[-1] * n, adapters=[0, 1, -1, 1, 0])
+    rows = torch.randn(44, d, device="cuda")
+    for c in (eager, cache):
+        block.serve(rows, c, prompts, ain)
+    tokens = RequestBatch([1] * n, adapters=[0, 1, -1, 1, 0])
+    x = torch.randn(n, d, device="cuda")
+    block.serve(x, block.new_cache(8), tokens, ain)  # the eager call before capture
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block.serve(x, cache, tokens, ain)
+    for k in range(4):
+        if k == 2:
+            tokens.update(slots=[0, 6, 2, -1, 4], sources=[0, 1, 2, -1, 4], adapters=[1, 0, 0, 0, -1])
+        if k == 3:
+            tokens.update(slots=[0, 6, 2, 3, 4])
+        x.copy_(torch.randn(n, d, device="cuda"))
+        want = block.serve(x, eager, tokens, ain)
+        graph.replay()
+        assert torch.equal(out, want) and torch.equal(cache.ssm, eager.ssm) and torch.equal(cache.conv, eager.conv)
+
+
 def test_block_serves_adapters():
     """Adapters on in_proj and out_proj are those projections with W + scale B A."""
     torch.manual_seed(1)
