@@ -1289,10 +1289,15 @@ struct PieceSplit {
 // Measured on B200 (gated): cycles that a row of 32 channels takes on a
 // scheduler with four warps, there only for its carry, and on a scheduler with
 // one warp (with odd bf16 rows, whose loads go through registers); a piece's
-// start (parameters, state, first rows); a launch in the middle of a call; a
-// piece in the chain.
+// start (parameters, state, first rows); a launch in the middle of a call,
+// on its own or overlapped (with one cost for both a call of 196 rows x 768 was
+// cut into 8 pieces chained in place, 13.5 us, instead of 12 chained by a
+// kernel, 11.6; 4 x 196 18.4, now 15.9; 64 x 768 10.9, now 8.4); a piece in the
+// chain.
 constexpr double kScanMainCycles = 185, kScanCarryCycles = 145, kScanAloneCycles = 255, kScanOddAloneCycles = 490,
-                 kScanStartCycles = 1200, kScanLaunchCycles = 8000, kScanChainCycles = 80;
+                 kScanStartCycles = 1200, kScanLaunchCycles = 8000, kScanOverlapCycles = 3000, kScanChainCycles = 80;
+// CTAs an SM up to which the launches of a call overlap.
+constexpr int kScanOverlapPerSm = 3;
 // how much longer a row takes with one, two, three warps on a scheduler than with four
 constexpr double kScanFew[4] = {1.38, 1.15, 1.06, 1.0};
 constexpr int64_t kScanMinRows = 16;
@@ -1428,10 +1433,10 @@ int launch_cached_scan(const CachedScanArgs& a, const ScanPieces& q, const Cache
   VM_TRY((launch_scan_phase<T, G, HAS_Z>(a, q.pieces, q.n_first, p.groups, q.uneven,
                                           q.n > q.n_first ? SCAN_FIRST : SCAN_WHOLE, false, k, s)));
   if (q.n == q.n_first) return VMSCAN_OK;
-  // Overlapped where the CTAs of both phases find room at once (196 rows x 768:
-  // 14.5 -> 13.5 us); else those that wait take the SMs' places unevenly (32
-  // uneven prompts: 377 -> 477 us).
-  const bool overlap = q.n * p.groups <= 3 * int64_t(sm_count());
+  // Overlapped where the CTAs of both phases find room at once (196 rows x 768
+  // in 8 pieces: 14.5 -> 13.5 us); else those that wait take the SMs' places
+  // unevenly (32 uneven prompts: 377 -> 477 us).
+  const bool overlap = q.n * p.groups <= kScanOverlapPerSm * int64_t(sm_count());
   if (q.longest > kChainInPiece) {
     float* start = reinterpret_cast<float*>(w + p.carry + p.sums);
     const int blocks = int((int64_t(a.dn) * NS + 127) / 128);
@@ -1510,6 +1515,8 @@ int launch_lora(const LoraArgs& l, int n_tiles, cudaStream_t s) {
   const int turns = (l.d_out + 16 * LORA_WARPS - 1) / (16 * LORA_WARPS), sms = sm_count();
   const int shares = n_tiles >= 2 * sms ? 1 : std::min(turns, (4 * sms + n_tiles - 1) / n_tiles);
   const int cols = (turns + shares - 1) / shares * 16 * LORA_WARPS;
+  // shared memory and fragments are laid out for ceil(rank / 16) steps of 16 columns
+  if (STEPS > 0 && STEPS != (l.rank + 15) / 16) return fail(VMSCAN_ERR_SHAPE, "lora: variant of another rank");
   const size_t smem = lora_smem<T>(l.rank);
   auto kern = lora_add_kernel<T, WIDE, STEPS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(lora_smem<T>(LORA_RMAX))) != cudaSuccess)
@@ -1576,9 +1583,10 @@ int64_t vmscan_cached_scan_rows(int64_t count, const int32_t* lengths, int64_t d
       }
       pieces = std::max(pieces, p.count);
     }
+    const double launch = (n1 + n2) * groups <= kScanOverlapPerSm * sms ? kScanOverlapCycles : kScanLaunchCycles;
     double t = phase(n1, work1, long1);
-    if (pieces > 1) t += phase(n2, work2, long2) + kScanLaunchCycles;
-    if (pieces > kChainInPiece) t += kScanLaunchCycles + double(pieces) * kScanChainCycles;
+    if (pieces > 1) t += phase(n2, work2, long2) + launch;
+    if (pieces > kChainInPiece) t += launch + double(pieces) * kScanChainCycles;
     if (k == 1 || t < best) {
       best = t;
       best_rows = rows;

@@ -126,7 +126,7 @@ __device__ __forceinline__ float4 ld_four(const T* p, bool wide) {
 // five CTAs an SM.
 // Whole calls: 32 prompts of 32768 rows x 1536, bf16: 357 us; one prompt of
 // 32768 x 768 fp32: 253 us (in 96 pieces; 4.3 ms in one); 24 requests, 9001
-// rows x 768, fp32: 75 us; 196 rows x 768: 13.6 us.
+// rows x 768, fp32: 75 us; 196 rows x 768: 11.6 us.
 // ---------------------------------------------------------------------------
 constexpr int CSC_WARPS = 4;
 constexpr int CSC_ROWS = 8;
