@@ -23,9 +23,9 @@
 //
 // Measured on B200: 16384 rows 384 -> 1536, rank 16, fp32 50 us, 4.6 TB/s of
 // the 227 MB that have to move (the floor is 35 us; 14 warps an SM wait for
-// base and B); 768 -> 1536, rank 64, bf16 67 us and fp32 128 us (three TF32
+// base and B); 768 -> 1536, rank 64, bf16 67 us and fp32 131 us (three TF32
 // products a term: the tensor pipe alone takes about 50); 64 rows of 32
-// adapters 384 -> 1536, rank 16: 6.1 us (latency: row list, x and A, S, B).
+// adapters 384 -> 1536, rank 16: 6.3 us (latency: row list, x and A, S, B).
 // Rings of asynchronous copies for x, base and B cost more occupancy than they
 // hid (62 to 74 us on the first case at the time, 53 without).
 #pragma once
@@ -150,9 +150,17 @@ __device__ __forceinline__ void st_quad(T* row, int c, int limit, const float4& 
   }
 }
 
+// TF32 parts of an fp32 word.  The integer rounding of hi carries a NaN whose
+// mantissa is all ones (the one the hardware makes) over to zero; the rounding
+// of lo is the conversion instruction, which keeps the NaN that x - hi then is,
+// as it is for infinities, so that neither is lost (lo rounded the integer way
+// too lost them and took 6.1 instead of 6.3 us for 64 rows of 32 adapters, rank
+// 16, 106 instead of 108 us at rank 64; both parts by conversion 6.7 and 113).
 __device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return (x + 0x1000u) & 0xFFFFE000u; }
 __device__ __forceinline__ uint32_t tf32_lo(uint32_t x, uint32_t hi) {
-  return __float_as_uint(tf32_round(__uint_as_float(x) - __uint_as_float(hi)));
+  uint32_t lo;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(__uint_as_float(x) - __uint_as_float(hi)));
+  return lo;
 }
 
 // Fragments of S for 16 rank columns and one 16-row block, as groups of four

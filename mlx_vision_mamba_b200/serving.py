@@ -336,6 +336,7 @@ def lora_add_cuda(base: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, b
     request are base's.  `out` (rows, d_out) receives the result: base itself
     for an update in place, or a tensor that overlaps neither base nor x
     (default: a new one).  Products and sums are fp32; a bf16 result is rounded
-    once.
+    once.  A row of x with a NaN or an infinity comes out as NaN (or infinite)
+    where its request has an adapter, whatever the factors.
     """
     return (_ext_module or _ext()).lora(base, x, adapters, batch, out)

@@ -277,6 +277,49 @@ def test_lora(lengths, d_in, d_out, rank, dtype):
     assert lora_add_cuda(inside, x, ads, batch, out=inside) is inside and torch.equal(inside, y)
 
 
+@pytest.mark.parametrize("rank", [5, 16, 24, 64, 100])
+@pytest.mark.parametrize("dtype,d_in,d_out", [(F32, 40, 72), (F32, 41, 70), (BF16, 40, 72)])
+def test_lora_keeps_what_is_not_finite(rank, dtype, d_in, d_out):
+    """NaN (of any pattern) and infinities in a row, or in a factor, reach the
+    outputs that the formula sums them into, and no others."""
+    batch = RequestBatch([20, 3, 1, 9, 2], adapters=[0, 1, -1, 2, 1])
+    base, x, ads = _lora_inputs(batch, 3, d_in, d_out, rank, dtype, seed=rank)
+    clean = lora_add_cuda(base, x, ads, batch)
+    assert torch.isfinite(clean).all()
+    patterns = {F32: [0x7FC00000, 0x7FFFFFFF, 0x7F800001, -1, -0x400000], BF16: [0x7FC0, 0x7FFF, 0x7F81, -1, -0x40]}[dtype]
+    bits = torch.int32 if dtype == F32 else torch.int16
+    nans = torch.tensor(patterns, device="cuda", dtype=bits).view(dtype)
+    assert torch.isnan(nans).all()
+    bad = x.clone()
+    for i in range(5):
+        bad[3 * i, (7 * i) % d_in] = nans[i]
+    bad[20, d_in - 1], bad[34, 0] = nans[1], nans[3]
+    bad[1, 2], bad[21, 5], bad[30, 1] = float("inf"), float("-inf"), float("inf")
+    bad[23] = nans[1]  # the request without an adapter
+    y = lora_add_cuda(base, bad, ads, batch)
+    nan_rows, inf_rows = [0, 3, 6, 9, 12, 20, 34], [1, 21, 30]
+    assert torch.isnan(y[nan_rows]).all() and not torch.isfinite(y[inf_rows]).any()
+    others = [i for i in range(35) if i not in nan_rows + inf_rows]
+    assert torch.equal(y[others], clean[others])
+    for nan in nans:
+        ads.a[1, rank - 1, 3] = nan
+        y = lora_add_cuda(base, x, ads, batch)
+        rows = [20, 21, 22, 33, 34]
+        assert torch.isnan(y[rows]).all()
+        others = [i for i in range(35) if i not in rows]
+        assert torch.equal(y[others], clean[others])
+        ads.a[1, rank - 1, 3] = 0.5
+        kept = ads.b[0, d_out - 1, rank - 1].clone()
+        ads.b[0, d_out - 1, rank - 1] = nan
+        y = lora_add_cuda(base, x, ads, batch)
+        assert torch.isnan(y[:20, d_out - 1]).all() and torch.equal(y[:20, :d_out - 1], clean[:20, :d_out - 1])
+        ads.b[0, d_out - 1, rank - 1] = kept
+        weird = base.clone()
+        weird[4, 6] = nan
+        y = lora_add_cuda(weird, x, ads, batch)
+        assert torch.isnan(y[4, 6]) and torch.isfinite(y).sum() == y.numel() - 1
+
+
 def test_lora_strides_and_rows_behind():
     batch = RequestBatch([5, 20, 1], adapters=[1, -1, 0])
     base, x, ads = _lora_inputs(batch, 2, 40, 30, 8, F32, rows=31)
