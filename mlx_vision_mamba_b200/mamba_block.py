@@ -29,7 +29,7 @@ from .direction import BACKWARD, ScanDirection, directions_for
 from .branches import block_core_forward, block_core_ok, branches_forward
 from .linear import linear_tc, supported as _tc_supported
 from .norm import layer_norm_cuda as _layer_norm_cuda, supported as _ln_supported
-from .scan import conv1d_silu_cuda, dt_softplus_cuda, selective_scan_cuda
+from .scan import D_STATE, conv1d_silu_cuda, dt_softplus_cuda, selective_scan_cuda
 from .serving import (
     LoraAdapters,
     RequestBatch,
@@ -192,6 +192,14 @@ class MambaBlock(nn.Module):
         if x.dim() != 2 or x.shape[1] != self.d_model or x.dtype != torch.float32:
             raise ValueError(f"MambaBlock.serve: x must be (rows, {self.d_model}) fp32, got {tuple(x.shape)} {x.dtype}")
         dn, r, n = self.d_inner, self.dt_rank, self.d_state
+        # what only a later step would refuse, before the conv windows move on
+        if n != D_STATE or cache.ssm.shape != (cache.conv.shape[0], dn, n) or cache.ssm.device != cache.conv.device:
+            raise ValueError(f"MambaBlock.serve: d_state must be {D_STATE} and the cache one of this block, got d_state "
+                             f"{n} and states {tuple(cache.ssm.shape)}")
+        if out_adapters is not None:
+            if not isinstance(out_adapters, LoraAdapters):
+                raise TypeError(f"MambaBlock.serve: out_adapters must be LoraAdapters, got {type(out_adapters).__name__}")
+            out_adapters.check("MambaBlock.serve", dn, self.d_model, x.dtype, batch)
         xz = project(x, self.in_proj.weight)
         if in_adapters is not None:
             lora_add_cuda(xz, x, in_adapters, batch, out=xz)

@@ -272,6 +272,22 @@ class LoraAdapters:
             raise ValueError(f"LoraAdapters: scale must have {self.count} entries, got {tuple(scale.shape)}")
         self.scale = scale.detach().to(a.device, copy=True).contiguous()
 
+    def check(self, where: str, d_in: int, d_out: int, dtype: torch.dtype, batch: RequestBatch) -> None:
+        """Raises unless lora_add_cuda takes these adapters for x (rows, d_in)
+        and base (rows, d_out) of a type and a batch."""
+        if not isinstance(batch, RequestBatch):
+            raise TypeError(f"{where}: `batch` must be a RequestBatch, got {type(batch).__name__}")
+        if (self.d_in, self.d_out) != (d_in, d_out):
+            raise ValueError(f"{where}: adapters of {self.d_in} -> {self.d_out} beside a projection {d_in} -> {d_out}")
+        if self.a.dtype != dtype:
+            raise TypeError(f"{where}: adapters are {self.a.dtype}, the activations {dtype}")
+        if self.a.get_device() != batch.index:
+            raise ValueError(f"{where}: the adapters are on {self.a.device}, the batch is for device {batch.index}")
+        if batch.max_adapter < -1:
+            raise ValueError(f"{where}: the batch was made without adapters")
+        if batch.max_adapter >= self.count:
+            raise ValueError(f"{where}: the batch uses adapter {batch.max_adapter}, there are {self.count}")
+
 
 _ext_module = None
 

@@ -587,6 +587,39 @@ def test_block_serves_in_a_graph():
         assert torch.equal(out, want) and torch.equal(cache.ssm, eager.ssm) and torch.equal(cache.conv, eager.conv)
 
 
+def test_a_refused_serve_leaves_the_cache_as_it_was():
+    d = 32
+    block = MambaBlock(d_model=d).cuda()
+    cache = block.new_cache(2)
+    batch, plain = RequestBatch([3, 1], adapters=[0, 1]), RequestBatch([3, 1])
+    x = torch.randn(4, d, device="cuda")
+    block.serve(x, cache, batch)
+    conv, ssm = cache.conv.clone(), cache.ssm.clone()
+
+    def adapters(count, d_in, d_out, dtype=F32):
+        return LoraAdapters(torch.ones(count, 4, d_in, device="cuda", dtype=dtype),
+                            torch.ones(count, d_out, 4, device="cuda", dtype=dtype))
+
+    good = adapters(2, 2 * d, d)
+    for out, bt, error in ((adapters(1, 2 * d, d), batch, ValueError), (adapters(2, d, d), batch, ValueError),
+                           (adapters(2, 2 * d, d + 1), batch, ValueError), (good, plain, ValueError),
+                           (adapters(2, 2 * d, d, BF16), batch, TypeError), (good.a, batch, TypeError)):
+        with pytest.raises(error):
+            block.serve(x, cache, bt, out_adapters=out)
+    other = block.new_cache(2)
+    other.conv = cache.conv
+    other.ssm = other.ssm[:1]
+    with pytest.raises(ValueError):
+        block.serve(x, other, batch)
+    narrow = MambaBlock(d_model=d, d_state=8).cuda()
+    nc = narrow.new_cache(2)
+    with pytest.raises(ValueError, match="d_state"):
+        narrow.serve(x, nc, batch)
+    assert torch.equal(cache.conv, conv) and torch.equal(cache.ssm, ssm) and not nc.conv.any()
+    block.serve(x, cache, batch, out_adapters=good)
+    assert not torch.equal(cache.conv, conv)
+
+
 def test_block_serves_adapters():
     """Adapters on in_proj and out_proj are those projections with W + scale B A."""
     torch.manual_seed(1)
