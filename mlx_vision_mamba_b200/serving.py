@@ -58,15 +58,30 @@ def _int_list(name: str, values, count: Optional[int] = None) -> np.ndarray:
 
 class _Table:
     """A device table, its pinned source, the stream it was made on and what the
-    operators are told of it: (address, sizes...).  limit: slots of the smallest
-    cache that a captured graph uses it with."""
+    operators are told of it: (address, sizes...).  captured: a graph uses it;
+    limit: slots of the smallest cache that one uses it with."""
 
-    __slots__ = ("tensor", "host", "stream", "told", "limit")
+    __slots__ = ("tensor", "host", "stream", "told", "captured", "limit")
 
     def __init__(self, host, info, device):
         self.host, self.stream = host, torch.cuda.current_stream(device)
-        self.tensor = host.to(device, non_blocking=True)
-        self.told, self.limit = (self.tensor.data_ptr(), *info), None
+        # an inference tensor could not be rewritten by an update outside inference mode
+        with torch.inference_mode(False):
+            self.tensor = torch.empty(host.shape, dtype=host.dtype, device=device)
+            self.tensor.copy_(host, non_blocking=True)
+        self.told, self.captured, self.limit = (self.tensor.data_ptr(), *info), False, None
+
+    def write(self, host, here):
+        """The table becomes `host` on stream `here`, after what its own stream
+        has been given and before what that one is given next."""
+        if self.stream != here:
+            here.wait_stream(self.stream)
+        try:
+            with torch.cuda.stream(here):
+                self.tensor.copy_(host, non_blocking=True)
+        finally:
+            if self.stream != here:
+                self.stream.wait_stream(here)
 
 
 class RequestBatch:
@@ -135,7 +150,8 @@ class RequestBatch:
         The device tables are rewritten on the current stream, after what other
         streams have run with this batch so far and before what they run later;
         graphs captured with it must be replayed in order with the current
-        stream.  Nothing changes when the new values are refused."""
+        stream.  Nothing changes when the new values are refused or a table
+        cannot be rewritten."""
         if _capturing():
             raise RuntimeError("RequestBatch.update: not while a CUDA graph is being captured")
         names = ("slots", "sources", "adapters", "_adapters_given", "max_slot", "max_adapter")
@@ -155,14 +171,23 @@ class RequestBatch:
         if not new:
             return
         here = torch.cuda.current_stream(self.device)
+        written = []
+        try:
+            for table, host, _ in new:
+                table.write(host, here)
+                written.append(table)
+        except Exception:
+            # The values go back, and with them what the graphs read; the tables
+            # that no graph holds are made anew by the next call that needs them.
+            for n, v in before.items():
+                setattr(self, n, v)
+            self._tables = {k: t for k, t in self._tables.items() if t.captured}
+            for table in written:
+                if table.captured:
+                    table.write(table.host, here)
+            raise
         for table, host, _ in new:
-            if table.stream != here:
-                here.wait_stream(table.stream)
-            with torch.cuda.stream(here):
-                table.tensor.copy_(host, non_blocking=True)
             table.host = host
-            if table.stream != here:
-                table.stream.wait_stream(here)
 
     def _build(self, key):
         """(pinned int32 host table, its sizes) of kind key[0]."""
@@ -206,6 +231,7 @@ class RequestBatch:
                 table = next((t for k, t in self._tables.items() if k[:2] == key[:2]), None)
             if table is None:
                 raise RuntimeError("RequestBatch: call the operator once with this batch before capturing it")
+            table.captured = True
             if kind != "lora":
                 table.limit = slots if table.limit is None else min(slots, table.limit)
         elif table is None:

@@ -2,6 +2,8 @@
 RequestBatch and of the operators, and the tables that tell the kernels which
 rows, slots and adapters they work on."""
 
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -219,3 +221,68 @@ def test_c_entry_points_validate():
     assert lora(r=0) == 2 and lora(r=129) == 2 and lora(rows=0) == 2 and lora(ni=5) == 2 and lora(nt=0) == 2
     assert lora(r=3) == 4 and lora(lda=6) == 4 and lora(lda=4) == 4 and lora(bf16=1, lda=12) == 4 and lora(a=P + 4) == 4
     assert lora(x=None) == 1 and lora(s=None) == 1 and lora(tiles=P + 4) == 4 and lora(ldo=7) == 2
+
+
+class _Stream:
+    """Stands in for a CUDA stream: notes what it was made to wait for."""
+
+    def __init__(self):
+        self.waits = []
+
+    def wait_stream(self, other):
+        self.waits.append(other)
+
+
+@pytest.fixture
+def host_streams(monkeypatch):
+    """The tables of a batch on the host, made and rewritten on stand-in
+    streams; returns the function that sets the current one."""
+    now = [_Stream()]
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now[0])
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    return lambda s: now.__setitem__(0, s)
+
+
+def _step_table(batch, key, capturing=False, slots=99):
+    batch._table("step", key, 0, capturing, slots)
+    return batch._tables[("step", 0, key)]
+
+
+def test_an_update_outside_inference_mode_reaches_tables_made_inside(host_streams):
+    a, b = _Stream(), _Stream()
+    batch = RequestBatch([1, 1], device="cpu")
+    with torch.inference_mode():
+        tables = [_step_table(batch, 1), batch._table("conv", 1, 64, False, 9) and batch._tables[("conv", 64, 1)]]
+        host_streams(a)
+        tables.append(_step_table(batch, 2))
+    host_streams(b)
+    batch.update(slots=[5, 6], sources=[-1, 6])
+    assert tables[0].tensor.tolist() == tables[2].tensor.tolist() == [5, 6, -1, 6]
+    assert tables[1].tensor.view(-1, 8)[:, 4:6].tolist() == [[-1, 5], [6, 6]]
+    assert all(t.tensor.tolist() == t.host.tolist() and set(t.stream.waits) == {b} for t in tables)
+    assert b.waits == [tables[0].stream, tables[0].stream, a]
+    with torch.inference_mode():
+        batch.update(slots=[7, 8])
+    assert tables[2].tensor.tolist() == [7, 8, 7, 8] and _step_table(batch, 2) is tables[2]
+
+
+def test_a_failed_update_leaves_batch_and_tables_as_they_were(host_streams):
+    batch = RequestBatch([1, 1], slots=[3, 4], device="cpu")
+    first, second, third = (_step_table(batch, k) for k in (1, 2, 3))
+    _step_table(batch, 1, capturing=True)  # a graph holds the first one
+    address = first.told
+
+    class Fails:
+        def copy_(self, *args, **kw):
+            raise RuntimeError("copy")
+
+    kept, third.tensor = third.tensor, Fails()
+    with pytest.raises(RuntimeError, match="copy"):
+        batch.update(slots=[5, 6])
+    assert batch.slots.tolist() == batch.sources.tolist() == [3, 4] and batch.max_slot == 4
+    assert first.tensor.tolist() == first.host.tolist() == [3, 4, 3, 4] and kept.tolist() == [3, 4, 3, 4]
+    assert _step_table(batch, 1) is first and first.told == address
+    for k, old in ((2, second), (3, third)):  # not held by a graph: made anew, with the batch's values
+        assert _step_table(batch, k) is not old and _step_table(batch, k).tensor.tolist() == [3, 4, 3, 4]
+    batch.update(slots=[5, 6])
+    assert all(t.tensor.tolist() == [5, 6, 5, 6] for t in batch._tables.values())
