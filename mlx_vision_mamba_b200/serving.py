@@ -145,8 +145,9 @@ class RequestBatch:
         self.max_adapter = -2 if adapters is None else int(adapters.max())  # -2: made without adapters
 
     def update(self, slots=None, sources=None, adapters=None) -> None:
-        """New slots, sources and adapters (slots and sources default as in the
-        constructor; adapters None keeps the present ones) for the same lengths.
+        """New slots, sources and adapters for the same lengths.  What is left
+        out stays as it is, but for the sources of new slots, which default to
+        the requests' own slots as in the constructor.
         The device tables are rewritten on the current stream, after what other
         streams have run with this batch so far and before what they run later;
         graphs captured with it must be replayed in order with the current
@@ -156,6 +157,8 @@ class RequestBatch:
             raise RuntimeError("RequestBatch.update: not while a CUDA graph is being captured")
         names = ("slots", "sources", "adapters", "_adapters_given", "max_slot", "max_adapter")
         before = {n: getattr(self, n) for n in names}
+        if slots is None:
+            slots, sources = self.slots, self.sources if sources is None else sources
         try:
             self._set(slots, sources, self._adapters_given if adapters is None else adapters)
             limit = min((t.limit for t in self._tables.values() if t.limit is not None), default=None)

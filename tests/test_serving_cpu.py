@@ -71,6 +71,20 @@ def test_a_batch_keeps_what_it_checked():
     assert b.slots.tolist() == [1, 2] and b.max_slot == 2
 
 
+def test_an_update_keeps_what_it_is_not_given():
+    b = RequestBatch([1, 1, 1], slots=[5, 6, -1], sources=[-1, 8, 0], adapters=[0, 1, 2])
+    b.update(adapters=[2, 2, 2])
+    assert b.slots.tolist() == [5, 6, -1] and b.sources.tolist() == [-1, 8, -1] and b.adapters.tolist() == [2, 2, -1]
+    b.update()
+    assert b.slots.tolist() == [5, 6, -1] and b.sources.tolist() == [-1, 8, -1] and b.max_slot == 8
+    b.update(sources=[5, -1, -1])
+    assert b.slots.tolist() == [5, 6, -1] and b.sources.tolist() == [5, -1, -1]
+    with pytest.raises(ValueError):
+        b.update(sources=[6, -1, -1])  # the second request writes it
+    b.update(slots=[7, 8, 9])  # new slots: their own are the sources
+    assert b.sources.tolist() == [7, 8, 9] and b.adapters.tolist() == [2, 2, 2] and b.max_slot == 9
+
+
 def _pieces(batch, rows, scan):
     lib = _native.load()
     info = np.zeros(5, dtype=np.int64)
