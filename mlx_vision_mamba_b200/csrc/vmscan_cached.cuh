@@ -63,7 +63,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
 // start while it runs (`launch_next`), and that one waits for all of it to be
 // done and visible (`wait_previous`) before it touches what they share.  Every
 // CTA of such a kernel waits, so that the end of the last one is the end of
-// all.  In a launch that does not overlap both do nothing.
+// all.  In a launch that does not overlap both do nothing.  What the launch
+// before writes (states, carries) is read through plain pointers only: a
+// `const __restrict__` parameter says that nobody writes the data while the
+// kernel runs, and its loads need not stay behind wait_previous.
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -455,8 +458,8 @@ __global__ void __launch_bounds__(CSC_WARPS * 32)
 // many pieces: a few are chained by the pieces themselves.
 constexpr int CCH_AHEAD = 8;
 __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const float* __restrict__ A,
-                                    const float* __restrict__ carry_h, const float* __restrict__ carry_s,
-                                    float* __restrict__ h_start, int64_t dn, int rows, int blocks) {
+                                    const float* carry_h, const float* carry_s, float* h_start, int64_t dn, int rows,
+                                    int blocks) {
   launch_next();
   wait_previous();
   const int64_t i = int64_t(blockIdx.x % blocks) * blockDim.x + threadIdx.x;

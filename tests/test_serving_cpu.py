@@ -3,6 +3,8 @@ RequestBatch and of the operators, and the tables that tell the kernels which
 rows, slots and adapters they work on."""
 
 import contextlib
+import os
+import re
 
 import numpy as np
 import pytest
@@ -12,6 +14,7 @@ from mlx_vision_mamba_b200 import (
     LoraAdapters,
     RequestBatch,
     _native,
+    build,
     conv1d_silu_cached_cuda,
     lora_add_cuda,
     selective_scan_cached_cuda,
@@ -300,3 +303,20 @@ def test_a_failed_update_leaves_batch_and_tables_as_they_were(host_streams):
         assert _step_table(batch, k) is not old and _step_table(batch, k).tensor.tolist() == [3, 4, 3, 4]
     batch.update(slots=[5, 6])
     assert all(t.tensor.tolist() == [5, 6, 5, 6] for t in batch._tables.values())
+
+
+def test_overlapped_kernels_read_carries_through_plain_pointers():
+    """A kernel that starts under the one before it must not declare what that
+    one writes read-only for its whole life (`const ... __restrict__`): only
+    parameters and host tables may be."""
+    with open(os.path.join(build.CSRC, "vmscan_cached.cuh")) as f:
+        kernels = re.split(r"__global__", f.read())[1:]
+    checked = []
+    for text in kernels:
+        name, params = re.match(r".*?(\w+_kernel)\((.*?)\)\s*\{", text, re.S).groups()
+        body = text.split("\n}\n")[0]
+        if "launch_next()" in body or "wait_previous()" in body:
+            qualified = {p.split()[-1] for p in params.split(",") if "__restrict__" in p}
+            assert qualified <= {"chains", "pieces", "A"}, (name, qualified)
+            checked.append(name)
+    assert checked == ["cached_scan_kernel", "cached_chain_kernel"]
