@@ -29,7 +29,7 @@ from .direction import BACKWARD, ScanDirection, directions_for
 from .branches import block_core_forward, block_core_ok, branches_forward
 from .linear import linear_tc, supported as _tc_supported
 from .norm import layer_norm_cuda as _layer_norm_cuda, supported as _ln_supported
-from .scan import D_STATE, conv1d_silu_cuda, dt_softplus_cuda, selective_scan_cuda
+from .scan import D_STATE, DT_RANK_MAX, DT_ROWS_MAX, conv1d_silu_cuda, dt_softplus_cuda, selective_scan_cuda
 from .serving import (
     LoraAdapters,
     RequestBatch,
@@ -193,9 +193,16 @@ class MambaBlock(nn.Module):
             raise ValueError(f"MambaBlock.serve: x must be (rows, {self.d_model}) fp32, got {tuple(x.shape)} {x.dtype}")
         dn, r, n = self.d_inner, self.dt_rank, self.d_state
         # what only a later step would refuse, before the conv windows move on
-        if n != D_STATE or cache.ssm.shape != (cache.conv.shape[0], dn, n) or cache.ssm.device != cache.conv.device:
+        ssm = cache.ssm
+        if n != D_STATE or ssm.shape != (cache.conv.shape[0], dn, n) or ssm.device != cache.conv.device:
             raise ValueError(f"MambaBlock.serve: d_state must be {D_STATE} and the cache one of this block, got d_state "
-                             f"{n} and states {tuple(cache.ssm.shape)}")
+                             f"{n} and states {tuple(ssm.shape)}")
+        if ssm.dtype != torch.float32 or not ssm.is_contiguous() or ssm.data_ptr() % 16:
+            raise ValueError("MambaBlock.serve: the cache's states must be fp32, contiguous and 16-byte aligned, got "
+                             f"{ssm.dtype}, strides {ssm.stride()}")
+        if r > DT_RANK_MAX or x.shape[0] > DT_ROWS_MAX:
+            raise ValueError(f"MambaBlock.serve: dt_rank {r} (at most {DT_RANK_MAX}), {x.shape[0]} rows (at most "
+                             f"{DT_ROWS_MAX})")
         if out_adapters is not None:
             if not isinstance(out_adapters, LoraAdapters):
                 raise TypeError(f"MambaBlock.serve: out_adapters must be LoraAdapters, got {type(out_adapters).__name__}")

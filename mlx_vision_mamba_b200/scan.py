@@ -27,6 +27,10 @@ from . import _native
 from .direction import ScanDirection
 
 D_STATE = 16
+# dt_softplus_cuda (csrc/vmscan_dt.cuh): ranks whose weights a thread holds, and
+# 64 rows a CTA in the second grid dimension
+DT_RANK_MAX = 64
+DT_ROWS_MAX = 65535 * 64
 
 
 def _stream(t: torch.Tensor) -> ctypes.c_void_p:

@@ -12,6 +12,7 @@ import torch
 
 from mlx_vision_mamba_b200 import (
     LoraAdapters,
+    MambaBlock,
     RequestBatch,
     _native,
     build,
@@ -320,3 +321,25 @@ def test_overlapped_kernels_read_carries_through_plain_pointers():
             assert qualified <= {"chains", "pieces", "A"}, (name, qualified)
             checked.append(name)
     assert checked == ["cached_scan_kernel", "cached_chain_kernel"]
+
+
+def test_serve_refuses_what_a_later_step_would():
+    """Before anything else runs, so that the conv windows cannot move on alone
+    (on the host the first operator would raise RuntimeError)."""
+    block, batch, x = MambaBlock(d_model=32), RequestBatch([3, 1], device="cpu"), torch.zeros(4, 32)
+    good = block.new_cache(2).ssm
+    with pytest.raises(RuntimeError, match="CUDA"):
+        block.serve(x, block.new_cache(2), batch)
+    shifted = torch.zeros(good.numel() + 1)[1:].view(good.shape)
+    assert shifted.data_ptr() % 16 != 0 and shifted.is_contiguous()
+    for ssm in (good.to(torch.bfloat16), good.double(), good.transpose(1, 2).contiguous().transpose(1, 2),
+                torch.zeros(2, 64, 32)[:, :, ::2], good[:1].expand(2, -1, -1), shifted, good[:1]):
+        cache = block.new_cache(2)
+        cache.ssm = ssm
+        with pytest.raises(ValueError, match="MambaBlock.serve"):
+            block.serve(x, cache, batch)
+    wide = MambaBlock(d_model=1040)  # dt_rank 65
+    with pytest.raises(ValueError, match="dt_rank"):
+        wide.serve(torch.zeros(4, 1040), wide.new_cache(2), batch)
+    with pytest.raises(ValueError, match="rows"):
+        block.serve(torch.zeros(1, 32).expand(65535 * 64 + 1, 32), block.new_cache(2), batch)
