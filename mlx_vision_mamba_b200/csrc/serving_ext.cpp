@@ -8,7 +8,7 @@
 //
 // Exceptions are the Python ones: TypeError, ValueError, RuntimeError.
 #include <ATen/ATen.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -85,10 +85,16 @@ void shaped(const char* where, const char* name, const at::Tensor& t, int64_t ro
         shape_of(t));
 }
 
+// Refuses inputs whose derivatives a caller asks for: reverse mode (off under
+// no_grad) and forward mode (dual tensors; not off there).
 void no_grad(const char* where, std::initializer_list<const at::Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : ts)
-    RUNTIME(t == nullptr || !t->requires_grad(), "a serving operator has no gradient; call it under torch.no_grad()");
+  const c10::AutogradState& on = c10::AutogradState::get_tls_state();
+  for (const at::Tensor* t : ts) {
+    if (t == nullptr) continue;
+    RUNTIME(!on.get_grad_mode() || !t->requires_grad(),
+            "a serving operator has no gradient; call it under torch.no_grad()");
+    RUNTIME(!on.get_fw_grad_mode() || !t->_fw_grad(0).defined(), "a serving operator has no forward-mode derivative");
+  }
 }
 
 struct Batch {

@@ -646,3 +646,37 @@ def test_block_serves_adapters():
         # a block whose gains are of order one
         assert (y[at:at + l] - want).abs().max() <= 2e-5 * want.abs().max()
         at += l
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor's tangent is not dropped in silence, and nothing is
+    written; with forward mode off, as in inference mode, the call runs."""
+    import torch.autograd.forward_ad as fwd
+
+    inp = _scan_inputs(4, 32, 2, seed=5)
+    batch = RequestBatch([3, 1], adapters=[0, 1])
+    base, x, ads = _lora_inputs(batch, 2, 24, 16, 4, F32)
+    w, b, win = torch.randn(32, 4, 1, device="cuda"), torch.randn(32, device="cuda"), torch.randn(2, 3, 32, device="cuda")
+    state, window = inp["state"].clone(), win.clone()
+    block = MambaBlock(d_model=16).cuda()
+    cache = block.new_cache(2)
+    with torch.no_grad(), fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for name in ("x", "delta", "A", "B", "C", "D", "z", "state"):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                selective_scan_cached_cuda(batch=batch, **dict(inp, **{name: dual(inp[name])}))
+        for args in ((dual(inp["x"]), w, b, win), (inp["x"], dual(w), b, win), (inp["x"], w, dual(b), win),
+                     (inp["x"], w, b, dual(win))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                conv1d_silu_cached_cuda(*args, batch)
+        for args in ((dual(base), x), (base, dual(x))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                lora_add_cuda(*args, ads, batch)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            lora_add_cuda(base, x, ads, batch, out=dual(torch.empty_like(base)))
+        with pytest.raises(RuntimeError):
+            block.serve(dual(torch.randn(4, 16, device="cuda")), cache, batch)
+        assert torch.equal(inp["state"], state) and torch.equal(win, window) and not cache.conv.any()
+        selective_scan_cached_cuda(batch=batch, **inp)
+        with torch.inference_mode():
+            lora_add_cuda(base, x, ads, batch)
