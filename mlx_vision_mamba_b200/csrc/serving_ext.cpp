@@ -97,6 +97,12 @@ void no_grad(const char* where, std::initializer_list<const at::Tensor*> ts) {
   }
 }
 
+// Notes for autograd that a kernel has written t: a graph that has saved it
+// must not use the new values.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct Batch {
   PyObject* self;
   int64_t tokens, index;
@@ -232,6 +238,7 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                              static_cast<float*>(state.data_ptr()), state.size(0), i32(t.ptr), i32(t.ptr) + t.info[0],
                              stream),
           where, "vmscan_cached_step");
+    written(state);
     return THPVariable_Wrap(y);
   }
   const Table t = table_of(b, g_names.scan, stream, 2 * dn + bf16, state.size(0));
@@ -250,6 +257,7 @@ PyObject* scan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                            chains > 0 ? i32(t.ptr) + 8 * n : nullptr, chains, carry_rows, t.info[4], int(t.info[5]),
                            ws.defined() ? ws.data_ptr() : nullptr, size_t(ws_bytes), stream),
         where, "vmscan_cached_scan");
+  written(state);
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -282,6 +290,7 @@ PyObject* conv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                   static_cast<const float*>(w_.data_ptr()), static_cast<const float*>(b_.data_ptr()),
                                   out.data_ptr(), c, state.data_ptr(), state.size(0), i32(t.ptr), t.info[0], stream),
         where, "vmscan_cached_conv1d_silu");
+  written(state);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -366,6 +375,7 @@ PyObject* lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                           a.stride(1), bb.data_ptr(), static_cast<const float*>(scale.data_ptr()), base_.data_ptr(), base_.stride(0),
                           out.data_ptr(), out.stride(0), i32(t.ptr) + 4 * tiles, b.tokens, i32(t.ptr), tiles, stream),
           where, "vmscan_lora_add");
+    if (given != nullptr) written(out);
   }
   if (given != nullptr) {
     Py_INCREF(args[4]);

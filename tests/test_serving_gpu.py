@@ -680,3 +680,78 @@ def test_forward_mode_tangents_are_refused():
         selective_scan_cached_cuda(batch=batch, **inp)
         with torch.inference_mode():
             lora_add_cuda(base, x, ads, batch)
+
+
+def test_updates_in_place_are_seen_by_autograd():
+    """State, window and `out` count as modified in place: a backward pass that
+    has saved one of them refuses to use the new values."""
+    inp = _scan_inputs(4, 32, 2, seed=6)
+    prompts, tokens = RequestBatch([3, 1], adapters=[0, 1]), RequestBatch([1, 1], slots=[1, 0])
+    base, x, ads = _lora_inputs(prompts, 2, 24, 16, 4, F32)
+    w, b, win = torch.randn(32, 4, 1, device="cuda"), torch.randn(32, device="cuda"), torch.randn(2, 3, 32, device="cuda")
+    two = {k: (v[:2] if k in "x delta B C z".split() else v) for k, v in inp.items()}
+
+    def saved(values, call):
+        leaf = values.clone().requires_grad_(True)
+        kept = leaf * 2
+        loss = (kept * kept).sum()  # saves `kept`
+        with torch.no_grad():
+            call(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+    saved(inp["state"], lambda s: selective_scan_cached_cuda(batch=prompts, **dict(inp, state=s)))
+    saved(inp["state"], lambda s: selective_scan_cached_cuda(batch=tokens, **dict(two, state=s)))
+    saved(win, lambda s: conv1d_silu_cached_cuda(inp["x"], w, b, s, prompts))
+    saved(base, lambda s: lora_add_cuda(s, x, ads, prompts, out=s))
+    saved(base, lambda s: lora_add_cuda(base, x, ads, prompts, out=s))
+    kept = x.clone().requires_grad_(True) * 2  # what is only read stays usable
+    loss = (kept * kept).sum()
+    with torch.no_grad():
+        lora_add_cuda(base, kept, ads, prompts)
+    loss.backward()
+    with torch.inference_mode():  # inference tensors have no version to count
+        state, window = inp["state"].clone(), win.clone()
+        selective_scan_cached_cuda(batch=prompts, **dict(inp, state=state))
+        conv1d_silu_cached_cuda(inp["x"], w, b, window, prompts)
+        lora_add_cuda(base, x, ads, prompts, out=torch.empty_like(base))
+
+
+def test_inference_mode():
+    """First calls inside inference mode, updates outside it and inside, also of
+    captured graphs."""
+    count, dn = 4, 48
+    inp = _scan_inputs(count, dn, 2 * count, seed=14)
+    base, xl, ads = _lora_inputs(RequestBatch([1] * count, adapters=[0] * count), 2, 24, 40, 4, F32, seed=3)
+    w, b, win = torch.randn(dn, 4, 1, device="cuda"), torch.randn(dn, device="cuda"), torch.randn(2 * count, 3, dn, device="cuda")
+    batch = RequestBatch([1] * count, adapters=[0, 1, 0, 1])
+
+    def step(state, window):
+        return (conv1d_silu_cached_cuda(inp["x"], w, b, window, batch),
+                selective_scan_cached_cuda(batch=batch, **dict(inp, state=state)), lora_add_cuda(base, xl, ads, batch))
+
+    with torch.inference_mode():
+        step(inp["state"].clone(), win.clone())
+        state, window = inp["state"].clone(), win.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step(state, window)
+    for inside, kw in ((False, dict(slots=[4, 5, 6, 7], sources=[0, 1, 2, 3])), (True, dict(slots=[3, 2, 1, 0])),
+                       (False, dict(adapters=[1, 1, -1, 0]))):
+        with torch.inference_mode(inside):
+            batch.update(**kw)
+        with torch.inference_mode():
+            state.copy_(inp["state"])
+            window.copy_(win)
+            graph.replay()
+            s, v = inp["state"].clone(), win.clone()
+            eager = step(s, v)
+        for p, q in zip(eager + (s, v), captured + (state, window)):
+            assert torch.equal(p, q)
+        want = ref.scan(batch=batch, **inp)
+        ref.check("y", captured[1], want[0], want[1])
+        ref.check("state", state, want[2], want[3])
+        want = ref.conv(inp["x"], w, b, win, batch)
+        ref.check("conv", captured[0], want[0], want[1])
+        want = ref.lora(base, xl, ads, batch)
+        ref.check("lora", captured[2], want[0], want[1])
