@@ -26,6 +26,7 @@ There is no CPU path: inputs must be CUDA tensors and libvmscan.so must load.
 
 from __future__ import annotations
 
+import threading
 from typing import Optional, Sequence
 
 import numpy as np
@@ -36,6 +37,9 @@ from .scan import D_STATE
 
 _DTYPES = (torch.float32, torch.bfloat16)
 _MAX_ROWS = 1 << 30
+# Held while a batch's tables are made, taken for a graph or rewritten, so that
+# threads agree on them (not by calls that find theirs).
+_TABLES = threading.Lock()
 
 
 def _int_list(name: str, values, count: Optional[int] = None) -> np.ndarray:
@@ -155,6 +159,10 @@ class RequestBatch:
         cannot be rewritten."""
         if _capturing():
             raise RuntimeError("RequestBatch.update: not while a CUDA graph is being captured")
+        with _TABLES:
+            self._update(slots, sources, adapters)
+
+    def _update(self, slots, sources, adapters) -> None:
         names = ("slots", "sources", "adapters", "_adapters_given", "max_slot", "max_adapter")
         before = {n: getattr(self, n) for n in names}
         if slots is None:
@@ -227,20 +235,28 @@ class RequestBatch:
         stream; called by the operators (slots: of the cache they are given)."""
         key = (kind, arg, stream)
         table = self._tables.get(key)
-        if capturing:
-            # any stream's table will do: capture starts after a device-wide
-            # synchronisation, so its upload has completed
-            if table is None:
-                table = next((t for k, t in self._tables.items() if k[:2] == key[:2]), None)
-            if table is None:
-                raise RuntimeError("RequestBatch: call the operator once with this batch before capturing it")
-            table.captured = True
-            if kind != "lora":
-                table.limit = slots if table.limit is None else min(slots, table.limit)
-        elif table is None:
+        if table is None or capturing:
+            with _TABLES:
+                table = self._table_for_graph(key, slots) if capturing else self._new_table(key)
+        return table.told
+
+    def _new_table(self, key):
+        table = self._tables.get(key)  # another thread's, made meanwhile
+        if table is None:
             host, info = self._build(key)
             self._tables[key] = table = _Table(host, info, self.device)
-        return table.told
+        return table
+
+    def _table_for_graph(self, key, slots: int):
+        # any stream's table will do: capture starts after a device-wide
+        # synchronisation, so its upload has completed
+        table = self._tables.get(key) or next((t for k, t in self._tables.items() if k[:2] == key[:2]), None)
+        if table is None:
+            raise RuntimeError("RequestBatch: call the operator once with this batch before capturing it")
+        table.captured = True
+        if key[0] != "lora":
+            table.limit = slots if table.limit is None else min(slots, table.limit)
+        return table
 
 
 def _check_count(n: int, where: str) -> int:

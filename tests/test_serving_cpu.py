@@ -5,6 +5,8 @@ rows, slots and adapters they work on."""
 import contextlib
 import os
 import re
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -343,3 +345,45 @@ def test_serve_refuses_what_a_later_step_would():
         wide.serve(torch.zeros(4, 1040), wide.new_cache(2), batch)
     with pytest.raises(ValueError, match="rows"):
         block.serve(torch.zeros(1, 32).expand(65535 * 64 + 1, 32), block.new_cache(2), batch)
+
+
+def test_threads_share_one_table(host_streams, monkeypatch):
+    """Two threads that need the same table get one, whose address a graph may
+    hold from then on."""
+    batch = RequestBatch([1, 1], device="cpu")
+    build_table, built = RequestBatch._build, []
+
+    def slow(self, key):
+        built.append(key)
+        time.sleep(0.3)
+        return build_table(self, key)
+
+    monkeypatch.setattr(RequestBatch, "_build", slow)
+    told = []
+    threads = [threading.Thread(target=lambda: told.append(batch._table("step", 1, 0, False, 9))) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert built == [("step", 0, 1)] and told[0] == told[1] == batch._tables[("step", 0, 1)].told
+
+
+def test_an_update_reaches_a_table_that_another_thread_is_making(host_streams, monkeypatch):
+    batch = RequestBatch([1, 1], device="cpu")
+    build_table, built, updated = RequestBatch._build, threading.Event(), threading.Event()
+
+    def slow(self, key):
+        table = build_table(self, key)
+        if not built.is_set():
+            built.set()
+            updated.wait(0.5)  # an update that does not wait for this table is over by then
+        return table
+
+    monkeypatch.setattr(RequestBatch, "_build", slow)
+    maker = threading.Thread(target=lambda: batch._table("step", 1, 0, False, 9))
+    maker.start()
+    assert built.wait(10)
+    batch.update(slots=[6, 7])
+    updated.set()
+    maker.join()
+    assert batch._tables[("step", 0, 1)].tensor.tolist() == [6, 7, 6, 7]
