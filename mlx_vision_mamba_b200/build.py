@@ -79,11 +79,22 @@ def _build_library(verbose: bool, extra_flags) -> None:
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
 
 
+def _ext_tag() -> str:
+    """What the extension is tied to besides its sources: the installed PyTorch
+    and the interpreter.  It is compiled in (serving_ext.cpp: kBuiltFor)."""
+    import torch
+
+    return f"serving_ext built for torch {torch.__version__} python {sys.version_info[0]}.{sys.version_info[1]};"
+
+
 def _ext_stale() -> bool:
     if not os.path.exists(EXT_PATH):
         return True
     header = os.path.join(os.path.dirname(PKG_DIR), "include", "vmscan.h")
-    return any(os.path.getmtime(p) > os.path.getmtime(EXT_PATH) for p in (EXT_SOURCE, header))
+    if any(os.path.getmtime(p) > os.path.getmtime(EXT_PATH) for p in (EXT_SOURCE, header)):
+        return True
+    with open(EXT_PATH, "rb") as f:
+        return _ext_tag().encode() not in f.read()
 
 
 def _build_ext() -> None:
@@ -94,7 +105,8 @@ def _build_ext() -> None:
 
     cuda_home = os.path.dirname(os.path.dirname(nvcc_path()))
     lib_dirs = [*cpp_extension.library_paths(), PKG_DIR]
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DVMSCAN_BUILT_FOR="{_ext_tag()}"']
     for inc in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda_home, "include")):
         cmd += ["-isystem", inc]
     cmd += ["-o", EXT_PATH + ".tmp", EXT_SOURCE]

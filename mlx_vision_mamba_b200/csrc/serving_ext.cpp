@@ -404,6 +404,10 @@ PyMethodDef g_methods[] = {
     {"lora", reinterpret_cast<PyCFunction>(lora), METH_FASTCALL, "serving.lora_add_cuda"},
     {nullptr, nullptr, 0, nullptr}};
 
+// The PyTorch and the interpreter that this was compiled for: build.py looks for
+// it and compiles anew for others.
+const char kBuiltFor[] = VMSCAN_BUILT_FOR;
+
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_serving_ext", "Calls of the serving operators.", -1, g_methods};
 
 }  // namespace
@@ -421,5 +425,10 @@ PyMODINIT_FUNC PyInit__serving_ext(void) {
                      {&g_names.conv, "conv"},             {&g_names.lora, "lora"}};
   for (const auto& n : names)
     if ((*n.at = PyUnicode_InternFromString(n.name)) == nullptr) return nullptr;
-  return PyModule_Create(&g_module);
+  PyObject* m = PyModule_Create(&g_module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", kBuiltFor) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
 }

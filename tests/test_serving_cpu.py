@@ -387,3 +387,13 @@ def test_an_update_reaches_a_table_that_another_thread_is_making(host_streams, m
     updated.set()
     maker.join()
     assert batch._tables[("step", 0, 1)].tensor.tolist() == [6, 7, 6, 7]
+
+
+def test_the_extension_is_built_anew_for_another_pytorch(monkeypatch):
+    from mlx_vision_mamba_b200 import _serving_ext
+
+    monkeypatch.setattr(os.path, "getmtime", lambda path: 0.0)  # the sources' times are another matter
+    assert not build._ext_stale()
+    assert _serving_ext.built_for == build._ext_tag()
+    monkeypatch.setattr(torch, "__version__", "99.1")
+    assert build._ext_stale()
