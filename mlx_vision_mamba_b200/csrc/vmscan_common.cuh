@@ -337,12 +337,15 @@ __device__ __forceinline__ void two_sum1(float& acc, float& x) {
 // rounded to 11 significant bits (to nearest, ties away from zero: add half a
 // TF32 unit to the magnitude bits, clear the 13 low bits), lo = (x - hi)
 // rounded the same way (x - hi is exact).  Integer ALU only, so producers can
-// emit the parts beside their fp32 output without loading the exp unit.
+// emit the parts beside their fp32 output without loading the exp unit.  The
+// integer rounding of a NaN may carry over to zero (the hardware's own NaN has
+// all mantissa bits set) or end in an infinity, so hi of a NaN is a NaN within
+// TF32's bits.
 __device__ __forceinline__ float tf32_round(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u);
 }
 __device__ __forceinline__ void split_tf32(float x, float& hi, float& lo) {
-  hi = tf32_round(x);
+  hi = x == x ? tf32_round(x) : __uint_as_float(0x7FFFE000u);
   lo = tf32_round(x - hi);
 }
 __device__ __forceinline__ void split_tf32_4(const float4& x, float4& hi, float4& lo) {

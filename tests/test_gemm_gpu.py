@@ -305,3 +305,67 @@ def test_tf32_split_many_matches_split():
     xs20 = [torch.randn(8 * (i + 1), generator=gen).cuda() for i in range(20)]  # more than one launch's 16
     for x, (h, l) in zip(xs20, tf32_split_many(xs20)):
         assert torch.equal(h, tf32_split(x)[0]) and torch.equal(l, tf32_split(x)[1])
+
+
+NAN_PATTERNS = (0x7FC00000, 0x7FFFFFFF, 0x7F800001, 0x7FFFF000, -1, -0x400000)  # quiet, the hardware's, signalling, negative
+
+
+def test_nan_reaches_the_products():
+    """A NaN of any bit pattern in an operand makes its row (x) or column (weight)
+    NaN, forward and backward, and changes nothing else."""
+    from mlx_vision_mamba_b200.linear import linear_tc
+
+    gen = torch.Generator().manual_seed(11)
+    dev = torch.device("cuda", 0)
+    nans = torch.tensor(NAN_PATTERNS, dtype=torch.int32, device=dev).view(torch.float32)
+    t, fin, fout = 300, 64, 96
+    x, w, dy = (torch.randn(s, generator=gen).to(dev) for s in ((t, fin), (fout, fin), (t, fout)))
+
+    def run(x, w, dy):
+        x, w = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = linear_tc(x, w)
+        y.backward(dy)
+        return y.detach(), x.grad, w.grad
+
+    y0, dx0, dw0 = run(x, w, dy)
+    for i, nan in enumerate(nans):
+        r, c, o = 37 * i + 5, 9 * i + 3, 14 * i + 1
+        rows, cols, outs = (torch.arange(n, device=dev) != k for n, k in ((t, r), (fin, c), (fout, o)))
+        bad = x.clone()
+        bad[r, c] = nan
+        y, dx, dw = run(bad, w, dy)
+        assert torch.isnan(y[r]).all() and torch.equal(y[rows], y0[rows]), i
+        assert torch.isnan(dw[:, c]).all() and torch.equal(dw[:, cols], dw0[:, cols]) and torch.equal(dx, dx0), i
+        bad = w.clone()
+        bad[o, c] = nan
+        y, dx, dw = run(x, bad, dy)
+        assert torch.isnan(y[:, o]).all() and torch.equal(y[:, outs], y0[:, outs]), i
+        assert torch.isnan(dx[:, c]).all() and torch.equal(dx[:, cols], dx0[:, cols]) and torch.equal(dw, dw0), i
+        bad = dy.clone()
+        bad[r, o] = nan
+        y, dx, dw = run(x, w, bad)
+        assert torch.isnan(dx[r]).all() and torch.equal(dx[rows], dx0[rows]), i
+        assert torch.isnan(dw[o]).all() and torch.equal(dw[outs], dw0[outs]) and torch.equal(y, y0), i
+
+
+def test_nan_reaches_the_block_output():
+    """From its token on, a NaN in a block's input makes the output NaN (the conv
+    and the scan write the next products' operands as parts themselves); earlier
+    tokens keep their values."""
+    from mlx_vision_mamba_b200 import MambaBlock, RequestBatch
+
+    torch.manual_seed(4)
+    block = MambaBlock(d_model=64).cuda()
+    x = torch.randn(2, 50, 64, device="cuda")
+    clean = block(x)
+    for pattern in NAN_PATTERNS:
+        bad = x.clone()
+        bad[1, 20, 7] = torch.tensor([pattern], dtype=torch.int32, device="cuda").view(torch.float32)[0]
+        leaf = bad.requires_grad_(True)
+        y = block(leaf)
+        assert torch.isnan(y[1, 20:]).all() and torch.equal(y[0], clean[0]) and torch.equal(y[1, :20], clean[1, :20])
+        grad, = torch.autograd.grad(y[1, 20].sum(), leaf)
+        assert torch.isnan(grad[1, 20]).all()
+        with torch.no_grad():
+            served = block.serve(bad.detach()[1], block.new_cache(1), RequestBatch([50], sources=[-1]))
+        assert torch.isnan(served[20:]).all() and torch.isfinite(served[:20]).all()
