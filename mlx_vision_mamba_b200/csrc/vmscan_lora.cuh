@@ -17,13 +17,21 @@
 // so a lane's four (fp32) or eight (bf16) adjacent elements stand for the
 // inner indices that its fragment registers hold, on both operands alike, and
 // every access is a 16-byte one.
-//   fp32: TF32 hi / lo parts, hi hi + hi lo + lo hi, fp32 accumulators.
+//   fp32: TF32 hi / lo parts, hi hi + hi lo + lo hi (lo lo is 2^-22 of a
+//         product at most).  The tensor pipe cuts off, towards zero, what lies
+//         below the last place of its accumulator, so that a chain of products
+//         in one accumulator drifts: 768 -> 1536, rank 64, was off by 1.2e-6
+//         of the norm (plain fp32 products: 3.7e-7).  A chain therefore covers
+//         16 inner indices, starts from zero, and is added to the sum in fp32,
+//         rounded to nearest: 1.7e-7, whatever the lengths, for 1 to 4 % of
+//         the time.
 //   bf16: x, A, B are exact operands; S enters the second product as three
-//         bf16 parts (24 bits).  The output is rounded once.
+//         bf16 parts (24 bits).  The output is rounded once, to 2^-9 of its
+//         norm, far above what the chains lose (3e-6).
 //
-// Measured on B200: 16384 rows 384 -> 1536, rank 16, fp32 50 us, 4.6 TB/s of
+// Measured on B200: 16384 rows 384 -> 1536, rank 16, fp32 51 us, 4.4 TB/s of
 // the 227 MB that have to move (the floor is 35 us; 14 warps an SM wait for
-// base and B); 768 -> 1536, rank 64, bf16 67 us and fp32 131 us (three TF32
+// base and B); 768 -> 1536, rank 64, bf16 67 us and fp32 128 us (three TF32
 // products a term: the tensor pipe alone takes about 50); 64 rows of 32
 // adapters 384 -> 1536, rank 16: 6.3 us (latency: row list, x and A, S, B).
 // Rings of asynchronous copies for x, base and B cost more occupancy than they
@@ -187,6 +195,14 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
                                           float* part, uint32_t* frag) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   constexpr int CN = Chunk<T>::N;
+  // The products with a lo part, 2^-11 of the others, may stay in accumulators
+  // of their own for the whole of d_in, which shortens the chains that a short
+  // call waits for: 1 x 768 -> 768, rank 8, 5.5 us (6.6 in the one chain), 64
+  // rows of 32 adapters, 384 -> 1536, rank 16, 6.3 (6.7).  More columns of S or
+  // unaligned rows leave no registers for them (16384 rows 768 -> 1536, rank 64:
+  // 180 us for 128).  By variant and not by the tile's rows, so that a row's
+  // result does not depend on the rows beside it.
+  constexpr bool APART = sizeof(T) == 4 && WIDE && STEPS == 1;
   constexpr int NT = STEPS == 1 ? 2 : LORA_RCHUNK / 8;  // 8-column blocks of S a warp holds
   int r[2 * MT];  // rows g, g + 8, ... of the tile; those past the last repeat it
 #pragma unroll
@@ -200,11 +216,12 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
     const float scale = a.scale[ad];
     for (int rc = 0; rc < a.rank; rc += LORA_RCHUNK) {
       float acc[MT][NT][4] = {};
+      float small[APART ? MT : 1][APART ? NT : 1][4] = {};
       const int nt = min(NT, (a.rank - rc + 7) / 8);
       const T* ar[NT];  // row of A whose products this lane's B fragments hold
 #pragma unroll
       for (int j = 0; j < NT; ++j) ar[j] = A + int64_t(min(rc + 8 * j + g, a.rank - 1)) * a.lda;
-#pragma unroll 2
+#pragma unroll (APART && MT == 2 ? 1 : 2)  // (16384 rows, rank 16: 51.4 us, 52.3 with two chunks)
       for (int c = (warp * 4 + t) * CN; c - t * CN < a.d_in; c += LORA_WARPS * 4 * CN) {
         Chunk<T> x[2 * MT], ab[NT];
 #pragma unroll
@@ -226,6 +243,7 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
         for (int j = 0; j < NT; ++j) {
           if (j < nt) {
             const Chunk<T>& b = ab[j];
+            float sum[MT][4] = {};  // fp32: the chain of this chunk
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // words 2h and 2h + 1 of the chunk are one step of the product
               uint32_t bh[2] = {b.w[2 * h], b.w[2 * h + 1]}, bl[2];
@@ -244,16 +262,30 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
                 if constexpr (sizeof(T) == 4) {
                   const uint32_t la[4] = {xl[2 * m][2 * h], xl[2 * m + 1][2 * h], xl[2 * m][2 * h + 1],
                                           xl[2 * m + 1][2 * h + 1]};
-                  mma_tf32(acc[m][j], la, bh[0], bh[1]);
-                  mma_tf32(acc[m][j], xa, bl[0], bl[1]);
-                  mma_tf32(acc[m][j], xa, bh[0], bh[1]);
+                  mma_tf32(APART ? small[m][j] : sum[m], la, bh[0], bh[1]);
+                  mma_tf32(APART ? small[m][j] : sum[m], xa, bl[0], bl[1]);
+                  mma_tf32(sum[m], xa, bh[0], bh[1]);
                 } else {
                   mma_bf16(acc[m][j], xa, bh[0], bh[1]);
                 }
               }
             }
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[m][j][q] += sum[m][q];
+            }
           }
         }
+      }
+      if constexpr (APART) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[m][j][q] += small[m][j][q];
       }
       // partial products of the warps, then their sum in a fixed order as the
       // fragments of the second product
@@ -364,6 +396,7 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
     for (int m = 0; m < MT; ++m) {
       const uint4* f = reinterpret_cast<const uint4*>(frag) + size_t(m * steps + s) * LoraFrag<T>::GROUPS * 32 + lane;
       if constexpr (sizeof(T) == 4) {
+        float sum[2][4] = {};  // the chain of this step
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint4 fh = f[32 * h], fl = f[32 * (2 + h)];
@@ -371,11 +404,15 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t h0 = tf32_hi(b[j].w[2 * h]), h1 = tf32_hi(b[j].w[2 * h + 1]);
-            mma_tf32(acc[m][j], sl, h0, h1);
-            mma_tf32(acc[m][j], sh, tf32_lo(b[j].w[2 * h], h0), tf32_lo(b[j].w[2 * h + 1], h1));
-            mma_tf32(acc[m][j], sh, h0, h1);
+            mma_tf32(sum[j], sl, h0, h1);
+            mma_tf32(sum[j], sh, tf32_lo(b[j].w[2 * h], h0), tf32_lo(b[j].w[2 * h + 1], h1));
+            mma_tf32(sum[j], sh, h0, h1);
           }
         }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[m][j][q] = STEPS == 1 ? sum[j][q] : acc[m][j][q] + sum[j][q];
       } else {
 #pragma unroll
         for (int w = 2; w >= 0; --w) {

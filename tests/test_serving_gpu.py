@@ -755,3 +755,34 @@ def test_inference_mode():
         ref.check("conv", captured[0], want[0], want[1])
         want = ref.lora(base, xl, ads, batch)
         ref.check("lora", captured[2], want[0], want[1])
+
+
+@pytest.mark.parametrize("rank", [8, 24, 64, 100])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("d_in,d_out", [(4096, 512), (4095, 510)])
+def test_lora_products_do_not_drift(d_in, d_out, rows, rank):
+    """Positive factors, so that what each product of 8 inner indices cuts off
+    below its accumulator's last place (2 EPS of the sum so far at most, always
+    towards zero) adds up.  A chain of two such products loses at most 4 EPS of
+    its own sum in each of the two products, whatever d_in and the rank are;
+    roundings to nearest average out (1 EPS for what is left of them)."""
+    g = _gen(rank)
+    u = lambda *s: 0.5 + torch.rand(s, generator=g, device="cuda")  # noqa: E731
+    ads = LoraAdapters(u(1, rank, d_in), u(1, d_out, rank))
+    x, zero = u(rows, d_in), torch.zeros(rows, d_out, device="cuda")
+    y = lora_add_cuda(zero, x, ads, RequestBatch([rows], adapters=[0])).double()
+    exact = (x.double() @ ads.a[0].double().t()) @ ads.b[0].double().t()
+    drift = ((y - exact) / exact).mean().item()
+    assert abs(drift) <= 9 * ref.EPS, drift / ref.EPS
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rank", [8, 24, 64, 100])
+@pytest.mark.parametrize("d_in,d_out", [(384, 520), (130, 257)])
+def test_lora_rows_do_not_depend_on_the_rows_beside_them(d_in, d_out, rank, dtype):
+    batch = RequestBatch([40, 1, 17, 3], adapters=[0, 0, 1, 1])
+    base, x, ads = _lora_inputs(batch, 2, d_in, d_out, rank, dtype, seed=rank)
+    y = lora_add_cuda(base, x, ads, batch)
+    for row, k in ((0, 0), (39, 0), (40, 0), (57, 1), (60, 1)):
+        alone = lora_add_cuda(base[row:row + 1], x[row:row + 1], ads, RequestBatch([1], adapters=[k]))
+        assert torch.equal(alone[0], y[row]), row
