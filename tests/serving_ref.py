@@ -76,6 +76,40 @@ def scan(x, delta, A, B, C, D, state, batch, z=None):
     return y, 1.05 * tol + y.abs() * HALF_STEP[dtype], new, 1.05 * state_tol
 
 
+def scan_together(x, delta, A, B, C, D, state, batch, z=None):
+    """`scan`, a step of all requests at a time (for many rows)."""
+    f = lambda t: t.detach().double()  # noqa: E731
+    dtype = x.dtype
+    x, delta, A, B, C, D, old = f(x), f(delta), f(A), f(B), f(C), f(D), f(state)
+    y, tol, new, state_tol = torch.zeros_like(x), torch.zeros_like(x), old.clone(), torch.zeros_like(old)
+    lengths, begins = batch.lengths.tolist(), _begins(batch.lengths.tolist())
+    order = sorted((i for i in range(batch.count) if batch.slots[i] >= 0), key=lambda i: -lengths[i])
+    source, slot = batch.sources[order].tolist(), batch.slots[order].tolist()
+    h = torch.stack([old[s] if s >= 0 else torch.zeros_like(old[0]) for s in source])
+    H, E = h.abs(), torch.zeros_like(h)
+    long = torch.tensor([float(lengths[i]) for i in order], device=x.device)[:, None, None]
+    at = torch.tensor([begins[i] for i in order], device=x.device)
+    on = len(order)
+    for t in range(max(lengths)):
+        while lengths[order[on - 1]] <= t:
+            on -= 1
+        r = at[:on] + t
+        arg = delta[r][:, :, None] * A
+        a, b = torch.exp(arg), (delta[r] * x[r])[:, :, None] * B[r][:, None, :]
+        e = a * (E[:on] + (5 + (3 + long[:on]) * arg.abs()) * EPS * H[:on]) + TINY * (1 + H[:on])
+        h[:on], H[:on] = a * h[:on] + b, a * H[:on] + b.abs()
+        E[:on] = e + (2 * b.abs() + H[:on]) * EPS
+        c = C[r][:, :, None]
+        y[r] = (h[:on] @ c)[:, :, 0] + x[r] * D
+        tol[r] = (E[:on] @ c.abs())[:, :, 0] + 18 * EPS * ((H[:on] @ c.abs())[:, :, 0] + (x[r] * D).abs()) + TINY
+    if z is not None:
+        g = _silu(f(z))
+        tol = tol * g.abs() + (y * g).abs() * (10 + 3 * f(z).abs()) * EPS
+        y = y * g
+    new[slot], state_tol[slot] = h, E
+    return y, 1.05 * tol + y.abs() * HALF_STEP[dtype], new, 1.05 * state_tol
+
+
 def conv(x, weight, bias, state, batch):
     f = lambda t: t.detach().double()  # noqa: E731
     dtype = x.dtype

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import serving_ref as ref
+from mlx_vision_mamba_b200 import _native
 from mlx_vision_mamba_b200 import (
     LoraAdapters,
     MambaBlock,
@@ -786,3 +787,91 @@ def test_lora_rows_do_not_depend_on_the_rows_beside_them(d_in, d_out, rank, dtyp
     for row, k in ((0, 0), (39, 0), (40, 0), (57, 1), (60, 1)):
         alone = lora_add_cuda(base[row:row + 1], x[row:row + 1], ads, RequestBatch([1], adapters=[k]))
         assert torch.equal(alone[0], y[row]), row
+
+
+SPLIT = {"few": [400] * 5 + [1] * 12, "three": [700] * 3 + [40] * 20, "ragged": [1 + i * i * 37 % 900 if i % 3 == 0 else 1 for i in range(40)],
+         "long": [1200, 100, 0, 50, 600, 300]}
+
+
+# the launches of a split scan: overlapped or not, chained by a kernel (more than 8 pieces) or by the pieces, first
+# launch with the shared memory of three CTAs an SM or not (of 148 SMs)
+@pytest.mark.parametrize("name,dn,dtype,overlapped,chained,claims", [
+    ("three", 768, F32, True, False, False),
+    ("long", 771, F32, True, True, False),
+    ("few", 768, BF16, False, False, False),
+    ("long", 768, F32, False, True, False),
+    ("ragged", 1536, F32, False, False, True),
+    ("ragged", 771, BF16, False, True, True),
+])
+def test_scan_splits_of_large_calls(name, dn, dtype, overlapped, chained, claims):
+    """Every way in which a split scan is launched, against the definition, and
+    captured: replayed with other rows and states, and after an update."""
+    lengths = SPLIT[name]
+    n, groups, sms = len(lengths), (dn + 127) // 128, torch.cuda.get_device_properties(0).multi_processor_count
+    batch = RequestBatch(lengths, slots=[2 * i + 1 for i in range(n)], sources=[2 * i if i % 4 else -1 for i in range(n)])
+    pieces, first, chains, _, most, uneven = batch._build(("scan", 2 * dn + (dtype == BF16)))[1]
+    if sms == 148:
+        assert chains > 0 and (pieces * groups <= 3 * sms, most > 8) == (overlapped, chained)
+        assert (bool(uneven) and first * groups > 3 * sms) == claims
+    inp = _scan_inputs(sum(lengths), dn, 2 * n, dtype, seed=n)
+    want = ref.scan_together(batch=batch, **inp)
+    run = dict(inp, state=inp["state"].clone())
+    y = selective_scan_cached_cuda(batch=batch, **run)
+    ref.check("y", y, want[0], want[1])
+    ref.check("state", run["state"], want[2], want[3])
+
+    graph, held = torch.cuda.CUDAGraph(), {k: v.clone() for k, v in inp.items()}
+    with torch.cuda.graph(graph):
+        captured = selective_scan_cached_cuda(batch=batch, **held)
+    for k in range(3):
+        if k == 2:
+            batch.update(slots=[2 * i for i in range(n)], sources=[2 * i + 1 if i % 3 else -1 for i in range(n)])
+        new = _scan_inputs(sum(lengths), dn, 2 * n, dtype, seed=n + k)
+        for t, v in new.items():
+            held[t].copy_(v)
+        graph.replay()
+        eager = dict(new, state=new["state"].clone())
+        assert torch.equal(selective_scan_cached_cuda(batch=batch, **eager), captured), k
+        assert torch.equal(eager["state"], held["state"]), k
+    want = ref.scan_together(batch=batch, **new)
+    ref.check("y after an update", captured, want[0], want[1])
+    ref.check("state after an update", held["state"], want[2], want[3])
+
+
+@pytest.mark.parametrize("c,k,dtype,rows", [(1536, 4, F32, 10000), (1536, 8, BF16, 10000), (771, 5, BF16, 5000), (1536, 1, F32, 9600)])
+def test_conv_of_large_calls(c, k, dtype, rows):
+    """Pieces of 32 rows, which only large calls have."""
+    lengths = [0, 31, 33, 1, 2, 500, 64, rows // 2]
+    lengths.append(rows - sum(lengths))
+    n = len(lengths)
+    assert _native.load().vmscan_cached_conv_rows(rows, c) == 32
+    g = _gen(c + k)
+    x = torch.randn(rows, c, generator=g, device="cuda").to(dtype)
+    w, b = torch.randn(c, k, 1, generator=g, device="cuda"), torch.randn(c, generator=g, device="cuda")
+    state = torch.randn(2 * n, k - 1, c, generator=g, device="cuda").to(dtype)
+    for batch in (_mixed(lengths), RequestBatch(lengths)):
+        want = ref.conv(x, w, b, state, batch)
+        new = state.clone()
+        ref.check("conv", conv1d_silu_cached_cuda(x, w, b, new, batch), want[0], want[1])
+        ref.check("window", new, want[2], torch.zeros_like(want[2]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rank", [16, 24, 64, 100])
+@pytest.mark.parametrize("rows,d_in,d_out", [(10000, 96, 520), (10000, 99, 515), (4800, 96, 520), (4800, 99, 515)])
+def test_lora_of_large_calls(rows, d_in, d_out, rank, dtype):
+    """Tiles enough that a warp goes over several column groups (all nine of a
+    tile in the larger call), beside base and in place."""
+    lengths = [rows // 2, 0, 77, rows // 4, 1]
+    lengths.append(rows - sum(lengths))
+    batch = RequestBatch(lengths, adapters=[0, 1, 1, 2, -1, 0])
+    base, x, ads = _lora_inputs(batch, 3, d_in, d_out, rank, dtype, seed=rank)
+    want = ref.lora(base, x, ads, batch)
+    y = lora_add_cuda(base, x, ads, batch)
+    ref.check("lora", y, want[0], want[1])
+    inside = base.clone()
+    lora_add_cuda(inside, x, ads, batch, out=inside)
+    assert torch.equal(inside, y)
+    wide = torch.zeros(rows, d_out + 8, device="cuda", dtype=dtype)[:, 4:4 + d_out]
+    lora_add_cuda(base, x, ads, batch, out=wide)
+    assert torch.equal(wide, y)
