@@ -127,9 +127,11 @@ __device__ __forceinline__ float4 ld_four(const T* p, bool wide) {
 // part of the decays by a polynomial on the FMA pipe (one of eight pairs:
 // within 3 %, two: +9 %), one channel and 16 states a lane (fp32 +3 to 5 %),
 // five CTAs an SM.
-// Whole calls: 32 prompts of 32768 rows x 1536, bf16: 357 us; one prompt of
-// 32768 x 768 fp32: 253 us (in 96 pieces; 4.3 ms in one); 24 requests, 9001
-// rows x 768, fp32: 75 us; 196 rows x 768: 11.6 us.
+// Whole calls: 32 prompts of 32768 rows x 1536, bf16: 358 us; one prompt of
+// 32768 x 768 fp32: 255 us (in 96 pieces; 4.3 ms in one); 24 requests, 9001
+// rows x 768, fp32: 75 us (1.8x rows from splitting, and single tokens are pieces
+// of this kernel); 196 rows x 768: 11.5 us (three dependent launches; pieces that
+// pass their states on inside a cluster, in one launch, are not built).
 // ---------------------------------------------------------------------------
 constexpr int CSC_WARPS = 4;
 constexpr int CSC_ROWS = 8;
@@ -499,7 +501,9 @@ __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const fl
 // states from HBM: 12.1 us, 4.7 TB/s (16.2 in scalar arithmetic, 390
 // instructions a warp instead of about 130; 13.4 with two rows a warp, whose
 // registers halve the warps an SM holds; 14.0 with ten CTAs an SM, which
-// spill); 1024 x 1536: 40 to 43 us, 5.3 to 5.7 TB/s; 1 x 768: 2.0 us.
+// spill); 1024 x 1536: 40 to 43 us, 5.3 to 5.7 TB/s; 333 x 768 bf16 8.2 us, fp32
+// 8.6, 333 x 771 8.4 to 9.0 (rows of scalars cost little beside the states);
+// 1 x 768: 2.0 us.
 // ---------------------------------------------------------------------------
 constexpr int CST_WARPS = 4;
 constexpr int CST_CTAS = 8;  // an SM is to hold
@@ -573,11 +577,11 @@ __global__ void __launch_bounds__(CST_WARPS * 32, CST_CTAS)
 // rows) reads the stored window, and writes the new one: the request's last
 // K - 1 rows, reaching back into the old window when it has fewer.  The same
 // thread reads the old window before it writes, so a slot may be both.
-// Bound: HBM, a read and a write of each element; with bf16 rows the
-// exponential unit is next (two of its operations an element, 22 us of the 46
-// below).  32768 x 1536, K = 4: fp32 70 us, 5.7 TB/s (148 with one row's loads
-// at a time), bf16 46 us; K = 8 fp32 111 us (the window of 7 rows before each
-// piece and 140 registers); 64 tokens x 768: 2.9 us.
+// Bound: HBM, a read and a write of each element.  32768 x 1536, K = 4: fp32
+// 70 us, 5.7 TB/s (148 with one row's loads at a time); bf16 46 us, more than
+// its bytes (31) or the exponential unit (22, two operations an element) take:
+// an access of four channels is 8 bytes there; K = 8 fp32 111 us (the window of 7
+// rows before each piece and 140 registers); 64 tokens x 768: 2.9 to 3.1 us.
 // ---------------------------------------------------------------------------
 constexpr int CCV_ROWS = 32;       // rows of a piece
 constexpr int CCV_FEW_ROWS = 16;   // where those would give the SMs too few threads (both at least K - 1)

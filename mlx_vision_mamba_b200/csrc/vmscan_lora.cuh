@@ -10,9 +10,11 @@
 // and then split the columns for out = base + S B^T.  Nothing but base, x and
 // out crosses HBM; the rank-wide S never leaves the SM.
 //
-// Both products run on mma.sync (a tile has a few rows of one adapter and a
-// rank of 4 to 64: far too little work per operand byte for tcgen05 to matter;
-// the kernel is bound by the bytes of base and out).  Operands go from global
+// Both products run on mma.sync: a tile has a few rows of one adapter, too
+// little work per operand byte for tcgen05 to matter at a rank of up to 16,
+// where the kernel is bound by the bytes of base and out.  That no longer holds
+// at a rank of 64 on many rows of one adapter (figures below), for which this is
+// not the best design.  Operands go from global
 // memory straight to fragments: the order of a product's inner index is free,
 // so a lane's four (fp32) or eight (bf16) adjacent elements stand for the
 // inner indices that its fragment registers hold, on both operands alike, and
@@ -23,17 +25,19 @@
 //         in one accumulator drifts: 768 -> 1536, rank 64, was off by 1.2e-6
 //         of the norm (plain fp32 products: 3.7e-7).  A chain therefore covers
 //         16 inner indices, starts from zero, and is added to the sum in fp32,
-//         rounded to nearest: 1.7e-7, whatever the lengths, for 1 to 4 % of
-//         the time.
+//         rounded to nearest: 1.7e-7, whatever the lengths, for 1 to 9 % of
+//         the time (9: rank 24 on unaligned rows).
 //   bf16: x, A, B are exact operands; S enters the second product as three
 //         bf16 parts (24 bits).  The output is rounded once, to 2^-9 of its
 //         norm, far above what the chains lose (3e-6).
 //
-// Measured on B200: 16384 rows 384 -> 1536, rank 16, fp32 51 us, 4.4 TB/s of
-// the 227 MB that have to move (the floor is 35 us; 14 warps an SM wait for
-// base and B); 768 -> 1536, rank 64, bf16 67 us and fp32 128 us (three TF32
-// products a term: the tensor pipe alone takes about 50); 64 rows of 32
-// adapters 384 -> 1536, rank 16: 6.3 us (latency: row list, x and A, S, B).
+// Measured on B200: 16384 rows of 16 uneven requests, 384 -> 1536, rank 16, fp32
+// 52 us, 4.4 TB/s of the 227 MB that have to move (the floor is 35 us; 14 warps
+// an SM wait for base and B); the same rows 768 -> 1536, rank 64, bf16 68 us and
+// fp32 139 us (128 with even requests; floors 20 and 39.  Three TF32 products a
+// term: the tensor pipe alone takes about 50; the rest is mostly A, B and their
+// parts, loaded and split again for each tile of 32 rows); 64 rows of 32
+// adapters 384 -> 1536, rank 16: 6.3 to 6.6 us (latency: row list, x and A, S, B).
 // Rings of asynchronous copies for x, base and B cost more occupancy than they
 // hid (62 to 74 us on the first case at the time, 53 without).
 #pragma once
@@ -162,8 +166,9 @@ __device__ __forceinline__ void st_quad(T* row, int c, int limit, const float4& 
 // mantissa is all ones (the one the hardware makes) over to zero; the rounding
 // of lo is the conversion instruction, which keeps the NaN that x - hi then is,
 // as it is for infinities, so that neither is lost (lo rounded the integer way
-// too lost them and took 6.1 instead of 6.3 us for 64 rows of 32 adapters, rank
-// 16, 106 instead of 108 us at rank 64; both parts by conversion 6.7 and 113).
+// too lost them and took 6.1 instead of 6.3 us for 64 rows of 32 adapters, 384 ->
+// 1536, rank 16, 106 instead of 108 us for 16384 rows of the same at rank 64;
+// both parts by conversion 6.7 and 113).
 __device__ __forceinline__ uint32_t tf32_hi(uint32_t x) { return (x + 0x1000u) & 0xFFFFE000u; }
 __device__ __forceinline__ uint32_t tf32_lo(uint32_t x, uint32_t hi) {
   uint32_t lo;
@@ -473,10 +478,10 @@ __device__ __forceinline__ void lora_tile(const LoraArgs& a, const int* row, int
   }
 }
 
-// CTAs an SM is to hold (registers): 16384 rows 384 -> 1536, rank 16, fp32
-// take 50 us with four, 54 with five, 72 with three; rank 64 fp32 141 with
-// four, 129 with three; 5000 rows 457 -> 763, rank 10, bf16 29 with four, 23
-// with five.
+// CTAs an SM is to hold (registers), measured with the fp32 products in one
+// chain: 16384 rows 384 -> 1536, rank 16, fp32 took 50 us with four, 54 with
+// five, 72 with three; 768 -> 1536, rank 64, fp32 141 with four, 129 with three;
+// 5000 rows 457 -> 763, rank 10, bf16 29 with four, 23 with five.
 template <typename T, bool WIDE, int STEPS>
 constexpr int lora_ctas() {
   return STEPS == 1 ? (WIDE ? 4 : 5) : STEPS == 4 && sizeof(T) == 4 ? 3 : 4;

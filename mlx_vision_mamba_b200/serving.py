@@ -15,8 +15,9 @@ where its state lies and which adapter it uses, and
 * `lora_add_cuda(base, x, adapters, batch, out=None)`
 
 run on it (`MambaBlock.serve` calls all three).  They update the state tensors
-in place and have no gradient: with grad mode on they refuse inputs that
-require one.  A call runs on the current stream of x's device, allocates only
+in place (which autograd is told of) and have no derivatives: with grad mode on
+they refuse inputs that require a gradient, and dual tensors while forward mode
+is on.  A call runs on the current stream of x's device, allocates only
 its outputs (and the scan's carries, when it splits long prompts) and never
 synchronises, so it can be captured into a CUDA graph after one eager call
 with the same batch.
@@ -398,6 +399,8 @@ def lora_add_cuda(base: torch.Tensor, x: torch.Tensor, adapters: LoraAdapters, b
     for an update in place, or a tensor that overlaps neither base nor x
     (default: a new one).  Products and sums are fp32; a bf16 result is rounded
     once.  A row of x with a NaN or an infinity comes out as NaN (or infinite)
-    where its request has an adapter, whatever the factors.
+    where its request has an adapter, whatever the factors; so does one whose
+    values, factors or inner products reach 3.39e38, the last step of fp32's
+    range.  A row's result does not depend on the rows beside it.
     """
     return (_ext_module or _ext()).lora(base, x, adapters, batch, out)
