@@ -195,6 +195,13 @@ struct ScanCarries {
   int rows;             // carry rows
 };
 
+// A later piece's map: half^2 h + local, half = exp(A sum delta / 2).  With
+// A > 0 the factor may leave fp32's range where the state does not (it is tiny,
+// or still zero); in halves it does so only with the state itself.
+__device__ __forceinline__ float apply_map(float half, float h, float local) {
+  return h == 0.f ? local : fmaf(half, half * h, local);
+}
+
 template <typename T, int G, bool HAS_Z, bool CARRY>
 __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const Piece& p, int group, int bc_grain,
                                                   bool later, const ScanCarries& k, unsigned char* smem_raw) {
@@ -311,7 +318,8 @@ __device__ __forceinline__ void cached_scan_piece(const CachedScanArgs& a, const
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 g = *reinterpret_cast<const float2*>(k.h + ch * NS + 8 * hb + 2 * j);
-          h[c][j] = fma2(make_float2(exp2f(A2[c][j].x * sum), exp2f(A2[c][j].y * sum)), h[c][j], g);
+          h[c][j].x = apply_map(exp2f(0.5f * (A2[c][j].x * sum)), h[c][j].x, g.x);
+          h[c][j].y = apply_map(exp2f(0.5f * (A2[c][j].y * sum)), h[c][j].y, g.y);
         }
       }
     }
@@ -485,7 +493,7 @@ __global__ void cached_chain_kernel(const int32_t* __restrict__ chains, const fl
     for (int q = 0; q < CCH_AHEAD; ++q) {
       if (k0 + q < c.y) {
         h_start[int64_t(c.x + k0 + q) * dn * NS + i] = h;
-        h = fmaf(expf(An * s[q]), h, g[q]);
+        h = apply_map(expf(0.5f * (An * s[q])), h, g[q]);
       }
     }
   }

@@ -875,3 +875,38 @@ def test_lora_of_large_calls(rows, d_in, d_out, rank, dtype):
     wide = torch.zeros(rows, d_out + 8, device="cuda", dtype=dtype)[:, 4:4 + d_out]
     lora_add_cuda(base, x, ads, batch, out=wide)
     assert torch.equal(wide, y)
+
+
+@pytest.mark.parametrize("lengths,dn", [([1500], 40), ([400] * 5 + [1] * 12, 768)])
+def test_growing_states_over_split_prompts(lengths, dn):
+    """A > 0: a later piece's factor exp(A sum delta) leaves fp32's range while
+    the states do not (nothing has come in yet, or the state is tiny)."""
+    n = len(lengths)
+    batch = RequestBatch(lengths)
+    host, (pieces, _, _, _, most, _) = batch._build(("scan", 2 * dn))
+    assert (most > 8) == (n == 1)  # chained by a kernel, by the pieces
+    inp = _scan_inputs(batch.tokens, dn, n, gate=False, seed=dn)
+    inp["A"] = torch.full((dn, 16), 4.0, device="cuda")
+    inp["delta"].fill_(2.0)
+    x, state = inp["x"], torch.zeros_like(inp["state"])
+    end = lengths[0]
+    x[:end - 5] = 0.0
+    y = selective_scan_cached_cuda(batch=batch, **dict(inp, state=state))
+    last = {k: (v[end - 10:end] if k in ("x", "delta", "B", "C") else v) for k, v in inp.items()}
+    alone = torch.zeros_like(state[:1])
+    want = selective_scan_cached_cuda(batch=RequestBatch([10]), **dict(last, state=alone))
+    assert torch.isfinite(want).all() and torch.equal(y[end - 10:end], want) and torch.equal(state[0], alone[0])
+    assert (y[:end - 10] == 0).all()
+
+    rec = host[:8 * pieces].view(-1, 8).tolist()
+    t0, t1 = next((r[0], r[1]) for r in rec if r[2] == 0 and r[7] == 2)
+    inp["A"].fill_(1.0)
+    inp["delta"].zero_()
+    inp["delta"][t0:t1] = 100.0 / (t1 - t0)
+    x.zero_()
+    state = torch.full_like(state, 1e-30)
+    selective_scan_cached_cuda(batch=batch, **dict(inp, state=state))
+    total = inp["delta"][:end, 0].double().sum()
+    want = state.new_tensor(1e-30).double() * torch.exp(total)
+    # serving_ref's bound of a split request: its sum of L steps, then the rest of the exponent and its exponentials
+    assert ((state[0].double() - want) / want).abs().max() <= (10 + (3 + end) * 100) * ref.EPS
